@@ -98,7 +98,9 @@ enum {
   TCRV_HIP_ELEM_U32 = 5,
   TCRV_HIP_ELEM_I64 = 6,
   TCRV_HIP_ELEM_F32 = 7,
-  TCRV_HIP_ELEM_F64 = 8
+  TCRV_HIP_ELEM_F64 = 8,
+  TCRV_HIP_ELEM_F16 = 9,  /* the cache entries at the end of this file; not tcrv_hip_binary */
+  TCRV_HIP_ELEM_BF16 = 10
 };
 TCRV_HIP_API int tcrv_hip_binary(int kind, int elem, const void *lhs, const void *rhs, void *out,
                     size_t n, void *stream);
@@ -378,6 +380,156 @@ TCRV_HIP_API int tcrv_hip_pack_q4_0_to_soa(size_t nrows, size_t nb, const uint8_
  * n/32 even; vx 16-byte aligned (as the pack writes it), vy 4-byte aligned. */
 TCRV_HIP_API int tcrv_hip_gemv_q4_0_soa_q8_0(size_t n, float *s, const uint8_t *vx,
                                 const uint8_t *vy, size_t nr, void *stream);
+
+/* ---- attention over a paged Q4_0 cache (no reference counterpart) ---------
+ * The operators between the query/key/value projections and the output
+ * projection of a step that serves several requests: tcrv_hip_kv_tables lays
+ * out the step's tokens, tcrv_hip_rope turns the queries, tcrv_hip_kv_store_q4_0
+ * turns the keys and stores keys and values, tcrv_hip_attn_q4_0 attends.
+ *
+ * Activations are f32, f16 or bf16 (`elem`: TCRV_HIP_ELEM_F32, _F16, _BF16) as
+ * [token][head][head_dim] with the last dimension dense and the strides of a
+ * token and of a head given in elements (the columns of one fused projection
+ * serve as they are); pointers need the element's alignment.  Sums, softmax
+ * statistics and rotations are computed in f32 for every `elem`.
+ *
+ * The cache of one layer is `pages` pages of page_size tokens (a multiple of
+ * 16) for `kv_heads` heads of head_dim 64, 128, 192 or 256; a page is
+ * tcrv_hip_kv_q4_0_page_bytes(page_size, kv_heads, head_dim) bytes and the cache
+ * 16-byte aligned.  Rows are ggml Q4_0 blocks (nb = head_dim / 32 a row, block b
+ * of fp16 d_b and 16 bytes q_b: element j low nibble of q_b[j], element j + 16
+ * high), their bytes arranged so that a wave's loads are whole lines and its
+ * matrix operands need no exchange between lanes.  Per page and head, in order:
+ *   keys' quants    [token][g < 4][b < nb][i < 4]                  q_b[4 g + i]
+ *   keys' scales    [token / 4][b < nb][token % 4]                 d_b
+ *   values' quants  [token / 4][m < 16][b / 2][token % 4][b % 2]   q_b[m]
+ *   values' scales  [token / 4][b < nb][token % 4]                 d_b
+ * A slot is page * page_size + the token's place in the page. */
+
+/* Bytes of a page, 0 for sizes that the cache does not have. */
+TCRV_HIP_API size_t tcrv_hip_kv_q4_0_page_bytes(size_t page_size, size_t kv_heads,
+                                                size_t head_dim);
+
+/* The cosines and sines that tcrv_hip_rope reads: for positions
+ * first .. first + count - 1 a row of n_dims / 2 pairs (cos, sin), float, times
+ * the amplitude; angles in double.  With f_i = base^(-2 i / n_dims), divided by
+ * divisors[i] where `divisors` (device, n_dims / 2 floats) is not NULL:
+ *   NONE    angle = p f_i
+ *   LINEAR  angle = p f_i / factor
+ *   NTK     base * factor^(n_dims / (n_dims - 2)) in the place of base
+ *   YARN    angle = p (f_i (1 - r_i) + f_i / factor r_i), where r_i goes from 0 to
+ *           1 between the i that turn beta_fast and beta_slow times over
+ *           trained_context tokens (rounded outwards, within 0 .. n_dims - 1)
+ * amplitude > 0 scales cosines and sines; 0 takes the form's own: 1, and
+ * 0.1 ln(factor) + 1 for YARN.  Arguments that a form does not name are ignored.
+ * n_dims even; base, factor, trained_context, beta_* positive and finite,
+ * beta_fast >= beta_slow, YARN with base > 1, NTK with n_dims > 2: else
+ * TCRV_HIP_ERR_BAD_SIZE.  A table is made once, or as contexts grow. */
+enum {
+  TCRV_HIP_ROPE_SCALE_NONE = 0,
+  TCRV_HIP_ROPE_SCALE_LINEAR = 1,
+  TCRV_HIP_ROPE_SCALE_NTK = 2,
+  TCRV_HIP_ROPE_SCALE_YARN = 3
+};
+TCRV_HIP_API int tcrv_hip_rope_table(int scaling, size_t n_dims, double base, double factor,
+                                     double trained_context, double beta_fast,
+                                     double beta_slow, double amplitude, const float *divisors,
+                                     size_t first, size_t count, float *table, void *stream);
+
+/* Rotary positions: the first n_dims elements (even, <= head_dim) of every head
+ * as n_dims / 2 pairs (a, b), elements (2 i, 2 i + 1) for INTERLEAVED and
+ * (i, i + n_dims / 2) for HALF:
+ *   y = (fl(a c) - fl(b s), fl(a s) + fl(b c)),  c, s = table[position][i]
+ * in f32, rounded once to `elem`; the other elements are copied.  `inverse`
+ * takes -s: the gradient of the turn, and its undoing where the amplitude is 1.
+ * A token whose position is outside 0 .. table_rows - 1 is copied unturned.
+ * y may be x (same strides), else must not overlap it. */
+enum { TCRV_HIP_ROPE_INTERLEAVED = 0, TCRV_HIP_ROPE_HALF = 1 };
+TCRV_HIP_API int tcrv_hip_rope(int elem, int layout, const void *x, size_t x_token,
+                               size_t x_head, void *y, size_t y_token, size_t y_head,
+                               const int32_t *positions, const float *table, size_t table_rows,
+                               size_t tokens, size_t heads, size_t head_dim, size_t n_dims,
+                               int inverse, void *stream);
+
+/* What a step's tokens need, from request lengths on the device.  Request r has
+ * context[r] tokens cached in the pages block_table[r * table_stride + ..] and
+ * gets added[r] more (negative counts as 0).  Written:
+ *   block_table  the pages of the new tokens, taken from free_pages in the
+ *                requests' order (entry i of the requests' new pages is
+ *                free_pages[i]); what is there already stays.  -1 where
+ *                free_pages (free_count entries) has run out
+ *   first        requests + 1: the requests' tokens start at first[r]; all of
+ *                them at the end
+ *   length       context[r] + added[r]
+ *   positions    max_tokens: of each token in its request; -1 past the last
+ *   slots        max_tokens: of each token; -1 past the last, where its page is
+ *                missing, and past table_stride pages (no page is taken there)
+ *   taken        one value: the new pages that the requests need.  Over
+ *                free_count: some are missing
+ * Sums are 64-bit; what does not fit an int32 output is written as INT32_MAX.
+ * Repeating a call with the same inputs gives the same outputs. */
+TCRV_HIP_API int tcrv_hip_kv_tables(const int32_t *context, const int32_t *added,
+                                    size_t requests, size_t page_size,
+                                    const int32_t *free_pages, size_t free_count,
+                                    int32_t *block_table, size_t table_stride, int32_t *first,
+                                    int32_t *length, int32_t *positions, int64_t *slots,
+                                    size_t max_tokens, int32_t *taken, void *stream);
+
+/* Keys and values into their slots.  Keys are turned first as tcrv_hip_rope turns
+ * them (in f32, not rounded to `elem` in between) where n_dims > 0; n_dims = 0
+ * stores them as they are and looks at neither layout, positions nor table.
+ * Blocks are quantized as ggml's quantize_row_q4_0_ref does: d = x / -8 of the
+ * element of largest magnitude (the first of several), q = min(15, trunc(x fl(1/d)
+ * + 8.5)), d stored as fp16 (nearest even).  A NaN in a block makes its d NaN.
+ * Tokens whose slot is negative or past the cache are skipped; no two tokens may
+ * have the same slot. */
+TCRV_HIP_API int tcrv_hip_kv_store_q4_0(int elem, const void *k, size_t k_token, size_t k_head,
+                                        const void *v, size_t v_token, size_t v_head,
+                                        int layout, const int32_t *positions,
+                                        const float *table, size_t table_rows, size_t n_dims,
+                                        const int64_t *slots, uint8_t *cache, size_t pages,
+                                        size_t page_size, size_t tokens, size_t kv_heads,
+                                        size_t head_dim, void *stream);
+
+/* The values that the cache holds for the tokens at `slots`, (q - 8) d, in `elem`
+ * (exact in f32); zeros for a slot that is negative or past the cache. */
+TCRV_HIP_API int tcrv_hip_kv_load_q4_0(int elem, const uint8_t *cache, size_t pages,
+                                       size_t page_size, const int64_t *slots, void *k,
+                                       size_t k_token, size_t k_head, void *v, size_t v_token,
+                                       size_t v_head, size_t tokens, size_t kv_heads,
+                                       size_t head_dim, void *stream);
+
+/* Attention of the requests' newest tokens over their cached tokens (these
+ * included: store them first).  Request r's rows are tokens first[r] ..
+ * first[r + 1] - 1 of q, at the last positions of its length[r] tokens; head h
+ * reads kv head h / (heads / kv_heads).  Row at position p sees token t when
+ * t < length[r], t <= p if `causal`, and t > p - window if window > 0:
+ *   z_t = scale sum_b d_tb sum_i q_i (n_ti - 8),  out = sum_t softmax(z)_t v_t
+ * A row that sees no token is zero.  What the cache holds in places that a row
+ * does not see (tokens past the length, infinities and NaN among them) does not
+ * reach it; a page outside 0 .. pages - 1 holds no token.  Rows that hold a NaN
+ * or infinity are NaN.  f32 rows: queries and weights enter the matrix cores as
+ * two f16 parts each (22 bits); f16 and bf16 rows: queries exactly, weights as
+ * f16.  out's rows past first[requests] are not written; out must not overlap q.
+ * max_added and max_length are the caller's bounds on added tokens and lengths
+ * (they size the launch): further rows are not written, further tokens not read.
+ * The workspace (device, 16-byte aligned, at least ..._workspace_bytes of the same
+ * arguments) joins the parts of long contexts; 0 bytes where none is needed, when
+ * `workspace` may be NULL.  What it holds after a call is unspecified; calls that
+ * share one must be ordered (one stream). */
+TCRV_HIP_API size_t tcrv_hip_attn_q4_0_workspace_bytes(int elem, size_t requests, size_t tokens,
+                                                       size_t max_added, size_t max_length,
+                                                       size_t heads, size_t kv_heads,
+                                                       size_t head_dim);
+TCRV_HIP_API int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
+                                    const uint8_t *cache, size_t pages, size_t page_size,
+                                    const int32_t *block_table, size_t table_stride,
+                                    const int32_t *first, const int32_t *length,
+                                    size_t requests, size_t tokens, size_t max_added,
+                                    size_t max_length, size_t heads, size_t kv_heads,
+                                    size_t head_dim, float scale, int causal, size_t window,
+                                    void *out, size_t out_token, size_t out_head,
+                                    void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -32,6 +32,11 @@ ERR_TOO_LARGE = -4
 ERR_UNSUPPORTED = -5
 ERR_SCRATCH_LIMIT = -6
 
+# element types of the cache entries (TCRV_HIP_ELEM_*)
+FLOAT_ELEM = {"f32": 7, "f16": 9, "bf16": 10}
+ROPE_LAYOUT = {"interleaved": 0, "half": 1}
+ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
 BINARY_ADD, BINARY_SUB, BINARY_MUL = 0, 1, 2
 ELEM = {"i8": 0, "u8": 1, "i16": 2, "u16": 3, "i32": 4, "u32": 5, "i64": 6, "f32": 7, "f64": 8}
 
@@ -48,6 +53,8 @@ _sz = ctypes.c_size_t
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _int = ctypes.c_int
+_f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 # name -> argtypes (all return int status, except the string getters)
 SIGNATURES = {
@@ -85,12 +92,24 @@ SIGNATURES = {
     "tcrv_hip_pack_q4_0_to_gemm_tiles": [_sz, _sz, _p, _sz, _p, _p],
     "tcrv_hip_q4_0_q8_0_gemm_tiles": [_sz, _p, _p, _p, _sz, _sz, _sz, _p],
     "tcrv_hip_q4_0_q8_0_gemm_ws": [_sz, _p, _p, _p, _sz, _sz, _sz, _sz, _sz, _p, _sz, _p],
+    "tcrv_hip_rope_table": [_int, _sz, _f64, _f64, _f64, _f64, _f64, _f64, _p, _sz, _sz, _p, _p],
+    "tcrv_hip_rope": [_int, _int, _p, _sz, _sz, _p, _sz, _sz, _p, _p, _sz, _sz, _sz, _sz, _sz,
+                      _int, _p],
+    "tcrv_hip_kv_tables": [_p, _p, _sz, _sz, _p, _sz, _p, _sz, _p, _p, _p, _p, _sz, _p, _p],
+    "tcrv_hip_kv_store_q4_0": [_int, _p, _sz, _sz, _p, _sz, _sz, _int, _p, _p, _sz, _sz, _p, _p,
+                               _sz, _sz, _sz, _sz, _sz, _p],
+    "tcrv_hip_kv_load_q4_0": [_int, _p, _sz, _sz, _p, _p, _sz, _sz, _p, _sz, _sz, _sz, _sz, _sz,
+                              _p],
+    "tcrv_hip_attn_q4_0": [_int, _p, _sz, _sz, _p, _sz, _sz, _p, _sz, _p, _p, _sz, _sz, _sz, _sz,
+                           _sz, _sz, _sz, _f32, _int, _sz, _p, _sz, _sz, _p, _sz, _p],
 }
 # size queries (return size_t)
 SIZE_FUNCS = {"tcrv_hip_gemm_tiles_bytes": [_sz, _sz],
               "tcrv_hip_q8_0_q8_0_gemm_workspace_bytes": [_sz, _sz, _sz],
               "tcrv_hip_q4_0_q8_0_gemm_workspace_bytes": [_sz, _sz, _sz],
-              "tcrv_hip_q8_0_q8_0_gemm_noalloc_max_bytes": []}
+              "tcrv_hip_q8_0_q8_0_gemm_noalloc_max_bytes": [],
+              "tcrv_hip_kv_q4_0_page_bytes": [_sz, _sz, _sz],
+              "tcrv_hip_attn_q4_0_workspace_bytes": [_int, _sz, _sz, _sz, _sz, _sz, _sz, _sz]}
 STRING_FUNCS = {"tcrv_hip_status_string": [_int], "tcrv_hip_version": []}
 
 _lib: Optional[ctypes.CDLL] = None
@@ -395,6 +414,71 @@ def q4_0_q8_0_gemm_ws(n: int, s, vx, vy, by: int, nr: int, nc: int, bx: int, bs:
                       ws_bytes: int, stream=None):
     return call("tcrv_hip_q4_0_q8_0_gemm_ws", n, s, vx, vy, by, nr, nc, bx, bs, ws, ws_bytes,
                 _stream(stream))
+
+
+# ---- attention over a paged Q4_0 cache (include/tcrv_hip.h has the layouts).  elem is a key of
+# FLOAT_ELEM, layout one of ROPE_LAYOUT; strides are in elements.
+
+def kv_q4_0_page_bytes(page_size: int, kv_heads: int, head_dim: int) -> int:
+    return load().tcrv_hip_kv_q4_0_page_bytes(page_size, kv_heads, head_dim)
+
+
+def rope_table(n_dims: int, table, count: int, first: int = 0, base: float = 10000.0,
+               scaling: str = "none", factor: float = 1.0, trained_context: float = 4096.0,
+               beta_fast: float = 32.0, beta_slow: float = 1.0, amplitude: float = 0.0,
+               divisors=None, stream=None):
+    return call("tcrv_hip_rope_table", ROPE_SCALING[scaling], n_dims, base, factor,
+                trained_context, beta_fast, beta_slow, amplitude, divisors, first, count, table,
+                _stream(stream))
+
+
+def rope(elem: str, layout: str, x, x_token: int, x_head: int, y, y_token: int, y_head: int,
+         positions, table, table_rows: int, tokens: int, heads: int, head_dim: int, n_dims: int,
+         inverse: bool = False, stream=None):
+    return call("tcrv_hip_rope", FLOAT_ELEM[elem], ROPE_LAYOUT[layout], x, x_token, x_head, y,
+                y_token, y_head, positions, table, table_rows, tokens, heads, head_dim, n_dims,
+                inverse, _stream(stream))
+
+
+def kv_tables(context, added, requests: int, page_size: int, free_pages, free_count: int,
+              block_table, table_stride: int, first, length, positions, slots, max_tokens: int,
+              taken, stream=None):
+    return call("tcrv_hip_kv_tables", context, added, requests, page_size, free_pages, free_count,
+                block_table, table_stride, first, length, positions, slots, max_tokens, taken,
+                _stream(stream))
+
+
+def kv_store_q4_0(elem: str, k, k_token: int, k_head: int, v, v_token: int, v_head: int,
+                  layout: str, positions, table, table_rows: int, n_dims: int, slots, cache,
+                  pages: int, page_size: int, tokens: int, kv_heads: int, head_dim: int,
+                  stream=None):
+    return call("tcrv_hip_kv_store_q4_0", FLOAT_ELEM[elem], k, k_token, k_head, v, v_token, v_head,
+                ROPE_LAYOUT[layout], positions, table, table_rows, n_dims, slots, cache, pages,
+                page_size, tokens, kv_heads, head_dim, _stream(stream))
+
+
+def kv_load_q4_0(elem: str, cache, pages: int, page_size: int, slots, k, k_token: int, k_head: int,
+                 v, v_token: int, v_head: int, tokens: int, kv_heads: int, head_dim: int,
+                 stream=None):
+    return call("tcrv_hip_kv_load_q4_0", FLOAT_ELEM[elem], cache, pages, page_size, slots, k,
+                k_token, k_head, v, v_token, v_head, tokens, kv_heads, head_dim, _stream(stream))
+
+
+def attn_q4_0_workspace_bytes(elem: str, requests: int, tokens: int, max_added: int,
+                              max_length: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    return load().tcrv_hip_attn_q4_0_workspace_bytes(FLOAT_ELEM[elem], requests, tokens, max_added,
+                                                     max_length, heads, kv_heads, head_dim)
+
+
+def attn_q4_0(elem: str, q, q_token: int, q_head: int, cache, pages: int, page_size: int,
+              block_table, table_stride: int, first, length, requests: int, tokens: int,
+              max_added: int, max_length: int, heads: int, kv_heads: int, head_dim: int,
+              scale: float, causal: bool, window: int, out, out_token: int, out_head: int, ws=None,
+              ws_bytes: int = 0, stream=None):
+    return call("tcrv_hip_attn_q4_0", FLOAT_ELEM[elem], q, q_token, q_head, cache, pages, page_size,
+                block_table, table_stride, first, length, requests, tokens, max_added, max_length,
+                heads, kv_heads, head_dim, scale, causal, window, out, out_token, out_head, ws,
+                ws_bytes, _stream(stream))
 
 
 def synchronize(stream=None):
