@@ -9,11 +9,13 @@
 // the order in which the second one reads them, and the row's maximum, sum and rescale are one
 // register each.
 //
-// A dword of 8 quants becomes four operand registers: 4 bits n over the bits of 1024.0 are 1024 + n,
-// and a packed subtraction leaves n - 8, exactly.  (Left at the bottom of a half, n is the denormal
-// n 2^-24, and four operations fewer would do; but the product aligns denormals by their exponent
-// field, and loses 3 bits.)  A block's scale multiplies what the product gives (keys) or the weight
-// (values), in f32.
+// A dword of 8 quants becomes four operand registers.  4 bits n at the bottom of a half are the f16
+// denormal n 2^-24: three shifts and four ands, and the offset -8 comes in with the keys' start value
+// and goes out with the sums of the values' weights.  The product aligns denormals by their exponent
+// field, which costs it 3 bits of 24: nothing beside 16-bit rows (one part), but f32 rows (two parts)
+// take n over the bits of 1024.0, which is 1024 + n, and subtract 1032.
+#include <algorithm>
+
 #include "kv_cache.h"
 
 namespace tcrv {
@@ -46,11 +48,13 @@ struct AttnArgs {
   const int32_t *block_table, *first, *length;
   float *parts;  // workspace: [split][token][head][head_dim], then [split][token][head][2]
   size_t q_token, q_head, out_token, out_head;
-  size_t table_stride, window;
+  size_t table_stride;
+  uint32_t table_tokens, window;  // tokens of a table's row; 0: no window
   uint32_t pages, page_size, tokens, heads, share, tiles, max_added, max_length;
   uint32_t split_tokens, splits;
   float scale;
   int causal;
+  bool q_vec, out_vec;  // groups of 4 values lie on aligned places
 };
 
 template <int n> struct Dwords {
@@ -80,15 +84,23 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// The quants in the lowest bits of a dword's halves, less 8; four dwords are an operand.
-__device__ __forceinline__ uint32_t quants_of(uint32_t w) {
-  const f16x2 v = __builtin_bit_cast(f16x2, (w & 0x000f000fu) | 0x64006400u);
-  return __builtin_bit_cast(uint32_t, v + f16x2{-1032, -1032});
-}
-__device__ __forceinline__ f16x8 operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  u32x4 v = {quants_of(a), quants_of(b), quants_of(c), quants_of(d)};
-  return __builtin_bit_cast(f16x8, v);
-}
+// Four dwords, each with a quant in the lowest bits of its halves, as an operand: n - 8 for two parts,
+// n 2^-24 for one.
+template <int NP> struct Quants {
+  uint32_t bits;  // of 1024.0, kept in a register: an instruction takes one constant
+  __device__ Quants() : bits(0x64006400u) { asm("" : "+v"(bits)); }
+  __device__ __forceinline__ uint32_t pair(uint32_t w) const {
+    if constexpr (NP == 1)
+      return w & 0x000f000fu;
+    const f16x2 v = __builtin_bit_cast(f16x2, (w & 0x000f000fu) | bits);
+    return __builtin_bit_cast(uint32_t, v + f16x2{-1032, -1032});
+  }
+  __device__ __forceinline__ f16x8 operator()(uint32_t a, uint32_t b, uint32_t c,
+                                              uint32_t d) const {
+    u32x4 v = {pair(a), pair(b), pair(c), pair(d)};
+    return __builtin_bit_cast(f16x8, v);
+  }
+};
 
 // Two values rounded to f16, and what the rounding left of them (kParts 2).  The rounded pair is
 // hidden from the compiler's sight: it would form it a second time for the remainder, from the
@@ -126,36 +138,120 @@ template <int NB> struct Tokens16 {
   Dwords<2 * NB> ks, vs;
 };
 
+// A wave's ring of steps in LDS, filled by DMA (global_load_lds: no registers, and a step's bytes once,
+// where lanes that load scales for themselves would take them sixteen times).  A stage: the keys'
+// quants of both halves, the values', then the keys' scales and the values'.
+constexpr int kStages = 3;
+template <int NB> struct Stage {
+  static constexpr int kQuants = NB * 256, kScales = NB * 32;  // of a half: 16 tokens
+  static constexpr int kBytes = 4 * (kQuants + kScales);
+  static constexpr int kLoads = (kBytes + 1023) / 1024;  // DMA instructions of 64 x 16 bytes
+};
+
+using lds_byte = __attribute__((address_space(3))) uint8_t;
+
+// 16 bytes a lane from `from` into LDS at `to` + 16 lane, out of the compiler's sight, which would
+// otherwise wait for all of them before any read of LDS.  M0 holds the place and is given back.
+__device__ __forceinline__ void dma16(const uint8_t *from, uint32_t to) {
+  uint32_t saved;
+  asm volatile("s_mov_b32 %0, m0\n\t"
+               "s_mov_b32 m0, %1\n\t"
+               "s_nop 0\n\t"
+               "global_load_lds_dwordx4 %2, off\n\t"
+               "s_mov_b32 m0, %0"
+               : "=&s"(saved)
+               : "s"(to), "v"(from)
+               : "memory");
+}
+
+template <int n> __device__ __forceinline__ void wait_loads() {
+  static_assert(n < 64, "");
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(n) : "memory");
+}
+
+// Until only the newest `steps` steps' loads are under way.
+template <int kLoads> __device__ __forceinline__ void wait_steps(int steps) {
+  if (steps >= 2)
+    wait_loads<2 * kLoads>();
+  else if (steps == 1)
+    wait_loads<kLoads>();
+  else
+    wait_loads<0>();
+}
+static_assert(kStages <= 3, "wait_steps");
+
+// The DMA of one step into the stage at LDS address `to`: at[h] is the place of half h's first token
+// in its page's head, place[h] that token's number in the page.
 template <int NB>
-__device__ __forceinline__ void load_tokens(Tokens16<NB> &t, const uint8_t *head_at,
-                                            const PageHead &lay, uint32_t place, int m, int g) {
-  const uint32_t group = (place >> 2) + g;
-  t.k = load_dwords<NB>(head_at + lay.key(NB, place + m, g, 0));
-  t.ks = load_dwords<2 * NB>(head_at + lay.quants + group * NB * 8);
-  t.v = load_dwords<NB>(head_at + lay.quants + lay.scales + (group * 16 + m) * NB * 4);
-  t.vs = load_dwords<2 * NB>(head_at + 2 * lay.quants + lay.scales + group * NB * 8);
+__device__ __forceinline__ void load_step(const uint8_t *const (&at)[2], const uint32_t (&place)[2],
+                                          const PageHead &lay, uint32_t to, int lane) {
+  using S = Stage<NB>;
+#pragma unroll
+  for (int i = 0; i < S::kLoads; ++i) {
+    const int o = i * 1024 + lane * 16;
+    // regions in their order: quants k0 k1 v0 v1, scales k0 k1 v0 v1
+    const bool quants = o < 4 * S::kQuants;
+    const int in_quants = o / S::kQuants, in_scales = (o - 4 * S::kQuants) / S::kScales;
+    const int region = quants ? in_quants : in_scales;
+    const int size = quants ? S::kQuants : S::kScales;
+    const uint32_t within = (quants ? o : o - 4 * S::kQuants) - region * size;
+    const bool values = region >= 2, second = region & 1;
+    const uint32_t base = (values ? lay.quants + lay.scales : 0) + (quants ? 0 : lay.quants);
+    const uint32_t p = second ? place[1] : place[0];
+    const uint8_t *from = (second ? at[1] : at[0]) + (base + within + p * (quants ? NB * 16 : NB * 2));
+    if (o < S::kBytes)
+      dma16(from, to + i * 1024);
+  }
+}
+
+template <int NB>
+__device__ __forceinline__ void read_step(Tokens16<NB> (&t)[2], const uint8_t *stage, int m, int g) {
+  using S = Stage<NB>;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    t[h].k = load_dwords<NB>(stage + h * S::kQuants + (m * 4 + g) * NB * 4);
+    t[h].v = load_dwords<NB>(stage + (2 + h) * S::kQuants + (g * 16 + m) * NB * 4);
+    t[h].ks = load_dwords<2 * NB>(stage + 4 * S::kQuants + h * S::kScales + g * NB * 8);
+    t[h].vs = load_dwords<2 * NB>(stage + 4 * S::kQuants + (2 + h) * S::kScales + g * NB * 8);
+  }
 }
 
 // What a lane holds of its row.  NP: the f16 parts that a query and a weight are split into.
 template <int NB, int NP> struct Row {
   f16x8 q[NB][NP];      // the block's elements in the order in which the keys' nibbles come
+  Quants<NP> quants;
   float unit;           // from the products' units to scores in powers of 2
   f32x4 o[2 * NB];      // 16 elements each: block o / 2, half o % 2
+  // for one part, whose quants lack the -8: the keys' products start at -8 sum q, and the values'
+  // take 8 times these sums of the weights off at the end
+  f32x4 start[NP == 1 ? NB : 1], weights[NP == 1 ? NB : 1];
   float m, base, l;     // maximum so far; shift - maximum; this lane's sum of weights
   int level;            // of the shift
 };
 
 template <int NB, int NP, typename T>
-__device__ __forceinline__ void load_row(Row<NB, NP> &row, const T *q, bool valid, int g,
+__device__ __forceinline__ void load_row(Row<NB, NP> &row, const T *q, bool valid, bool vec, int g,
                                          float scale) {
+  // pairs of nibbles (i, i + 4) of a dword: bytes 0 and 2 low, 0 and 2 high, then 1 and 3
   float x[NB][8], top = 0.0f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    float low[4], high[4];
+    load_values<4>(low, q + 32 * b + 4 * g, vec);
+    load_values<4>(high, q + 32 * b + 16 + 4 * g, vec);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x[b][4 * i] = low[i];
+      x[b][4 * i + 1] = low[i + 2];
+      x[b][4 * i + 2] = high[i];
+      x[b][4 * i + 3] = high[i + 2];
+    }
+  }
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      // pairs of nibbles (i, i + 4) of a dword: bytes 0 and 2 low, 0 and 2 high, then 1 and 3
-      constexpr int kElement[8] = {0, 2, 16, 18, 1, 3, 17, 19};
-      x[b][i] = valid ? widen(q[32 * b + 4 * g + kElement[i]]) : 0.0f;
+      x[b][i] = valid ? x[b][i] : 0.0f;
       top = fmaxf(top, fabsf(x[b][i]));
     }
   }
@@ -168,19 +264,28 @@ __device__ __forceinline__ void load_row(Row<NB, NP> &row, const T *q, bool vali
     (void)frexpf(top, &e);
   e = min(max(e - 1, -100), 100);
   const float into = ldexpf(scale < 0.0f ? -1.0f : 1.0f, -e);
-  row.unit = ldexpf(fabsf(scale) * kLog2e, e);
+  // not 0, so that a hidden token's score stays what it is
+  row.unit = fmaxf(ldexpf(fabsf(scale) * kLog2e, NP == 1 ? e + 24 : e), 0x1p-100f);
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
+    float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2)
+    for (int i = 0; i < 8; i += 2) {
       split_pair<NP>(x[b][i] * into, x[b][i + 1] * into, row.q[b], i);
+      sum += static_cast<float>(row.q[b][0][i]) + static_cast<float>(row.q[b][0][i + 1]);
+    }
+    if constexpr (NP == 1) {
+      const float c = row_sum(sum) * -0x1p-21f;
+      row.start[b] = f32x4{c, c, c, c};
+      row.weights[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
   }
 #pragma unroll
   for (int i = 0; i < 2 * NB; ++i)
     row.o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   row.m = kNone;
-  row.level = 0;
-  row.base = shift_of(0);
+  row.level = NP == 1 ? 2 : 0;
+  row.base = shift_of(row.level);
   row.l = 0.0f;
 }
 
@@ -188,13 +293,19 @@ template <int NB, int NP> __device__ __forceinline__ void rescale(Row<NB, NP> &r
 #pragma unroll
   for (int i = 0; i < 2 * NB; ++i)
     row.o[i] *= f;
+  if constexpr (NP == 1) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      row.weights[b] *= f;
+  }
   row.l *= f;
 }
 
-// 32 tokens.  kEdge: not all of them are seen by all rows of the tile; token 4 g + r of half h is
-// seen by this lane's row where bit 4 h + r of `seen` is set.
-template <int NB, int NP, bool kEdge>
-__device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], uint32_t seen) {
+// 32 tokens.  edge (the same in all lanes): not all of them are seen by all rows of the tile; token
+// 4 g + r of half h is seen by this lane's row where bit 4 h + r of `seen` is set.
+template <int NB, int NP>
+__device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], bool edge,
+                                       uint32_t seen) {
   float z[8];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -202,76 +313,92 @@ __device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], u
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const uint32_t w = t[h].k.v[b];
-      const f16x8 keys = operand(w, w >> 4, w >> 8, w >> 12);
-      f32x4 s = mfma(keys, row.q[b][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-      if constexpr (NP == 2)
+      const f16x8 keys = row.quants(w, w >> 4, w >> 8, w >> 12);
+      f32x4 s;
+      if constexpr (NP == 1) {
+        s = mfma(keys, row.q[b][0], row.start[b]);
+      } else {
+        s = mfma(keys, row.q[b][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
         s = mfma(keys, row.q[b][1], s);
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         sum[r] = fmaf(s[r], half_of(t[h].ks.v + 2 * b, r), sum[r]);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      z[4 * h + r] = kEdge && !(seen >> (4 * h + r) & 1u) ? kNone : sum[r];
+      z[4 * h + r] = sum[r];
+  }
+  if (edge) {
+    // what this lane's row does not see may hold anything, and a weight of 0 does not cover it
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      z[i] = seen >> i & 1u ? z[i] : kNone;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t keep = (seen >> (2 * i) & 1u ? 0xffffu : 0u) |
+                            (seen >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        t[i >> 1].vs.v[2 * b + (i & 1)] &= keep;
+    }
   }
   uint32_t any = 0;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int i = 0; i < 2 * NB; ++i) {
-      if constexpr (kEdge) {
-        // what this lane's row does not see may hold anything, and a weight of 0 not cover it
-        const uint32_t keep = (seen >> (4 * h + 2 * (i & 1)) & 1u ? 0xffffu : 0u) |
-                              (seen >> (4 * h + 2 * (i & 1) + 1) & 1u ? 0xffff0000u : 0u);
-        t[h].vs.v[i] &= keep;
-      }
-      any |= t[h].vs.v[i];
-    }
-  }
-  if (__any((any & bits_over(row.level)) != 0)) {
-    any |= __shfl_xor(any, 16);
-    any |= __shfl_xor(any, 32);
-    int level = row.level;
-#pragma unroll
-    for (int i = 0; i + 1 < kLevels; ++i)
-      level = max(level, any & bits_over(i) ? i + 1 : 0);
-    const float change = shift_of(level) - shift_of(row.level);
-    rescale(row, exp2_fast(change));
-    row.base += change;
-    row.level = level;
-  }
+  for (int i = 0; i < 2 * NB; ++i)
+    any |= t[0].vs.v[i] | t[1].vs.v[i];
   float top = z[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i)
     top = fmaxf(top, z[i]);
   top = row_max(top) * row.unit;
-  if (__any(top > row.m + kSlack)) {
+  if (__any(top > row.m + kSlack || (any & bits_over(row.level)) != 0)) {
+    any |= __shfl_xor(any, 16);
+    any |= __shfl_xor(any, 32);
+    int level = row.level;
+#pragma unroll
+    for (int i = NP == 1 ? 2 : 0; i + 1 < kLevels; ++i)
+      level = max(level, any & bits_over(i) ? i + 1 : 0);
     const float m = top > row.m + kSlack ? top : row.m;
-    rescale(row, m == row.m ? 1.0f : exp2_fast(row.m - m));  // by 0 from no token to the first
-    row.base = m == kNone ? row.base : shift_of(row.level) - m;
+    float f = exp2_fast(shift_of(level) - shift_of(row.level));
+    if (m != row.m)
+      f *= exp2_fast(row.m - m);  // by 0 from no token to the first
+    rescale(row, f);
+    row.level = level;
     row.m = m;
+    row.base = shift_of(level) - (m == kNone ? 0.0f : m);
   }
   float p[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     p[i] = exp2_fast(fmaf(z[i], row.unit, row.base));
-    if (kEdge && !(seen >> i & 1u))
-      p[i] = 0.0f;
     row.l += p[i];
   }
+  f16x2 ph[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    ph[i] = f16x2{static_cast<_Float16>(p[2 * i]), static_cast<_Float16>(p[2 * i + 1])};
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     f16x8 w[NP];
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       const uint32_t *d = t[i >> 2].vs.v + 2 * b;
-      split_pair<NP>(p[i] * half_of(d, i & 3), p[i + 1] * half_of(d, (i & 3) + 1), w, i);
+      if constexpr (NP == 1) {
+        const f16x2 x = ph[i / 2] * __builtin_bit_cast(f16x2, d[(i & 3) / 2]);
+        w[0][i] = x[0];
+        w[0][i + 1] = x[1];
+      } else {
+        split_pair<NP>(p[i] * half_of(d, i & 3), p[i + 1] * half_of(d, (i & 3) + 1), w, i);
+      }
     }
+    if constexpr (NP == 1)
+      row.weights[b] = mfma(f16x8{1, 1, 1, 1, 1, 1, 1, 1}, w[0], row.weights[b]);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int at = 4 * (2 * (b & 1) + half);
       const uint32_t *v0 = t[0].v.v + (b & ~1), *v1 = t[1].v.v + (b & ~1);
-      const f16x8 values = operand(v0[0] >> at, v0[1] >> at, v1[0] >> at, v1[1] >> at);
+      const f16x8 values = row.quants(v0[0] >> at, v0[1] >> at, v1[0] >> at, v1[1] >> at);
 #pragma unroll
       for (int s = 0; s < NP; ++s)
         row.o[2 * b + half] = mfma(values, w[s], row.o[2 * b + half]);
@@ -282,36 +409,34 @@ __device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], u
 // One request's rows and what they see, from its lengths; the same in every kernel here.
 struct Span {
   uint32_t first, added, rows;  // of its tokens in q; rows a kv head
-  int64_t position0, length;    // of its first new token; tokens that may be read
+  int position0, length;        // of its first new token; tokens that may be read
   __device__ Span(const AttnArgs &a, uint32_t request) {
-    const int64_t begin = max(a.first[request], 0), end = max(a.first[request + 1], 0);
-    const int64_t last = min(end, static_cast<int64_t>(a.tokens));
-    const int64_t whole = max(a.length[request], 0);
+    const int begin = max(a.first[request], 0), end = max(a.first[request + 1], 0);
+    const int whole = max(a.length[request], 0);
     first = static_cast<uint32_t>(begin);
-    position0 = whole - max(end - begin, int64_t{0});
+    position0 = whole - max(end - begin, 0);
     added = static_cast<uint32_t>(
-        min(max(last - begin, int64_t{0}), static_cast<int64_t>(a.max_added)));
+        min(max(min(end, static_cast<int>(a.tokens)) - begin, 0), static_cast<int>(a.max_added)));
     rows = added * a.share;
-    length = min(min(whole, static_cast<int64_t>(a.max_length)),
-                 static_cast<int64_t>(min(a.table_stride, size_t{0x7fffffff} / a.page_size)) *
-                     a.page_size);
+    length = min(min(whole, static_cast<int>(a.max_length)), static_cast<int>(a.table_tokens));
   }
   // tokens lo <= t < hi that the row of the i-th new token sees
-  __device__ int64_t lo(const AttnArgs &a, uint32_t i) const {
-    if (!a.window || a.window > static_cast<size_t>(0x7fffffff))
-      return 0;
-    return max(position0 + i + 1 - static_cast<int64_t>(a.window), int64_t{0});
+  __device__ int lo(const AttnArgs &a, uint32_t i) const {
+    return a.window ? max(position0 + static_cast<int>(i) + 1 - static_cast<int>(a.window), 0) : 0;
   }
-  __device__ int64_t hi(const AttnArgs &a, uint32_t i) const {
-    return max(a.causal ? min(position0 + i + 1, length) : length, int64_t{0});
+  __device__ int hi(const AttnArgs &a, uint32_t i) const {
+    return max(a.causal ? min(position0 + static_cast<int>(i) + 1, length) : length, 0);
   }
 };
 
 template <int NB, int NP, typename T>
-__global__ __launch_bounds__(kWaves * 64) void attn_q4_0_rows16(AttnArgs a) {
+__global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16(AttnArgs a) {
   constexpr int D = NB * 32;
-  __shared__ f32x4 s_o[kWaves / 2][2 * NB][64];
-  __shared__ float s_ml[kWaves / 2][2][64];
+  // the waves' rings, and where they meet at the end
+  __shared__ __align__(16) uint8_t s_ring[kWaves * kStages * Stage<NB>::kBytes];
+  static_assert(sizeof(s_ring) >= kWaves / 2 * (2 * NB * 16 + 8) * 64, "");
+  auto s_o = reinterpret_cast<f32x4(*)[2 * NB][64]>(s_ring);
+  auto s_ml = reinterpret_cast<float(*)[2][64]>(s_ring + kWaves / 2 * 2 * NB * 64 * 16);
   const uint32_t request = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
   const uint32_t kv_head = blockIdx.y, split = blockIdx.z;
   const Span span(a, request);
@@ -328,53 +453,92 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_0_rows16(AttnArgs a) {
   const uint32_t token = span.first + mine / a.share;
   const uint32_t head = kv_head * a.share + mine % a.share;
   // what the tile sees: its first row's first token to its last row's last
-  const int64_t begin = span.lo(a, i0) / kStep * kStep + static_cast<int64_t>(split) * a.split_tokens;
-  const int64_t end = min(span.hi(a, i1), begin + static_cast<int64_t>(a.split_tokens));
+  const int begin = (span.lo(a, i0) & -kStep) + static_cast<int>(split * a.split_tokens);
+  const int end = min(span.hi(a, i1), begin + static_cast<int>(a.split_tokens));
   if (split && begin >= end)
     return;
-  const int64_t all_lo = span.lo(a, i1), all_hi = span.hi(a, i0);  // what every row sees
-  const int64_t my_lo = span.lo(a, mine / a.share), my_hi = span.hi(a, mine / a.share);
+  const int all_lo = span.lo(a, i1), all_hi = min(span.hi(a, i0), end);  // what every row sees
+  const int my_lo = span.lo(a, mine / a.share), my_hi = min(span.hi(a, mine / a.share), end);
 
-  Row<NB, NP> row;
-  load_row<NB, NP, T>(row,
-                      static_cast<const T *>(a.q) + static_cast<size_t>(token) * a.q_token +
-                          static_cast<size_t>(head) * a.q_head,
-                      valid, g, a.scale);
   const PageHead lay(a.page_size, D);
   const uint32_t kv_heads = a.heads / a.share;
   const int32_t *const table = a.block_table + static_cast<size_t>(request) * a.table_stride;
+  const size_t page_bytes = static_cast<size_t>(lay.bytes()) * kv_heads;
+  const uint8_t *const head_at = a.cache + static_cast<size_t>(kv_head) * lay.bytes();
 
-  for (int64_t t0 = begin + wave * kStep; t0 < end; t0 += kWaves * kStep) {
-    Tokens16<NB> t[2];
-    bool there[2];
+  // The wave's steps: tokens t_n = begin + 32 (wave + 4 n).  Lane 2 (n % 32) + h holds the page and the
+  // place of step n's half h, for 32 steps at a time.
+  const uint32_t from = static_cast<uint32_t>(begin) + wave * kStep;
+  const uint32_t stop = static_cast<uint32_t>(max(end, begin));
+  const int steps = from < stop ? static_cast<int>((stop - from - 1) / (kWaves * kStep)) + 1 : 0;
+  uint32_t my_page = 0, my_place = 0;
+  const auto look_up = [&](int n) {
+    uint32_t t = from + (n + (lane >> 1)) * (kWaves * kStep) + (lane & 1) * 16;
+    t = t < stop ? t : from;  // past the end the first ones are read again and not seen
+    const uint32_t column = t / a.page_size;
+    my_page = static_cast<uint32_t>(table[column]);
+    my_place = t - column * a.page_size;
+  };
+  uint8_t *const ring = s_ring + wave * (kStages * Stage<NB>::kBytes);
+  const uint32_t ring_at = static_cast<uint32_t>(
+      __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>(
+          (lds_byte *)ring))));
+  uint32_t there = 0;  // bit 2 (n % 16) + h: whether step n's half h lies in a page
+  const auto load = [&](int n) {
+    if (n % 32 == 0)
+      look_up(n);
+    const uint8_t *at[2];
+    uint32_t place[2];
+    uint32_t bits = 0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      // 16 tokens lie in one page; past the end the first ones are read again and not seen
-      const int64_t t1 = t0 + 16 * h < end ? t0 + 16 * h : t0;
-      const uint32_t column = static_cast<uint32_t>(t1) / a.page_size;
-      const uint32_t page = static_cast<uint32_t>(table[column]);
-      there[h] = page < a.pages;
-      load_tokens<NB>(t[h],
-                      a.cache + (static_cast<size_t>(there[h] ? page : 0) * kv_heads + kv_head) *
-                                    lay.bytes(),
-                      lay, static_cast<uint32_t>(t1) - column * a.page_size, m, g);
+      const uint32_t page = __builtin_amdgcn_readlane(my_page, 2 * (n % 32) + h);
+      place[h] = __builtin_amdgcn_readlane(my_place, 2 * (n % 32) + h);
+      const bool in = page < a.pages;
+      at[h] = head_at + (in ? page : 0) * page_bytes;
+      bits |= in ? 1u << h : 0u;
     }
-    if (t0 >= all_lo && t0 + kStep <= min(all_hi, end) && there[0] && there[1]) {
-      attend<NB, NP, false>(row, t, 0);
-    } else {
-      uint32_t seen = 0;
+    there = (there & ~(3u << (2 * (n % 16)))) | bits << (2 * (n % 16));
+    load_step<NB>(at, place, lay, ring_at + (n % kStages) * Stage<NB>::kBytes, lane);
+  };
+  for (int n = 0; n < kStages - 1; ++n)
+    if (n < steps)
+      load(n);
+  Row<NB, NP> row;  // its loads behind those of the first steps, which take longer
+  load_row<NB, NP, T>(row,
+                      static_cast<const T *>(a.q) + static_cast<size_t>(token) * a.q_token +
+                          static_cast<size_t>(head) * a.q_head,
+                      valid, a.q_vec, g, a.scale);
+  for (int n = 0; n < steps; ++n) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage before this one is read
+    if (n + kStages - 1 < steps)
+      load(n + kStages - 1);
+    wait_steps<Stage<NB>::kLoads>(min(steps - 1 - n, kStages - 1));
+    Tokens16<NB> t[2];
+    read_step<NB>(t, ring + (n % kStages) * Stage<NB>::kBytes, m, g);
+    const int t0 = static_cast<int>(from) + n * (kWaves * kStep);
+    const uint32_t both = there >> (2 * (n % 16)) & 3u;
+    const bool edge = t0 < all_lo || t0 + kStep > all_hi || both != 3u;
+    uint32_t seen = 0;
+    if (edge) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int64_t at = t0 + 16 * (i >> 2) + 4 * g + (i & 3);
-        seen |= at >= my_lo && at < min(my_hi, end) && there[i >> 2] ? 1u << i : 0u;
+        const int at = t0 + 16 * (i >> 2) + 4 * g + (i & 3);
+        seen |= at >= my_lo && at < my_hi && (both >> (i >> 2) & 1u) ? 1u << i : 0u;
       }
-      attend<NB, NP, true>(row, t, seen);
     }
+    attend<NB, NP>(row, t, edge, seen);
   }
 
   // to plain units, then the waves' parts together: waves 2, 3 to 0, 1 and then 1 to 0
   row.l = row_sum(row.l);
+  if constexpr (NP == 1) {
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i)
+      row.o[i] = row.o[i] * 0x1p24f - 8.0f * row.weights[i / 2];
+  }
   rescale(row, exp2_fast(-shift_of(row.level)));
+  __syncthreads();
 #pragma unroll
   for (int half = kWaves / 2; half > 0; half >>= 1) {
     if (wave >= half && wave < 2 * half) {
@@ -420,13 +584,15 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_0_rows16(AttnArgs a) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       v[r] = row.o[i][r] * inverse;
-    store_values<4>(out + 16 * i + 4 * g, v, false);
+    store_values<4>(out + 16 * i + 4 * g, v, a.out_vec);
   }
 }
 
-// The parts of a row together: a work-group a row, a thread an element.
+// The parts of a row together: a work-group a row, a thread an element.  The parts' factors are formed
+// side by side first, so that the sum's loads wait for nothing.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_q4_0_join(AttnArgs a, uint32_t head_dim) {
+  __shared__ float s_f[64], s_l[64], s_top;
   const uint32_t request = blockIdx.x / a.max_added, i = blockIdx.x % a.max_added;
   const uint32_t head = blockIdx.y;
   const Span span(a, request);
@@ -437,25 +603,40 @@ __global__ __launch_bounds__(256) void attn_q4_0_join(AttnArgs a, uint32_t head_
   const uint32_t tile = (i * a.share + head % a.share) / kRows;
   const uint32_t i0 = tile * kRows / a.share;
   const uint32_t i1 = min(tile * kRows + kRows - 1, span.rows - 1) / a.share;
-  const int64_t begin = span.lo(a, i0) / kStep * kStep;
-  const int64_t tokens = span.hi(a, i1) - begin;
-  const int64_t cut = a.split_tokens;
-  const uint32_t splits =
-      static_cast<uint32_t>(min(max((tokens + cut - 1) / cut, int64_t{1}),
-                                static_cast<int64_t>(a.splits)));
+  const int tokens = max(span.hi(a, i1) - (span.lo(a, i0) & -kStep), 1);
+  const uint32_t splits = min((tokens + a.split_tokens - 1) / a.split_tokens, a.splits);
   const size_t row = static_cast<size_t>(token) * a.heads + head;
   const size_t stride = static_cast<size_t>(a.tokens) * a.heads;
-  const float *const ml = a.parts + a.splits * stride * head_dim;
-  float m = kNone;
-  for (uint32_t s = 0; s < splits; ++s)
-    m = fmaxf(m, ml[2 * (s * stride + row)]);
-  float o = 0.0f, l = 0.0f;
+  const float2 *const ml = reinterpret_cast<const float2 *>(a.parts + a.splits * stride * head_dim);
   const uint32_t e = threadIdx.x;
-  for (uint32_t s = 0; s < splits; ++s) {
-    const size_t at = s * stride + row;
-    const float ms = ml[2 * at], f = ms == m ? 1.0f : exp2_fast(ms - m);
-    l += ml[2 * at + 1] * f;
-    o += a.parts[at * head_dim + e] * f;
+  float m = kNone, o = 0.0f, l = 0.0f;
+  for (uint32_t s0 = 0; s0 < splits; s0 += 64) {  // 64 parts at a time
+    const uint32_t n = min(splits - s0, 64u);
+    float top = kNone;
+    if (e < 64) {
+      const float2 mine = e < n ? ml[(s0 + e) * stride + row] : make_float2(kNone, 0.0f);
+      top = fmaxf(mine.x, m);
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1)
+        top = fmaxf(top, __shfl_xor(top, d));
+      s_f[e] = mine.x == top ? 1.0f : exp2_fast(mine.x - top);
+      s_l[e] = mine.y;
+      if (e == 0)
+        s_top = top;
+    }
+    __syncthreads();
+    top = s_top;
+    const float f = m == top ? 1.0f : exp2_fast(m - top);
+    o *= f;
+    l *= f;
+    m = top;
+    const float *part = a.parts + (s0 * stride + row) * head_dim + e;
+#pragma unroll 8
+    for (uint32_t s = 0; s < n; ++s) {
+      o += part[s * stride * head_dim] * s_f[s];
+      l += s_l[s] * s_f[s];
+    }
+    __syncthreads();
   }
   static_cast<T *>(a.out)[static_cast<size_t>(token) * a.out_token +
                           static_cast<size_t>(head) * a.out_head + e] =
@@ -473,8 +654,9 @@ struct Plan {
   size_t tiles, splits, split_tokens, workspace;
 };
 
-// Work-groups of one tile each; the tokens of few tiles are split, so that the card is filled, into
-// parts of at least 256 tokens (two steps a wave).
+// Work-groups of one tile each, two a CU; the tokens of fewer tiles are split into parts of at least
+// 256 tokens (two steps a wave).  More parts cost more in work-groups' beginnings than they even out:
+// decode over two contexts of 131072 75 us in 512 parts, 81 in 1024, 86 in 1536.
 Plan plan_of(size_t requests, size_t tokens, size_t max_added, size_t max_length, size_t heads,
              size_t kv_heads, size_t head_dim) {
   const size_t share = heads / kv_heads;
@@ -482,7 +664,7 @@ Plan plan_of(size_t requests, size_t tokens, size_t max_added, size_t max_length
   p.tiles = (max_added * share + tcrv::kRows - 1) / tcrv::kRows;
   const size_t groups = requests * p.tiles * kv_heads;
   const size_t most = (max_length + 255) / 256;
-  size_t splits = groups >= 1024 ? 1 : (1024 + groups - 1) / groups;
+  size_t splits = groups >= 512 ? 1 : (512 + groups - 1) / groups;
   splits = splits > most ? most : splits;
   splits = splits < 1 ? 1 : splits;
   const size_t cut = ((max_length + splits - 1) / splits + 127) / 128 * 128;
@@ -529,7 +711,7 @@ bool attn_sizes_ok(size_t heads, size_t kv_heads, size_t head_dim) {
 bool attn_too_large(size_t requests, size_t tokens, size_t max_added, size_t max_length,
                     size_t heads) {
   const size_t most = 0x7fffffffu;
-  return requests > most || tokens > most || max_added > most || max_length > most - 4096 ||
+  return requests > most || tokens > most || max_added > most || max_length > (size_t{1} << 30) ||
          max_added * heads > most || requests * max_added > most ||
          requests * max_added * heads > (size_t{1} << 40);
 }
@@ -598,7 +780,9 @@ int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
              out_token,
              out_head,
              table_stride,
-             window,
+             static_cast<uint32_t>(std::min(table_stride, size_t{0x7fffffff} / page_size) *
+                                   page_size),
+             window < 0x7fffffffu ? static_cast<uint32_t>(window) : 0,
              static_cast<uint32_t>(pages),
              static_cast<uint32_t>(page_size),
              static_cast<uint32_t>(tokens),
@@ -610,7 +794,9 @@ int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
              static_cast<uint32_t>(p.split_tokens),
              static_cast<uint32_t>(p.splits),
              scale,
-             causal};
+             causal,
+             groups_of_4(q, q_token, q_head, size),
+             groups_of_4(out, out_token, out_head, size)};
   const dim3 grid(static_cast<unsigned>(requests * p.tiles), static_cast<unsigned>(kv_heads),
                   static_cast<unsigned>(p.splits));
   hipStream_t st = as_stream(stream);

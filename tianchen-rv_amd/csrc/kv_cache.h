@@ -130,6 +130,11 @@ inline bool cache_sizes_ok(size_t page_size, size_t kv_heads, size_t head_dim) {
          (head_dim == 64 || head_dim == 128 || head_dim == 192 || head_dim == 256);
 }
 
+// Whether groups of 4 values of every row lie on aligned places.
+inline bool groups_of_4(const void *p, size_t token, size_t head, size_t size) {
+  return aligned_to(p, 4 * size) && token % 4 == 0 && head % 4 == 0;
+}
+
 // Rows of `heads` heads: a head lies beside the next, and a token's heads before the next
 // token's or interleaved with them; only what would make two rows overlap in part is refused.
 inline bool strides_ok(size_t token, size_t head, size_t tokens, size_t heads, size_t dim) {

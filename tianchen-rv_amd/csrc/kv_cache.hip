@@ -338,11 +338,6 @@ __global__ __launch_bounds__(kStoreThreads) void kv_load_q4_0(LoadArgs a) {
 
 namespace {
 
-// Groups of 4 values at the aligned places of every row.
-bool groups_of_4(const void *p, size_t token, size_t head, size_t size) {
-  return tcrv_host::aligned_to(p, 4 * size) && token % 4 == 0 && head % 4 == 0;
-}
-
 // Work-groups of 16 items a token: enough for few tokens, else one that walks all of them.
 unsigned item_groups(size_t tokens, size_t items) {
   const size_t all = (items + 15) / 16, wanted = (2048 + tokens - 1) / tokens;
