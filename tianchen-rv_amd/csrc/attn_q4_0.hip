@@ -51,6 +51,7 @@ struct AttnArgs {
   size_t table_stride;
   uint32_t table_tokens, window;  // tokens of a table's row; 0: no window
   uint32_t pages, page_size, tokens, heads, share, tiles, max_added, max_length;
+  uint32_t few_least, few_most;  // the kernel at hand serves requests of so many rows a kv head
   uint32_t split_tokens, splits;
   float scale;
   int causal;
@@ -109,7 +110,8 @@ template <int kParts>
 __device__ __forceinline__ void split_pair(float x0, float x1, f16x8 (&part)[kParts], int i) {
   uint32_t hi = __builtin_bit_cast(
       uint32_t, f16x2{static_cast<_Float16>(x0), static_cast<_Float16>(x1)});
-  asm("" : "+v"(hi));
+  if constexpr (kParts == 2)
+    asm("" : "+v"(hi));
   const f16x2 h = __builtin_bit_cast(f16x2, hi);
   part[0][i] = h[0];
   part[0][i + 1] = h[1];
@@ -119,14 +121,28 @@ __device__ __forceinline__ void split_pair(float x0, float x1, f16x8 (&part)[kPa
   }
 }
 
+// A lane's own value and that of lane ^ 32 (lane ^ 16), in an order that both lanes share.
+__device__ __forceinline__ float2 with_lane32(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t x = r[0], y = r[1];
+  return make_float2(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
+__device__ __forceinline__ float2 with_lane16(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t x = r[0], y = r[1];
+  return make_float2(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
+__device__ __forceinline__ float max_of(float2 v) { return fmaxf(v.x, v.y); }
+__device__ __forceinline__ float sum_of(float2 v) { return v.x + v.y; }
+
 // Over the four lanes of a row (lane, lane ^ 16, ^ 32, ^ 48).
 __device__ __forceinline__ float row_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  return max_of(with_lane32(max_of(with_lane16(v))));
 }
 __device__ __forceinline__ float row_sum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  return sum_of(with_lane32(sum_of(with_lane16(v))));
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -440,7 +456,7 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16
   const uint32_t request = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
   const uint32_t kv_head = blockIdx.y, split = blockIdx.z;
   const Span span(a, request);
-  if (tile * kRows >= span.rows)
+  if (tile * kRows >= span.rows || span.rows < a.few_least || span.rows > a.few_most)
     return;
   const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -588,59 +604,602 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16
   }
 }
 
-// The parts of a row together: a work-group a row, a thread an element.  The parts' factors are formed
-// side by side first, so that the sum's loads wait for nothing.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_q4_0_join(AttnArgs a, uint32_t head_dim) {
-  __shared__ float s_f[64], s_l[64], s_top;
-  const uint32_t request = blockIdx.x / a.max_added, i = blockIdx.x % a.max_added;
-  const uint32_t head = blockIdx.y;
+// ---------------------------------------------------------------------------
+// Many rows: prompts.  A work-group takes its waves of 32 rows each through the tokens in steps, and
+// the cache's values become f16 once for all of them: a step's quants are read 4-bit, scaled, and
+// written to LDS in the order in which the matrix operands are read back, the next step's while this
+// one is computed.  Both products are v_mfma_f32_32x32x16_f16, rows as columns as above, so that the
+// weights again leave the first one where the second one reads them.
+// A key is two f16 parts, which hold all of its 15 bits: a score's error would grow with the score.
+// f16 and bf16 rows take values and weights as one part each; for f32 rows queries, values and weights
+// are two parts as well, and a product three: the larger parts', and the mixed ones.
+// ---------------------------------------------------------------------------
+using f32x16 = float __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+constexpr float kTileShift = 10.0f;       // weights: 2^4 2^10, within f16
+constexpr uint32_t kKeyBig = 1, kValueBig = 2, kValueBad = 4;  // a step's scales
+
+template <int NB, int NP> struct TileStep {
+  // eight waves, two a SIMD, while a wave's queries and output fit 256 registers; a thread brings a
+  // piece of a step, and two steps fit the LDS
+  static constexpr int kWaves = NB == 8 || (NP == 2 && NB == 6) ? 4 : 8;
+  static constexpr int kThreads = kWaves * 64, kTokens = kWaves * 8, kRows = kWaves * 32;
+  // LDS rows: a token's keys, an element's values; 16 bytes apart from a multiple of the banks
+  static constexpr int kKeyRow = NB * 64 + 16, kValueRow = kTokens * 2 + 16;
+  static constexpr int kKeys = kTokens * kKeyRow, kValues = NB * 32 * kValueRow;  // of one part
+  static constexpr int kBytes = 2 * kKeys + NP * kValues;
+  static_assert(2 * kBytes <= 159 * 1024, "");
+};
+
+// What a thread carries from the cache to LDS: quarter g of a token's keys (the lower half of the
+// threads) or byte m of four tokens' values, with their scales.
+template <int NB> struct Raw {
+  Dwords<NB> q;
+  Dwords<2 * NB> d;  // keys: a scale a dword
+};
+
+// (n - 8) / 16 of the quants in the lowest bits of a dword's halves: over the bits of 64.0 they are
+// sixteenths.  Times a scale below fp16's largest this stays below it.
+__device__ __forceinline__ f16x2 sixteenths(uint32_t w) {
+  const f16x2 v = __builtin_bit_cast(f16x2, (w & 0x000f000fu) | 0x54005400u);
+  return v + f16x2{static_cast<_Float16>(-64.5f), static_cast<_Float16>(-64.5f)};
+}
+
+template <int NP> __device__ __forceinline__ void scaled(uint32_t w, f16x2 d, uint32_t (&part)[NP]) {
+  const f16x2 n = sixteenths(w);
+  const f16x2 hi = n * d;
+  part[0] = __builtin_bit_cast(uint32_t, hi);
+  if constexpr (NP == 2)
+    part[1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, d, -hi));
+}
+
+template <int NB, int NP, typename T>
+__global__ __launch_bounds__((TileStep<NB, NP>::kThreads), (TileStep<NB, NP>::kWaves / 4)) void
+attn_q4_0_tiles(AttnArgs a) {
+  using S = TileStep<NB, NP>;
+  constexpr int D = NB * 32, kTokens = S::kTokens;
+  __shared__ __align__(16) uint8_t s_step[2][S::kBytes];
+  __shared__ uint32_t s_flags[2][S::kWaves];
+  __shared__ uint32_t s_bad[2][NB][kTokens / 32];
+  // the last tiles of a prompt see the most tokens: they go first
+  const uint32_t kv_heads = a.heads / a.share, kv_head = blockIdx.x % kv_heads;
+  const uint32_t tile = a.tiles - 1 - blockIdx.y, split = blockIdx.z;
+  const uint32_t request = blockIdx.x / kv_heads;
   const Span span(a, request);
-  if (i >= span.added)
+  if (tile * S::kRows >= span.rows || span.rows < a.few_least || span.rows > a.few_most)
     return;
-  const uint32_t token = span.first + i;
-  // the tile's own range, as the kernel above cut it
-  const uint32_t tile = (i * a.share + head % a.share) / kRows;
-  const uint32_t i0 = tile * kRows / a.share;
-  const uint32_t i1 = min(tile * kRows + kRows - 1, span.rows - 1) / a.share;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t last = span.rows - 1;
+  const uint32_t i0 = tile * S::kRows / a.share;
+  const uint32_t i1 = min(tile * S::kRows + S::kRows - 1, last) / a.share;
+  const int begin = (span.lo(a, i0) & -kStep) + static_cast<int>(split * a.split_tokens);
+  const int end = min(span.hi(a, i1), begin + static_cast<int>(a.split_tokens));
+  if (split && begin >= end)
+    return;
+  const int steps = begin < end ? (end - begin + kTokens - 1) / kTokens : 0;
+
+  // the wave's rows, and what they see
+  const uint32_t row0 = tile * S::kRows + wave * 32;
+  const uint32_t w0 = min(row0, last) / a.share, w1 = min(row0 + 31, last) / a.share;
+  const int wave_lo = span.lo(a, w0), wave_hi = row0 <= last ? min(span.hi(a, w1), end) : 0;
+  const int all_lo = span.lo(a, w1), all_hi = min(span.hi(a, w0), end);
+  const uint32_t r = min(row0 + col, last);
+  const bool valid = row0 + col <= last;
+  const int lo = span.lo(a, r / a.share), hi = min(span.hi(a, r / a.share), end);
+  const uint32_t token = span.first + r / a.share, head = kv_head * a.share + r % a.share;
+
+  // the thread's piece of a step
+  const bool keys_piece = wave < S::kWaves / 2;
+  const int piece = tid & (S::kThreads / 2 - 1);
+  const int key_token = piece >> 2, g = piece & 3, value_group = piece >> 4, m = piece & 15;
+  const int piece_token = keys_piece ? key_token : 4 * value_group;
+  const PageHead lay(a.page_size, D);
+  const int32_t *const table = a.block_table + static_cast<size_t>(request) * a.table_stride;
+  const size_t page_bytes = static_cast<size_t>(lay.bytes()) * kv_heads;
+  const uint8_t *const head_at = a.cache + static_cast<size_t>(kv_head) * lay.bytes();
+  struct Place {
+    uint32_t page, token;  // of the piece's first token
+  };
+  const auto find = [&](int n) {
+    int t = begin + n * kTokens + piece_token;
+    t = t < span.length ? t : begin;  // past the end something is read, and not used
+    const uint32_t column = static_cast<uint32_t>(t) / a.page_size;
+    return Place{static_cast<uint32_t>(table[column]),
+                 static_cast<uint32_t>(t) - column * a.page_size};
+  };
+  Raw<NB> raw;
+  const auto bring = [&](int n, const Place &p) {
+    const bool in = p.page < a.pages;
+    const uint8_t *at = head_at + (in ? p.page : 0) * page_bytes;
+    if (keys_piece) {
+      raw.q = load_dwords<NB>(at + lay.key(NB, p.token, g, 0));
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        raw.d.v[b] = *reinterpret_cast<const uint16_t *>(at + lay.key_scale(NB, p.token, b));
+    } else {
+      raw.q = load_dwords<NB>(at + lay.value(NB, p.token, m, 0));
+      raw.d = load_dwords<2 * NB>(at + lay.value_scale(NB, p.token, 0));
+    }
+    // tokens that are not there: scales of 0
+    const int t0 = begin + n * kTokens;
+    if (t0 + kTokens > span.length || !__all(in)) {
+      const int left = in ? span.length - (t0 + piece_token) : 0;
+      if (keys_piece) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          raw.d.v[b] = left > 0 ? raw.d.v[b] : 0;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t keep =
+              (left > 2 * i ? 0xffffu : 0u) | (left > 2 * i + 1 ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            raw.d.v[2 * b + i] &= keep;
+        }
+      }
+    }
+  };
+  // what the step's scales are, a word a wave
+  const auto tell = [&](int n) {
+    uint32_t any = 0, said = 0;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      any |= raw.d.v[i];
+    if (keys_piece) {
+      said = __any(any & 0x4000u) ? kKeyBig : 0;
+    } else {
+#pragma unroll
+      for (int i = NB; i < 2 * NB; ++i)
+        any |= raw.d.v[i];
+      if (__any((any & 0x40004000u) != 0)) {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i)
+          bad |= (raw.d.v[i] & 0x7c00u) == 0x7c00u || (raw.d.v[i] >> 16 & 0x7c00u) == 0x7c00u;
+        said = kValueBig | (__any(bad) ? kValueBad : 0);
+      }
+    }
+    if (lane == 0)
+      s_flags[n & 1][wave] = said;
+  };
+  const auto told = [&](int n) {
+    uint32_t f = 0;
+#pragma unroll
+    for (int w = 0; w < S::kWaves; ++w)
+      f |= s_flags[n & 1][w];
+    return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(f)));
+  };
+  const auto lay_out = [&](int n, uint32_t flags, bool v_big) {
+    if (flags & kValueBad) {  // infinite and NaN scales: noted, and taken out of the product
+      if (tid < NB * (kTokens / 32))
+        s_bad[n & 1][tid / (kTokens / 32)][tid % (kTokens / 32)] = 0;
+      __syncthreads();
+      if (!keys_piece) {
+#pragma unroll
+        for (int i = 0; i < 4 * NB; ++i) {
+          const int token = 4 * value_group + (i & 3), s = 16 * (i & 1);
+          uint32_t &w = raw.d.v[i >> 1];
+          if ((w >> s & 0x7c00u) == 0x7c00u) {
+            atomicOr(&s_bad[n & 1][i >> 2][token >> 5], 1u << (token & 31));
+            w &= ~(0xffffu << s);
+          }
+        }
+      }
+    }
+    uint8_t *const keys = s_step[n & 1], *const values = keys + 2 * S::kKeys;
+    const _Float16 up = static_cast<_Float16>(32768.0f), one = static_cast<_Float16>(1.0f);
+    if (keys_piece) {
+      const _Float16 f = flags & kKeyBig ? one : up;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const _Float16 d = __builtin_bit_cast(_Float16, static_cast<uint16_t>(raw.d.v[b])) * f;
+        uint32_t x[4][2];
+        uint8_t *const to = keys + key_token * S::kKeyRow + (g * NB + b) * 16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          scaled<2>(raw.q.v[b] >> 4 * i, f16x2{d, d}, x[i]);
+        *reinterpret_cast<u32x4 *>(to + S::kKeys) = u32x4{x[0][1], x[1][1], x[2][1], x[3][1]};
+        *reinterpret_cast<u32x4 *>(to) = u32x4{x[0][0], x[1][0], x[2][0], x[3][0]};
+      }
+    } else {
+      const _Float16 f = v_big ? one : up;
+      // tokens in the order in which the weights lie: 4 of a lane's half, 4 of the other half's,
+      // then 4 and 4 again
+      const int at = 16 * (value_group >> 2) + 8 * (value_group & 1) + 2 * (value_group & 2);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const f16x2 d0 = __builtin_bit_cast(f16x2, raw.d.v[2 * b]) * f16x2{f, f};
+        const f16x2 d1 = __builtin_bit_cast(f16x2, raw.d.v[2 * b + 1]) * f16x2{f, f};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int shift = 4 * (2 * (b & 1) + half);
+          uint32_t x[2][NP];
+          scaled<NP>(raw.q.v[b & ~1] >> shift, d0, x[0]);
+          scaled<NP>(raw.q.v[b | 1] >> shift, d1, x[1]);
+#pragma unroll
+          for (int s = 0; s < NP; ++s)
+            *reinterpret_cast<u32x2 *>(values + s * S::kValues +
+                                       (32 * b + 16 * half + m) * S::kValueRow + at * 2) =
+                u32x2{x[0][s], x[1][s]};
+        }
+      }
+    }
+  };
+
+  Place place{};
+  if (steps > 0) {
+    bring(0, find(0));
+    place = find(1);
+  }
+
+  // The wave's rows by whole lines into LDS, where the steps will be: chunk c of a row, 8 elements,
+  // holds those of keys' dword c.  (Fetched by the lanes that need them, 16 loads of 64 places each,
+  // the rows take as long as four steps.)
+  constexpr int kRowBytes = D * sizeof(T) + 16;
+  static_assert(S::kWaves * 32 * kRowBytes <= 2 * S::kBytes, "");
+  uint8_t *const rows_at = &s_step[0][0] + wave * 32 * kRowBytes;
+  if (row0 <= last) {
+#pragma unroll 4
+    for (int i = lane; i < 32 * (D / 4); i += 64) {
+      const uint32_t at = min(row0 + i / (D / 4), last), e = 4 * (i % (D / 4));
+      const T *p = static_cast<const T *>(a.q) +
+                   static_cast<size_t>(span.first + at / a.share) * a.q_token +
+                   static_cast<size_t>(kv_head * a.share + at % a.share) * a.q_head + e;
+      Values<T, 4> x;
+      if (a.q_vec) {
+        x = *reinterpret_cast<const Values<T, 4> *>(p);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          x.v[k] = p[k];
+      }
+      *reinterpret_cast<Values<T, 4> *>(rows_at + i / (D / 4) * kRowBytes + e * sizeof(T)) = x;
+    }
+  }
+  // a wave reads only what it wrote
+  f16x8 q[2 * NB][NP];
+  float unit = 0.0f, sign = a.scale < 0.0f ? -1.0f : 1.0f, most = 0.0f;
+  const T *const from = reinterpret_cast<const T *>(rows_at + col * kRowBytes);
+#pragma unroll
+  for (int pass = 0; pass < 2; ++pass) {  // the largest first, then the parts
+    if (pass) {
+      int e = 0;
+      most = max_of(with_lane32(most));
+      if (most > 0.0f && most < __builtin_inff())
+        (void)frexpf(most, &e);
+      e = min(max(e - 1, -100), 100);
+      sign = ldexpf(sign, -e);
+      unit = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, e + 4), 0x1p-100f);
+    }
+#pragma unroll
+    for (int s = 0; s < 2 * NB; ++s) {
+      const int c = 2 * s + hh;
+      const T *at = from + 32 * (c % NB) + 4 * (c / NB);
+      float low[4], high[4];
+      load_values<4>(low, at, true);
+      load_values<4>(high, at + 16, true);
+      const float x[8] = {low[0], low[2], high[0], high[2], low[1], low[3], high[1], high[3]};
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        if (pass)
+          split_pair<NP>(valid ? x[i] * sign : 0.0f, valid ? x[i + 1] * sign : 0.0f, q[s], i);
+        else
+          most = fmaxf(most, valid ? fmaxf(fabsf(x[i]), fabsf(x[i + 1])) : 0.0f);
+      }
+    }
+  }
+  f32x16 o[NB];
+  float top = kNone, base = kTileShift, l = 0.0f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+    o[b] = f32x16{};
+
+  uint32_t flags = 0;
+  bool v_big = false;
+  if (steps > 0) {
+    tell(0);
+    __syncthreads();  // and all have their queries
+    flags = told(0);
+    v_big = flags & kValueBig;
+    lay_out(0, flags, v_big);
+    bring(1, place);
+    place = find(2);
+  }
+  bool was_big = v_big;
+  // The keys' threads bring the next step in before they compute, the values' afterwards: of the two
+  // waves of a SIMD one is at its matrix products while the other is not.
+  const auto next_step = [&](int n) {
+    lay_out(n + 1, flags, v_big);
+    bring(n + 2, place);
+    place = find(n + 3);
+  };
+  for (int n = 0; n < steps; ++n) {
+    const uint32_t mine = flags;
+    const bool mine_big = v_big;
+    if (n + 1 < steps)
+      tell(n + 1);
+    __syncthreads();  // this step is laid out, and the one before it read
+    if (n + 1 < steps) {
+      flags = told(n + 1);
+      v_big = v_big || (flags & kValueBig);
+      if (keys_piece)
+        next_step(n);
+    }
+    const uint8_t *const keys = s_step[n & 1], *const values = keys + 2 * S::kKeys;
+    if (mine_big && !was_big) {
+      was_big = true;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        o[b] *= 0x1p-15f;
+    }
+    const float u = unit * (mine & kKeyBig ? 1.0f : 0x1p-15f);
+    const int t0 = begin + n * kTokens;
+    if (t0 < wave_hi && t0 + kTokens > wave_lo) {
+      const bool edge = t0 < all_lo || t0 + kTokens > all_hi;
+      // 32 tokens' scores
+      const auto scores = [&](int sub) {
+        __builtin_amdgcn_s_setprio(1);
+        f32x16 z{};
+        const uint8_t *const key = keys + (32 * sub + col) * S::kKeyRow + hh * 16;
+#pragma unroll
+        for (int s = 0; s < 2 * NB; ++s) {
+          const f16x8 k0 = *reinterpret_cast<const f16x8 *>(key + s * 32);
+          z = mfma32(k0, q[s][0], z);
+          const f16x8 k1 = *reinterpret_cast<const f16x8 *>(key + S::kKeys + s * 32);
+          z = mfma32(k1, q[s][0], z);
+          if constexpr (NP == 2)
+            z = mfma32(k0, q[s][1], z);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        return z;
+      };
+      // hides what the row does not see, and returns by how much a new maximum scales what is there
+      const auto settle = [&](f32x16 &z, int sub) {
+        if (edge) {
+          // register i: token 8 (i / 4) + 4 hh + i % 4
+          const int lo_at = lo - t0 - 32 * sub - 4 * hh, hi_at = hi - t0 - 32 * sub - 4 * hh;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int at = 8 * (i >> 2) + (i & 3);
+            z[i] = at >= lo_at && at < hi_at ? z[i] : kNone;
+          }
+        }
+        float high = z[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i)
+          high = fmaxf(high, z[i]);
+        high = max_of(with_lane32(high)) * u;
+        float f = 1.0f;
+        if (__any(high > top + kSlack)) {
+          // by a power of two, which leaves the weights that wait for their product exact
+          const bool up = high > top + kSlack;
+          const float next = !up ? top : top == kNone ? high : top + ceilf(high - top);
+          f = next == top ? 1.0f : exp2_fast(top - next);
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            o[b] *= f;
+          l *= f;
+          top = next;
+          base = kTileShift - (next == kNone ? 0.0f : next);
+        }
+        return f;
+      };
+      const auto weigh = [&](const f32x16 &z, f16x8 (&w)[2][NP]) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float p0 = exp2_fast(fmaf(z[i], u, base)), p1 = exp2_fast(fmaf(z[i + 1], u, base));
+          l += p0 + p1;
+          split_pair<NP>(p0, p1, w[i >> 3], i & 7);
+        }
+      };
+      const auto add_values = [&](const f16x8 (&w)[2][NP], int sub) {
+        const uint8_t *const value = values + col * S::kValueRow + (32 * sub + 8 * hh) * 2;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            f16x8 v[NP];
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+              v[p] = *reinterpret_cast<const f16x8 *>(value + p * S::kValues + b * 32 * S::kValueRow +
+                                                      s * 32);
+            o[b] = mfma32(v[0], w[s][0], o[b]);
+            if constexpr (NP == 2) {
+              o[b] = mfma32(v[0], w[s][1], o[b]);
+              o[b] = mfma32(v[1], w[s][0], o[b]);
+            }
+          }
+        }
+      };
+      // The second 32 tokens' scores are formed between the first ones' exponentials, and the first
+      // ones' output between the second ones': a wave's matrix instructions run beside its others only
+      // where they alternate.
+      f32x16 z0 = scores(0);
+      (void)settle(z0, 0);
+      f16x8 w0[2][NP];
+      if constexpr (kTokens == 32) {
+        weigh(z0, w0);
+        add_values(w0, 0);
+      } else {
+        f32x16 z1 = scores(1);
+        weigh(z0, w0);
+        const float f = settle(z1, 1);
+        if (__any(f != 1.0f)) {
+          const _Float16 h = static_cast<_Float16>(f);
+#pragma unroll
+          for (int i = 0; i < 2 * NP; ++i)
+            w0[i / NP][i % NP] *= h;
+        }
+        f16x8 w1[2][NP];
+        weigh(z1, w1);
+        add_values(w0, 0);
+        add_values(w1, 1);
+      }
+      if (mine & kValueBad) {
+        // a row that sees a value scale that is not finite is NaN in that block
+#pragma unroll
+        for (int sub = 0; sub < kTokens / 32; ++sub) {
+          const int first = min(max(lo - t0 - 32 * sub, 0), 32);
+          const int stop = min(max(hi - t0 - 32 * sub, 0), 32);
+          const uint32_t sees = static_cast<uint32_t>((1ull << stop) - (1ull << min(first, stop)));
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            o[b] += s_bad[n & 1][b][sub] & sees ? __builtin_nanf("") : 0.0f;
+        }
+      }
+    }
+    if (n + 1 < steps && !keys_piece)
+      next_step(n);
+  }
+
+  if (row0 > last && a.splits > 1)
+    return;
+  const float sum = sum_of(with_lane32(l));
+  const float out_unit = exp2_fast(was_big ? 4.0f : -11.0f);
+  if (a.splits > 1) {
+    if (!valid)
+      return;
+    const size_t at = (static_cast<size_t>(split) * a.tokens + token) * a.heads + head;
+    const size_t all = static_cast<size_t>(a.splits) * a.tokens * a.heads;
+    const float f = out_unit * exp2_fast(-kTileShift);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4 *>(a.parts + at * D + 32 * b + 8 * i + 4 * hh) =
+            f32x4{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]} * f;
+    if (hh == 0) {
+      a.parts[all * D + 2 * at] = top;
+      a.parts[all * D + 2 * at + 1] = sum * exp2_fast(-kTileShift);
+    }
+    return;
+  }
+  // rows leave as they came, by whole lines through LDS
+  __syncthreads();
+  const float f = sum == 0.0f ? 0.0f : out_unit / sum;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float v[4] = {o[b][4 * i] * f, o[b][4 * i + 1] * f, o[b][4 * i + 2] * f,
+                          o[b][4 * i + 3] * f};
+      store_values<4>(reinterpret_cast<T *>(rows_at + col * kRowBytes) + 32 * b + 8 * i + 4 * hh, v,
+                      true);
+    }
+  }
+  const int rows = static_cast<int>(min(last + 1 - min(row0, last + 1), 32u));
+#pragma unroll 4
+  for (int i = lane; i < rows * (D / 4); i += 64) {
+    const uint32_t at = row0 + i / (D / 4), e = 4 * (i % (D / 4));
+    T *p = static_cast<T *>(a.out) + static_cast<size_t>(span.first + at / a.share) * a.out_token +
+           static_cast<size_t>(kv_head * a.share + at % a.share) * a.out_head + e;
+    const Values<T, 4> x = *reinterpret_cast<const Values<T, 4> *>(
+        rows_at + i / (D / 4) * kRowBytes + e * sizeof(T));
+    if (a.out_vec) {
+      *reinterpret_cast<Values<T, 4> *>(p) = x;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        p[k] = x.v[k];
+    }
+  }
+}
+
+// The parts of a row together, 4 elements a thread; one launch joins both kernels' rows, a Cut each: how
+// the kernel had cut them.  Of few parts a group of head_dim / 4 threads takes a head, and the groups of
+// a work-group heads side by side; from kManyParts on the groups share out one head's parts.
+struct Cut {
+  const float *parts;
+  uint32_t tile_rows, split_tokens, splits;
+};
+constexpr int kJoinThreads = 256, kManyParts = 8;
+
+template <typename T, bool kShared>
+__global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join(AttnArgs a, uint32_t requests,
+                                                               uint32_t head_dim, Cut few,
+                                                               Cut many) {
+  __shared__ f32x4 s_o[kJoinThreads];
+  __shared__ float2 s_ml[kJoinThreads];
+  const uint32_t token = blockIdx.x, lane = threadIdx.x & 63;
+  // the token's request: the last one that begins at or before it, found 64 ways at a time
+  uint32_t request = 0;
+  for (uint32_t n = requests; n > 1;) {
+    const uint32_t step = (n + 63) / 64, at = lane * step;
+    const bool before = at < n && a.first[request + at] <= static_cast<int>(token);
+    const uint32_t ways = __popcll(__ballot(before));
+    const uint32_t skip = ways ? (ways - 1) * step : 0;
+    request += skip;
+    n = min(step, n - skip);
+  }
+  const Span span(a, request);
+  if (token < span.first || token - span.first >= span.added)
+    return;
+  const Cut cut = span.rows <= a.few_most ? few : many;
+  if (cut.splits <= 1)
+    return;
+  const uint32_t per_head = head_dim / 4, groups = kJoinThreads / per_head;
+  const uint32_t e = 4 * (threadIdx.x % per_head), group = threadIdx.x / per_head;
+  const uint32_t head = kShared ? blockIdx.y : blockIdx.y * groups + group;
+  const bool works = head < a.heads && group < groups;
+  // the tile's own range, as the kernels above cut it
+  const uint32_t i = token - span.first;
+  const uint32_t row0 = (i * a.share + head % a.share) / cut.tile_rows * cut.tile_rows;
+  const uint32_t i0 = row0 / a.share, i1 = min(row0 + cut.tile_rows - 1, span.rows - 1) / a.share;
   const int tokens = max(span.hi(a, i1) - (span.lo(a, i0) & -kStep), 1);
-  const uint32_t splits = min((tokens + a.split_tokens - 1) / a.split_tokens, a.splits);
+  const uint32_t splits = min((tokens + cut.split_tokens - 1) / cut.split_tokens, cut.splits);
   const size_t row = static_cast<size_t>(token) * a.heads + head;
   const size_t stride = static_cast<size_t>(a.tokens) * a.heads;
-  const float2 *const ml = reinterpret_cast<const float2 *>(a.parts + a.splits * stride * head_dim);
-  const uint32_t e = threadIdx.x;
-  float m = kNone, o = 0.0f, l = 0.0f;
-  for (uint32_t s0 = 0; s0 < splits; s0 += 64) {  // 64 parts at a time
-    const uint32_t n = min(splits - s0, 64u);
-    float top = kNone;
-    if (e < 64) {
-      const float2 mine = e < n ? ml[(s0 + e) * stride + row] : make_float2(kNone, 0.0f);
-      top = fmaxf(mine.x, m);
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1)
-        top = fmaxf(top, __shfl_xor(top, d));
-      s_f[e] = mine.x == top ? 1.0f : exp2_fast(mine.x - top);
-      s_l[e] = mine.y;
-      if (e == 0)
-        s_top = top;
-    }
-    __syncthreads();
-    top = s_top;
-    const float f = m == top ? 1.0f : exp2_fast(m - top);
-    o *= f;
-    l *= f;
-    m = top;
-    const float *part = a.parts + (s0 * stride + row) * head_dim + e;
+  const float2 *const ml =
+      reinterpret_cast<const float2 *>(cut.parts + cut.splits * stride * head_dim) + row;
+  const float *const part = cut.parts + row * head_dim + e;
+  const uint32_t s0 = kShared ? group : 0, by = kShared ? groups : 1;
+  float m = kNone, l = 0.0f;
+  f32x4 o{};
+  if (works) {
 #pragma unroll 8
-    for (uint32_t s = 0; s < n; ++s) {
-      o += part[s * stride * head_dim] * s_f[s];
-      l += s_l[s] * s_f[s];
+    for (uint32_t s = s0; s < splits; s += by)
+      m = fmaxf(m, ml[s * stride].x);
+#pragma unroll 8
+    for (uint32_t s = s0; s < splits; s += by) {
+      const float2 x = ml[s * stride];
+      const float f = x.x == m ? 1.0f : exp2_fast(x.x - m);
+      l += x.y * f;
+      o += *reinterpret_cast<const f32x4 *>(part + s * stride * head_dim) * f;
     }
-    __syncthreads();
   }
-  static_cast<T *>(a.out)[static_cast<size_t>(token) * a.out_token +
-                          static_cast<size_t>(head) * a.out_head + e] =
-      narrow<T>(l == 0.0f ? 0.0f : o / l);
+  if constexpr (kShared) {
+    s_o[threadIdx.x] = o;
+    s_ml[threadIdx.x] = make_float2(m, l);
+    __syncthreads();
+    if (group != 0)
+      return;
+    float top = kNone;
+    for (uint32_t k = 0; k < groups; ++k)
+      top = fmaxf(top, s_ml[k * per_head + threadIdx.x].x);
+    o = f32x4{};
+    l = 0.0f;
+    for (uint32_t k = 0; k < groups; ++k) {
+      const float2 x = s_ml[k * per_head + threadIdx.x];
+      const float f = x.x == top ? 1.0f : exp2_fast(x.x - top);
+      l += x.y * f;
+      o += s_o[k * per_head + threadIdx.x] * f;
+    }
+  }
+  if (!works)
+    return;
+  float v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    v[k] = l == 0.0f ? 0.0f : o[k] / l;
+  store_values<4>(static_cast<T *>(a.out) + static_cast<size_t>(token) * a.out_token +
+                      static_cast<size_t>(head) * a.out_head + e,
+                  v, a.out_vec);
 }
 
 }  // namespace
@@ -650,57 +1209,154 @@ namespace {
 
 using tcrv::AttnArgs;
 
+// Requests of few rows a kv head (decode, drafted tokens) run on attn_q4_0_rows16, the others (prompts
+// and their chunks) on attn_q4_0_tiles; a call that may hold both launches both, and each leaves the
+// other's requests alone.  Few is one tile of 16; in a call of nothing longer up to four of them, where
+// the requests and kv heads alone are 64 work-groups and more (us, f16, head_dim 128, 8 kv heads, rows16
+// / tiles: 64 requests of 4096 tokens and 8 new ones, 32 rows, 100 / 205, 32 of 2048 42 / 75, 8 of 4096
+// and 16 new 42 / 56; one request of 4096 and 16 new 32 / 24; 8 of 4096 and 64 new, up to 256 rows, with
+// the limit at 64 rows 77, at 16 63).
+size_t few_rows_of(size_t requests, size_t max_rows, size_t kv_heads) {
+  return max_rows <= 64 && requests * kv_heads >= 64 ? 64 : 16;
+}
+
+// Rows of a tile of attn_q4_0_tiles.
+size_t many_rows(int elem, size_t head_dim) {
+  using tcrv::TileStep;
+  const bool two = elem == TCRV_HIP_ELEM_F32;
+  return head_dim <= 128   ? TileStep<4, 2>::kRows
+         : head_dim == 192 ? (two ? TileStep<6, 2>::kRows : TileStep<6, 1>::kRows)
+                           : TileStep<8, 1>::kRows;
+}
+
 struct Plan {
-  size_t tiles, splits, split_tokens, workspace;
+  size_t tile_rows, tiles, splits, split_tokens, workspace;
 };
 
-// Work-groups of one tile each, two a CU; the tokens of fewer tiles are split into parts of at least
-// 256 tokens (two steps a wave).  More parts cost more in work-groups' beginnings than they even out:
-// decode over two contexts of 131072 75 us in 512 parts, 81 in 1024, 86 in 1536.
-Plan plan_of(size_t requests, size_t tokens, size_t max_added, size_t max_length, size_t heads,
-             size_t kv_heads, size_t head_dim) {
+// Work-groups of one tile each, as many as the card runs at a time; the tokens of fewer tiles are
+// split into parts of at least 256 tokens.  More parts cost more in work-groups' beginnings than they
+// even out: decode over two contexts of 131072 75 us in 512 parts, 81 in 1024, 86 in 1536.
+Plan plan_of(bool few, int elem, size_t requests, size_t tokens, size_t max_added,
+             size_t max_length, size_t window, size_t heads, size_t kv_heads, size_t head_dim) {
   const size_t share = heads / kv_heads;
   Plan p;
-  p.tiles = (max_added * share + tcrv::kRows - 1) / tcrv::kRows;
+  p.tile_rows = few ? tcrv::kRows : many_rows(elem, head_dim);
+  size_t rows = max_added * share;
+  if (few)
+    rows = std::min(rows, few_rows_of(requests, rows, kv_heads));
+  p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const size_t groups = requests * p.tiles * kv_heads;
-  const size_t most = (max_length + 255) / 256;
-  size_t splits = groups >= 512 ? 1 : (512 + groups - 1) / groups;
-  splits = splits > most ? most : splits;
-  splits = splits < 1 ? 1 : splits;
-  const size_t cut = ((max_length + splits - 1) / splits + 127) / 128 * 128;
-  p.split_tokens = cut ? cut : 128;
-  // a window's first step may begin 31 tokens before it
-  p.splits = splits == 1 ? 1 : (max_length + 31 + p.split_tokens - 1) / p.split_tokens;
-  if (p.splits == 1)
-    p.split_tokens = max_length + 32;
-  p.workspace = p.splits == 1 ? 0 : p.splits * tokens * heads * (head_dim + 2) * sizeof(float);
+  const auto parts_of = [&](size_t seen) {
+    const size_t most = std::max((seen + 255) / 256, size_t{1});
+    return std::min(std::max((512 + groups - 1) / groups, size_t{1}), most);
+  };
+  // what a tile sees begins at a multiple of 32; `window` is 0 where it does not bound that
+  size_t seen = max_length + 31;
+  if (window && window < seen)
+    seen = std::min(seen, window + p.tile_rows / share + 34);
+  const size_t parts = parts_of(seen);
+  p.split_tokens = parts == 1 ? seen : ((seen + parts - 1) / parts + 127) / 128 * 128;
+  p.splits = (seen + p.split_tokens - 1) / p.split_tokens;
+  // for any window: a smaller one has no more parts
+  const size_t most = parts_of(max_length + 31);
+  p.workspace = most == 1 ? 0 : most * tokens * heads * (head_dim + 2) * sizeof(float);
   return p;
 }
 
-template <int NB, int NP, typename T> void launch(const AttnArgs &a, dim3 grid, hipStream_t st) {
-  tcrv::attn_q4_0_rows16<NB, NP, T><<<grid, dim3(tcrv::kWaves * 64), 0, st>>>(a);
+// Which of the two kernels a call launches, and the rows up to which the first serves.
+struct Kernels {
+  bool few, many;
+  size_t few_rows;
+};
+Kernels kernels_of(size_t requests, size_t tokens, size_t max_added, size_t heads, size_t kv_heads) {
+  const size_t rows = max_added * (heads / kv_heads), few = few_rows_of(requests, rows, kv_heads);
+  if (rows <= few)
+    return {true, false, few};
+  // one request, or all as long as the longest: none is short
+  return {requests > 1 && tokens < requests * max_added, true, few};
 }
 
 template <int NP, typename T>
-void launch_dim(const AttnArgs &a, size_t head_dim, dim3 grid, size_t requests, hipStream_t st) {
+void launch_rows16(const AttnArgs &a, size_t head_dim, dim3 grid, hipStream_t st) {
+  const dim3 block(tcrv::kWaves * 64);
   switch (head_dim) {
   case 64:
-    launch<2, NP, T>(a, grid, st);
+    tcrv::attn_q4_0_rows16<2, NP, T><<<grid, block, 0, st>>>(a);
     break;
   case 128:
-    launch<4, NP, T>(a, grid, st);
+    tcrv::attn_q4_0_rows16<4, NP, T><<<grid, block, 0, st>>>(a);
     break;
   case 192:
-    launch<6, NP, T>(a, grid, st);
+    tcrv::attn_q4_0_rows16<6, NP, T><<<grid, block, 0, st>>>(a);
     break;
   default:
-    launch<8, NP, T>(a, grid, st);
+    tcrv::attn_q4_0_rows16<8, NP, T><<<grid, block, 0, st>>>(a);
     break;
   }
-  if (a.splits > 1)
-    tcrv::attn_q4_0_join<T>
-        <<<dim3(static_cast<unsigned>(requests * a.max_added), a.heads),
-           dim3(static_cast<unsigned>(head_dim)), 0, st>>>(a, static_cast<uint32_t>(head_dim));
+}
+
+template <int NB, int NP, typename T>
+void launch_tiles(const AttnArgs &a, dim3 grid, hipStream_t st) {
+  tcrv::attn_q4_0_tiles<NB, NP, T><<<grid, dim3(tcrv::TileStep<NB, NP>::kThreads), 0, st>>>(a);
+}
+
+template <int NP, typename T>
+void launch_tiles(const AttnArgs &a, size_t head_dim, dim3 grid, hipStream_t st) {
+  switch (head_dim) {
+  case 64:
+    launch_tiles<2, NP, T>(a, grid, st);
+    break;
+  case 128:
+    launch_tiles<4, NP, T>(a, grid, st);
+    break;
+  case 192:
+    launch_tiles<6, NP, T>(a, grid, st);
+    break;
+  default:
+    launch_tiles<8, NP, T>(a, grid, st);
+    break;
+  }
+}
+
+template <int NP, typename T>
+void launch_all(AttnArgs a, Kernels k, const Plan &few, const Plan &many, size_t head_dim,
+                size_t requests, hipStream_t st) {
+  const unsigned kv_heads = a.heads / a.share, n = static_cast<unsigned>(requests);
+  float *const workspace = a.parts;
+  const auto set = [&](const Plan &p, float *parts) {
+    a.parts = parts;
+    a.tiles = static_cast<uint32_t>(p.tiles);
+    a.split_tokens = static_cast<uint32_t>(p.split_tokens);
+    a.splits = static_cast<uint32_t>(p.splits);
+    return tcrv::Cut{parts, static_cast<uint32_t>(p.tile_rows), a.split_tokens, a.splits};
+  };
+  tcrv::Cut cut_few{nullptr, 1, 1, 0}, cut_many{nullptr, 1, 1, 0};
+  const uint32_t few_most = !k.few ? 0 : k.many ? static_cast<uint32_t>(k.few_rows) : 0xffffffffu;
+  if (k.few) {
+    cut_few = set(few, workspace);
+    a.few_least = 0;
+    a.few_most = few_most;
+    launch_rows16<NP, T>(a, head_dim, dim3(n * a.tiles, kv_heads, a.splits), st);
+  }
+  if (k.many) {
+    cut_many = set(many, workspace + (k.few ? few.workspace / sizeof(float) : 0));
+    a.few_least = few_most ? few_most + 1 : 0;
+    a.few_most = 0xffffffffu;
+    launch_tiles<NP, T>(a, head_dim, dim3(n * kv_heads, a.tiles, a.splits), st);
+  }
+  const uint32_t parts = std::max(cut_few.splits, cut_many.splits);
+  if (parts > 1) {
+    a.few_most = few_most;
+    const uint32_t dim = static_cast<uint32_t>(head_dim), groups = tcrv::kJoinThreads / (dim / 4);
+    const dim3 block(tcrv::kJoinThreads);
+    // shared out while the rows alone are few work-groups
+    if (parts >= tcrv::kManyParts && static_cast<size_t>(a.tokens) * a.heads <= 4096)
+      tcrv::attn_q4_0_join<T, true>
+          <<<dim3(a.tokens, a.heads), block, 0, st>>>(a, n, dim, cut_few, cut_many);
+    else
+      tcrv::attn_q4_0_join<T, false><<<dim3(a.tokens, (a.heads + groups - 1) / groups), block, 0, st>>>(
+          a, n, dim, cut_few, cut_many);
+  }
 }
 
 bool attn_sizes_ok(size_t heads, size_t kv_heads, size_t head_dim) {
@@ -727,7 +1383,13 @@ size_t tcrv_hip_attn_q4_0_workspace_bytes(int elem, size_t requests, size_t toke
       attn_too_large(requests, tokens, max_added, max_length, heads) || !requests || !tokens ||
       !max_added)
     return 0;
-  return plan_of(requests, tokens, max_added, max_length, heads, kv_heads, head_dim).workspace;
+  const Kernels k = kernels_of(requests, tokens, max_added, heads, kv_heads);
+  size_t need = 0;
+  for (const bool few : {true, false})
+    if (few ? k.few : k.many)
+      need += plan_of(few, elem, requests, tokens, max_added, max_length, 0, heads, kv_heads, head_dim)
+                  .workspace;
+  return need;
 }
 
 int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
@@ -757,15 +1419,21 @@ int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
     return TCRV_HIP_ERR_TOO_LARGE;
   if (pages == 0)
     max_length = 0;  // nothing to read
-  const Plan p = plan_of(requests, tokens, max_added, max_length, heads, kv_heads, head_dim);
-  if (requests * p.tiles > 0x7fffffffu || p.splits > 65535u)
+  const Kernels k = kernels_of(requests, tokens, max_added, heads, kv_heads);
+  const Plan few = plan_of(true, elem, requests, tokens, max_added, max_length, causal ? window : 0, heads,
+                            kv_heads, head_dim);
+  const Plan many =
+      plan_of(false, elem, requests, tokens, max_added, max_length, causal ? window : 0, heads, kv_heads, head_dim);
+  if (requests * few.tiles > 0x7fffffffu || few.splits > 65535u || many.splits > 65535u ||
+      (k.many && (many.tiles > 65535u || requests * kv_heads > 0x7fffffffu)))
     return TCRV_HIP_ERR_TOO_LARGE;
-  if (p.workspace) {
+  const size_t need = (k.few ? few.workspace : 0) + (k.many ? many.workspace : 0);
+  if (need) {
     if (!workspace)
       return TCRV_HIP_ERR_NULL_POINTER;
     if (!aligned16(workspace))
       return TCRV_HIP_ERR_MISALIGNED;
-    if (workspace_bytes < p.workspace)
+    if (workspace_bytes < need)
       return TCRV_HIP_ERR_BAD_SIZE;
   }
   AttnArgs a{q,
@@ -788,27 +1456,27 @@ int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
              static_cast<uint32_t>(tokens),
              static_cast<uint32_t>(heads),
              static_cast<uint32_t>(heads / kv_heads),
-             static_cast<uint32_t>(p.tiles),
+             0,  // the plan's: launch_attn
              static_cast<uint32_t>(max_added),
              static_cast<uint32_t>(max_length),
-             static_cast<uint32_t>(p.split_tokens),
-             static_cast<uint32_t>(p.splits),
+             0,
+             0,
+             0,
+             0,
              scale,
              causal,
              groups_of_4(q, q_token, q_head, size),
              groups_of_4(out, out_token, out_head, size)};
-  const dim3 grid(static_cast<unsigned>(requests * p.tiles), static_cast<unsigned>(kv_heads),
-                  static_cast<unsigned>(p.splits));
   hipStream_t st = as_stream(stream);
   switch (elem) {
   case TCRV_HIP_ELEM_F32:
-    launch_dim<2, float>(a, head_dim, grid, requests, st);
+    launch_all<2, float>(a, k, few, many, head_dim, requests, st);
     break;
   case TCRV_HIP_ELEM_F16:
-    launch_dim<1, _Float16>(a, head_dim, grid, requests, st);
+    launch_all<1, _Float16>(a, k, few, many, head_dim, requests, st);
     break;
   default:
-    launch_dim<1, tcrv::Bf16>(a, head_dim, grid, requests, st);
+    launch_all<1, tcrv::Bf16>(a, k, few, many, head_dim, requests, st);
     break;
   }
   return launch_status();

@@ -38,47 +38,38 @@ template <> __device__ __forceinline__ Bf16 narrow<Bf16>(float x) {
   return Bf16{static_cast<uint16_t>((x != x ? (u | 0x400000u) : up) >> 16)};
 }
 
-// `n` values from p, at once where `vec` says that p is aligned to them all, to 16 bytes at most
-// (n * sizeof(T) is 8, 16 or 32 then).
+// n values as one access, of 16 bytes at a time where they are more.
+template <typename T, int n> struct alignas(n * sizeof(T) < 16 ? n * sizeof(T) : 16) Values {
+  T v[n];
+};
+
+// `n` values from p, at once where `vec` says that p is aligned to them all, to 16 bytes at most.
 template <int n, typename T>
 __device__ __forceinline__ void load_values(float *out, const T *p, bool vec) {
-  alignas(16) T v[n];
   if (vec) {
-    if constexpr (n * sizeof(T) % 16 == 0) {
+    const Values<T, n> x = *reinterpret_cast<const Values<T, n> *>(p);
 #pragma unroll
-      for (unsigned i = 0; i < n * sizeof(T) / 16; ++i)
-        reinterpret_cast<u32x4 *>(v)[i] = reinterpret_cast<const u32x4 *>(p)[i];
-    } else if constexpr (n * sizeof(T) == 8) {
-      *reinterpret_cast<u32x2 *>(v) = *reinterpret_cast<const u32x2 *>(p);
-    }
+    for (int i = 0; i < n; ++i)
+      out[i] = widen(x.v[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < n; ++i)
-      v[i] = p[i];
+      out[i] = widen(p[i]);
   }
-#pragma unroll
-  for (int i = 0; i < n; ++i)
-    out[i] = widen(v[i]);
 }
 
 template <int n, typename T>
 __device__ __forceinline__ void store_values(T *p, const float *x, bool vec) {
-  alignas(16) T v[n];
+  Values<T, n> y;
 #pragma unroll
   for (int i = 0; i < n; ++i)
-    v[i] = narrow<T>(x[i]);
+    y.v[i] = narrow<T>(x[i]);
   if (vec) {
-    if constexpr (n * sizeof(T) % 16 == 0) {
-#pragma unroll
-      for (unsigned i = 0; i < n * sizeof(T) / 16; ++i)
-        reinterpret_cast<u32x4 *>(p)[i] = reinterpret_cast<u32x4 *>(v)[i];
-    } else if constexpr (n * sizeof(T) == 8) {
-      *reinterpret_cast<u32x2 *>(p) = *reinterpret_cast<u32x2 *>(v);
-    }
+    *reinterpret_cast<Values<T, n> *>(p) = y;
   } else {
 #pragma unroll
     for (int i = 0; i < n; ++i)
-      p[i] = v[i];
+      p[i] = y.v[i];
   }
 }
 
