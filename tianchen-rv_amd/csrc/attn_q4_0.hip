@@ -21,6 +21,9 @@
 namespace tcrv {
 namespace {
 
+#ifndef OCC
+#define OCC 2
+#endif
 constexpr int kRows = 16;          // rows of a tile
 constexpr int kWaves = 4;          // waves of a work-group, which share out a tile's tokens
 constexpr int kStep = 32;          // tokens that a wave takes at a time
@@ -157,7 +160,10 @@ template <int NB> struct Tokens16 {
 // A wave's ring of steps in LDS, filled by DMA (global_load_lds: no registers, and a step's bytes once,
 // where lanes that load scales for themselves would take them sixteen times).  A stage: the keys'
 // quants of both halves, the values', then the keys' scales and the values'.
-constexpr int kStages = 3;
+#ifndef STG
+#define STG 3
+#endif
+constexpr int kStages = STG;
 template <int NB> struct Stage {
   static constexpr int kQuants = NB * 256, kScales = NB * 32;  // of a half: 16 tokens
   static constexpr int kBytes = 4 * (kQuants + kScales);
@@ -187,20 +193,23 @@ template <int n> __device__ __forceinline__ void wait_loads() {
 
 // Until only the newest `steps` steps' loads are under way.
 template <int kLoads> __device__ __forceinline__ void wait_steps(int steps) {
-  if (steps >= 2)
+  if (steps >= 3)
+    wait_loads<3 * kLoads>();
+  else if (steps == 2)
     wait_loads<2 * kLoads>();
   else if (steps == 1)
     wait_loads<kLoads>();
   else
     wait_loads<0>();
 }
-static_assert(kStages <= 3, "wait_steps");
+static_assert(kStages <= 4, "wait_steps");
 
-// The DMA of one step into the stage at LDS address `to`: at[h] is the place of half h's first token
-// in its page's head, place[h] that token's number in the page.
+// The DMA of one step into the stage at LDS address `to`: at0 and at1 are the page's head that holds
+// each half, place0 and place1 the number of its first token in the page.
 template <int NB>
-__device__ __forceinline__ void load_step(const uint8_t *const (&at)[2], const uint32_t (&place)[2],
-                                          const PageHead &lay, uint32_t to, int lane) {
+__device__ __forceinline__ void load_step(const uint8_t *at0, const uint8_t *at1, uint32_t place0,
+                                          uint32_t place1, const PageHead &lay, uint32_t to,
+                                          int lane) {
   using S = Stage<NB>;
 #pragma unroll
   for (int i = 0; i < S::kLoads; ++i) {
@@ -213,8 +222,8 @@ __device__ __forceinline__ void load_step(const uint8_t *const (&at)[2], const u
     const uint32_t within = (quants ? o : o - 4 * S::kQuants) - region * size;
     const bool values = region >= 2, second = region & 1;
     const uint32_t base = (values ? lay.quants + lay.scales : 0) + (quants ? 0 : lay.quants);
-    const uint32_t p = second ? place[1] : place[0];
-    const uint8_t *from = (second ? at[1] : at[0]) + (base + within + p * (quants ? NB * 16 : NB * 2));
+    const uint32_t p = second ? place1 : place0;
+    const uint8_t *from = (second ? at1 : at0) + (base + within + p * (quants ? NB * 16 : NB * 2));
     if (o < S::kBytes)
       dma16(from, to + i * 1024);
   }
@@ -446,13 +455,14 @@ struct Span {
 };
 
 template <int NB, int NP, typename T>
-__global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16(AttnArgs a) {
+__global__ __launch_bounds__(kWaves * 64, NB <= 4 ? OCC : 1) void attn_q4_0_rows16(AttnArgs a) {
   constexpr int D = NB * 32;
   // the waves' rings, and where they meet at the end
-  __shared__ __align__(16) uint8_t s_ring[kWaves * kStages * Stage<NB>::kBytes];
-  static_assert(sizeof(s_ring) >= kWaves / 2 * (2 * NB * 16 + 8) * 64, "");
+  constexpr int kMeet = kWaves * (2 * NB * 16 + 8) * 64;
+  constexpr int kRing = kWaves * kStages * Stage<NB>::kBytes;
+  __shared__ __align__(16) uint8_t s_ring[kRing > kMeet ? kRing : kMeet];
   auto s_o = reinterpret_cast<f32x4(*)[2 * NB][64]>(s_ring);
-  auto s_ml = reinterpret_cast<float(*)[2][64]>(s_ring + kWaves / 2 * 2 * NB * 64 * 16);
+  auto s_ml = reinterpret_cast<float2(*)[64]>(s_ring + kWaves * 2 * NB * 64 * 16);
   const uint32_t request = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
   const uint32_t kv_head = blockIdx.y, split = blockIdx.z;
   const Span span(a, request);
@@ -503,19 +513,17 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16
   const auto load = [&](int n) {
     if (n % 32 == 0)
       look_up(n);
-    const uint8_t *at[2];
-    uint32_t place[2];
-    uint32_t bits = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t page = __builtin_amdgcn_readlane(my_page, 2 * (n % 32) + h);
-      place[h] = __builtin_amdgcn_readlane(my_place, 2 * (n % 32) + h);
-      const bool in = page < a.pages;
-      at[h] = head_at + (in ? page : 0) * page_bytes;
-      bits |= in ? 1u << h : 0u;
-    }
-    there = (there & ~(3u << (2 * (n % 16)))) | bits << (2 * (n % 16));
-    load_step<NB>(at, place, lay, ring_at + (n % kStages) * Stage<NB>::kBytes, lane);
+    const int from_lane = 2 * (n % 32);
+    const uint32_t page0 = __builtin_amdgcn_readlane(my_page, from_lane);
+    const uint32_t page1 = __builtin_amdgcn_readlane(my_page, from_lane + 1);
+    const bool in0 = page0 < a.pages, in1 = page1 < a.pages;
+    there = (there & ~(3u << (2 * (n % 16)))) |
+            ((in0 ? 1u : 0u) | (in1 ? 2u : 0u)) << (2 * (n % 16));
+    load_step<NB>(head_at + (in0 ? page0 : 0) * page_bytes,
+                  head_at + (in1 ? page1 : 0) * page_bytes,
+                  __builtin_amdgcn_readlane(my_place, from_lane),
+                  __builtin_amdgcn_readlane(my_place, from_lane + 1), lay,
+                  ring_at + (n % kStages) * Stage<NB>::kBytes, lane);
   };
   for (int n = 0; n < kStages - 1; ++n)
     if (n < steps)
@@ -546,7 +554,7 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16
     attend<NB, NP>(row, t, edge, seen);
   }
 
-  // to plain units, then the waves' parts together: waves 2, 3 to 0, 1 and then 1 to 0
+  // to plain units, then the waves' parts together, a share of the elements a wave
   row.l = row_sum(row.l);
   if constexpr (NP == 1) {
 #pragma unroll
@@ -554,53 +562,47 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16
       row.o[i] = row.o[i] * 0x1p24f - 8.0f * row.weights[i / 2];
   }
   rescale(row, exp2_fast(-shift_of(row.level)));
+  __syncthreads();  // all have read their rings
+#pragma unroll
+  for (int i = 0; i < 2 * NB; ++i)
+    s_o[wave][i][lane] = row.o[i];
+  s_ml[wave][lane] = make_float2(row.m, row.l);
   __syncthreads();
-#pragma unroll
-  for (int half = kWaves / 2; half > 0; half >>= 1) {
-    if (wave >= half && wave < 2 * half) {
-#pragma unroll
-      for (int i = 0; i < 2 * NB; ++i)
-        s_o[wave - half][i][lane] = row.o[i];
-      s_ml[wave - half][0][lane] = row.m;
-      s_ml[wave - half][1][lane] = row.l;
-    }
-    __syncthreads();
-    if (wave < half) {
-      const float m1 = s_ml[wave][0][lane], top = fmaxf(row.m, m1);
-      const float f0 = row.m == top ? 1.0f : exp2_fast(row.m - top);
-      const float f1 = m1 == top ? 1.0f : exp2_fast(m1 - top);
-#pragma unroll
-      for (int i = 0; i < 2 * NB; ++i)
-        row.o[i] = row.o[i] * f0 + s_o[wave][i][lane] * f1;
-      row.l = row.l * f0 + s_ml[wave][1][lane] * f1;
-      row.m = top;
-    }
-    __syncthreads();
-  }
-  if (wave != 0 || !valid)
+  if (!valid)
     return;
-  if (a.splits > 1) {
-    const size_t at = (static_cast<size_t>(split) * a.tokens + token) * a.heads + head;
-    const size_t all = static_cast<size_t>(a.splits) * a.tokens * a.heads;
+  float top = kNone, l = 0.0f, f[kWaves];
 #pragma unroll
-    for (int i = 0; i < 2 * NB; ++i)
-      *reinterpret_cast<f32x4 *>(a.parts + at * D + 16 * i + 4 * g) = row.o[i];
-    if (g == 0) {
-      a.parts[all * D + 2 * at] = row.m;
-      a.parts[all * D + 2 * at + 1] = row.l;
-    }
-    return;
+  for (int w = 0; w < kWaves; ++w)
+    top = fmaxf(top, s_ml[w][lane].x);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float2 x = s_ml[w][lane];
+    f[w] = x.x == top ? 1.0f : exp2_fast(x.x - top);
+    l += x.y * f[w];
   }
-  const float inverse = row.l == 0.0f ? 0.0f : 1.0f / row.l;
+  const float inverse = a.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+  const size_t at = (static_cast<size_t>(split) * a.tokens + token) * a.heads + head;
   T *const out = static_cast<T *>(a.out) + static_cast<size_t>(token) * a.out_token +
                  static_cast<size_t>(head) * a.out_head;
 #pragma unroll
-  for (int i = 0; i < 2 * NB; ++i) {
+  for (int k = 0; k < 2 * NB / kWaves; ++k) {
+    const int i = wave * (2 * NB / kWaves) + k;
+    f32x4 o{};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+      o += s_o[w][i][lane] * f[w];
     float v[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      v[r] = row.o[i][r] * inverse;
-    store_values<4>(out + 16 * i + 4 * g, v, a.out_vec);
+      v[r] = o[r] * inverse;
+    if (a.splits > 1)
+      store_values<4>(a.parts + at * D + 16 * i + 4 * g, v, true);
+    else
+      store_values<4>(out + 16 * i + 4 * g, v, a.out_vec);
+  }
+  if (a.splits > 1 && g == 0 && wave == 0) {
+    const size_t all = static_cast<size_t>(a.splits) * a.tokens * a.heads;
+    *reinterpret_cast<float2 *>(a.parts + all * D + 2 * at) = make_float2(top, l);
   }
 }
 
@@ -1247,7 +1249,7 @@ Plan plan_of(bool few, int elem, size_t requests, size_t tokens, size_t max_adde
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const size_t groups = requests * p.tiles * kv_heads;
   const auto parts_of = [&](size_t seen) {
-    const size_t most = std::max((seen + 255) / 256, size_t{1});
+    const size_t most = std::max((seen + 511) / 512, size_t{1});
     return std::min(std::max((512 + groups - 1) / groups, size_t{1}), most);
   };
   // what a tile sees begins at a multiple of 32; `window` is 0 where it does not bound that
