@@ -707,7 +707,7 @@ attn_q4_0_tiles(AttnArgs a) {
   struct Place {
     uint32_t page, token;  // of the piece's first token
   };
-  const auto find = [&](int n) {
+  const auto find = [&](int n) __attribute__((always_inline)) {
     int t = begin + n * kTokens + piece_token;
     t = t < span.length ? t : begin;  // past the end something is read, and not used
     const uint32_t column = static_cast<uint32_t>(t) / a.page_size;
@@ -715,7 +715,7 @@ attn_q4_0_tiles(AttnArgs a) {
                  static_cast<uint32_t>(t) - column * a.page_size};
   };
   Raw<NB> raw;
-  const auto bring = [&](int n, const Place &p) {
+  const auto bring = [&](int n, const Place &p) __attribute__((always_inline)) {
     const bool in = p.page < a.pages;
     const uint8_t *at = head_at + (in ? p.page : 0) * page_bytes;
     if (keys_piece) {
@@ -748,7 +748,7 @@ attn_q4_0_tiles(AttnArgs a) {
     }
   };
   // what the step's scales are, a word a wave
-  const auto tell = [&](int n) {
+  const auto tell = [&](int n) __attribute__((always_inline)) {
     uint32_t any = 0, said = 0;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
@@ -770,14 +770,14 @@ attn_q4_0_tiles(AttnArgs a) {
     if (lane == 0)
       s_flags[n & 1][wave] = said;
   };
-  const auto told = [&](int n) {
+  const auto told = [&](int n) __attribute__((always_inline)) {
     uint32_t f = 0;
 #pragma unroll
     for (int w = 0; w < S::kWaves; ++w)
       f |= s_flags[n & 1][w];
     return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(f)));
   };
-  const auto lay_out = [&](int n, uint32_t flags, bool v_big) {
+  const auto lay_out = [&](int n, uint32_t flags, bool v_big) __attribute__((always_inline)) {
     if (flags & kValueBad) {  // infinite and NaN scales: noted, and taken out of the product
       if (tid < NB * (kTokens / 32))
         s_bad[n & 1][tid / (kTokens / 32)][tid % (kTokens / 32)] = 0;
@@ -916,7 +916,7 @@ attn_q4_0_tiles(AttnArgs a) {
   bool was_big = v_big;
   // The keys' threads bring the next step in before they compute, the values' afterwards: of the two
   // waves of a SIMD one is at its matrix products while the other is not.
-  const auto next_step = [&](int n) {
+  const auto next_step = [&](int n) __attribute__((always_inline)) {
     lay_out(n + 1, flags, v_big);
     bring(n + 2, place);
     place = find(n + 3);
@@ -945,7 +945,7 @@ attn_q4_0_tiles(AttnArgs a) {
     if (t0 < wave_hi && t0 + kTokens > wave_lo) {
       const bool edge = t0 < all_lo || t0 + kTokens > all_hi;
       // 32 tokens' scores
-      const auto scores = [&](int sub) {
+      const auto scores = [&](int sub) __attribute__((always_inline)) {
         __builtin_amdgcn_s_setprio(1);
         f32x16 z{};
         const uint8_t *const key = keys + (32 * sub + col) * S::kKeyRow + hh * 16;
@@ -962,7 +962,7 @@ attn_q4_0_tiles(AttnArgs a) {
         return z;
       };
       // hides what the row does not see, and returns by how much a new maximum scales what is there
-      const auto settle = [&](f32x16 &z, int sub) {
+      const auto settle = [&](f32x16 &z, int sub) __attribute__((always_inline)) {
         if (edge) {
           // register i: token 8 (i / 4) + 4 hh + i % 4
           const int lo_at = lo - t0 - 32 * sub - 4 * hh, hi_at = hi - t0 - 32 * sub - 4 * hh;
