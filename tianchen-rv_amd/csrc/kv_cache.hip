@@ -141,7 +141,7 @@ struct StoreArgs {
   size_t k_token, k_head, v_token, v_head;
   size_t table_rows, slots_in_all;
   uint32_t page_size, kv_heads, nb, n_dims;
-  bool k_vec, v_vec;
+  bool k_vec, v_vec, row_vec;  // aligned groups of 4 values, of 4 pairs
 };
 
 template <int kControl> __device__ __forceinline__ uint32_t dpp(uint32_t v) {
@@ -182,8 +182,19 @@ __device__ __forceinline__ uint32_t quantize4(const float *x, int lane8, float *
     const float t = fminf(fmaxf(x[i] * id + 8.5f, 0.0f), 15.0f);
     q |= static_cast<uint32_t>(t) << (8 * i);
   }
-  *scale = d;
+  // out of the compiler's sight: it would round the division to f16 as fma(x, -1/8, +0), which takes the
+  // scale of an empty block from -0 to +0
+  float kept = d;
+  asm("" : "+v"(kept));
+  *scale = kept;
   return q;
+}
+
+// The page of a slot that lies in the cache, by a 32-bit division where that does (the 64-bit one is long).
+// A page takes 1152 bytes or more, so that pages number less than 2^32 in any memory.
+__device__ __forceinline__ uint32_t page_of(int64_t slot, uint32_t page_size) {
+  return slot >> 32 ? static_cast<uint32_t>(static_cast<uint64_t>(slot) / page_size)
+                    : static_cast<uint32_t>(slot) / page_size;
 }
 
 // Lane i of a row of 16 takes lane i + kBy.
@@ -193,6 +204,48 @@ template <int kBy> __device__ __forceinline__ uint32_t from_lane_above(uint32_t 
 
 constexpr int kStoreThreads = 256;
 
+// 4 elements of a key, those of places e .. e + 3 of `x`, turned.
+template <typename T, bool kHalf>
+__device__ __forceinline__ void turn4(float *v, const T *x, const float *row, uint32_t e,
+                                      uint32_t n_dims, bool vec, bool row_vec) {
+  if constexpr (kHalf) {
+    const uint32_t half = n_dims / 2;
+    if (half % 4 == 0) {  // the partners are four neighbours, n_dims / 2 away
+      const bool second = e >= half;
+      const uint32_t j = second ? e - half : e;
+      float w[4], cs[8];
+      load_values<4>(w, x + (second ? j : e + half), vec);
+      load_values<8>(cs, row + 2 * j, row_vec);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = second ? w[i] * cs[2 * i + 1] + v[i] * cs[2 * i]
+                      : v[i] * cs[2 * i] - w[i] * cs[2 * i + 1];
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = e + i;
+      if (at < n_dims) {
+        const bool second = at >= half;
+        const uint32_t j = second ? at - half : at;
+        const float c = row[2 * j], s = row[2 * j + 1];
+        const float w = widen(x[second ? j : at + half]);
+        v[i] = second ? w * s + v[i] * c : v[i] * c - w * s;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      if (e + i < n_dims) {
+        const float c = row[e + i], s = row[e + i + 1];
+        const float y = v[i] * c - v[i + 1] * s;
+        v[i + 1] = v[i] * s + v[i + 1] * c;
+        v[i] = y;
+      }
+    }
+  }
+}
+
 template <typename T, bool kHalf>
 __global__ __launch_bounds__(kStoreThreads) void kv_store_q4_0(StoreArgs a) {
   const size_t token = blockIdx.x;
@@ -200,7 +253,7 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_q4_0(StoreArgs a) {
   if (slot < 0 || static_cast<size_t>(slot) >= a.slots_in_all)
     return;
   const uint32_t nb = a.nb, dim = nb * 32;
-  const size_t page = static_cast<size_t>(slot) / a.page_size;
+  const size_t page = page_of(slot, a.page_size);
   const uint32_t place = static_cast<uint32_t>(static_cast<size_t>(slot) - page * a.page_size);
   const PageHead lay(a.page_size, dim);
   uint8_t *const page_at = a.cache + page * lay.bytes() * a.kv_heads;
@@ -225,33 +278,8 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_q4_0(StoreArgs a) {
     const bool vec = values ? a.v_vec : a.k_vec;
     float v[4];
     load_values<4>(v, x + e, vec);
-    if (!values && row && e < a.n_dims) {
-      if constexpr (kHalf) {
-        // the partner n_dims / 2 away; n_dims / 2 need not be a multiple of 4
-        const uint32_t half = a.n_dims / 2;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t at = e + i;
-          if (at < a.n_dims) {
-            const bool second = at >= half;
-            const uint32_t j = second ? at - half : at;
-            const float c = row[2 * j], s = row[2 * j + 1];
-            const float w = widen(x[second ? j : at + half]);
-            v[i] = second ? w * s + v[i] * c : v[i] * c - w * s;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          if (e + i < a.n_dims) {
-            const float c = row[e + i], s = row[e + i + 1];
-            const float y = v[i] * c - v[i + 1] * s;
-            v[i + 1] = v[i] * s + v[i + 1] * c;
-            v[i] = y;
-          }
-        }
-      }
-    }
+    if (!values && row && e < a.n_dims)
+      turn4<T, kHalf>(v, x, row, e, a.n_dims, vec, a.row_vec);
     float d;
     uint32_t q = quantize4(v, lane8, &d);
     q |= from_lane_above<4>(q) << 4;  // lanes 0..3 of 8: bytes 4 lane8 .. + 3 of the block
@@ -295,7 +323,7 @@ __global__ __launch_bounds__(kStoreThreads) void kv_load_q4_0(LoadArgs a) {
   const int64_t slot = a.slots[token];
   const bool known = slot >= 0 && static_cast<size_t>(slot) < a.slots_in_all;
   const uint32_t nb = a.nb, dim = nb * 32;
-  const size_t page = known ? static_cast<size_t>(slot) / a.page_size : 0;
+  const size_t page = known ? page_of(slot, a.page_size) : 0;
   const uint32_t place =
       known ? static_cast<uint32_t>(static_cast<size_t>(slot) - page * a.page_size) : 0;
   const PageHead lay(a.page_size, dim);
@@ -416,7 +444,8 @@ int tcrv_hip_kv_store_q4_0(int elem, const void *k, size_t k_token, size_t k_hea
                     cache,   k_token, k_head,    v_token,    v_head,
                     table_rows, pages * page_size, static_cast<uint32_t>(page_size),
                     static_cast<uint32_t>(kv_heads), nb, static_cast<uint32_t>(n_dims),
-                    groups_of_4(k, k_token, k_head, size), groups_of_4(v, v_token, v_head, size)};
+                    groups_of_4(k, k_token, k_head, size), groups_of_4(v, v_token, v_head, size),
+                    aligned16(table) && n_dims % 4 == 0};
   const dim3 grid(static_cast<unsigned>(tokens), item_groups(tokens, kv_heads * nb));
   const dim3 block(tcrv::kStoreThreads);
   hipStream_t st = as_stream(stream);
