@@ -21,9 +21,6 @@
 namespace tcrv {
 namespace {
 
-#ifndef OCC
-#define OCC 2
-#endif
 constexpr int kRows = 16;          // rows of a tile
 constexpr int kWaves = 4;          // waves of a work-group, which share out a tile's tokens
 constexpr int kStep = 32;          // tokens that a wave takes at a time
@@ -49,13 +46,17 @@ struct AttnArgs {
   void *out;
   const uint8_t *cache;
   const int32_t *block_table, *first, *length;
-  float *parts;  // workspace: [split][token][head][head_dim], then [split][token][head][2]
+  // workspace: outputs of parts of rows, [part][head_dim], then their maxima and sums, [part][2]; for
+  // the kernel of many rows part [split][token][head], for that of few [work-group][2][row of a tile]
+  float *parts;
+  uint4 *plan;  // workspace, for the kernel of few rows: a work-group's tile that others end
   size_t q_token, q_head, out_token, out_head;
   size_t table_stride;
   uint32_t table_tokens, window;  // tokens of a table's row; 0: no window
   uint32_t pages, page_size, tokens, heads, share, tiles, max_added, max_length;
   uint32_t few_least, few_most;  // the kernel at hand serves requests of so many rows a kv head
   uint32_t split_tokens, splits;
+  uint32_t requests, groups, unit_shift;  // few rows: work-groups that share out the work, 0: one a tile
   float scale;
   int causal;
   bool q_vec, out_vec;  // groups of 4 values lie on aligned places
@@ -160,10 +161,7 @@ template <int NB> struct Tokens16 {
 // A wave's ring of steps in LDS, filled by DMA (global_load_lds: no registers, and a step's bytes once,
 // where lanes that load scales for themselves would take them sixteen times).  A stage: the keys'
 // quants of both halves, the values', then the keys' scales and the values'.
-#ifndef STG
-#define STG 3
-#endif
-constexpr int kStages = STG;
+constexpr int kStages = 3;
 template <int NB> struct Stage {
   static constexpr int kQuants = NB * 256, kScales = NB * 32;  // of a half: 16 tokens
   static constexpr int kBytes = 4 * (kQuants + kScales);
@@ -193,16 +191,14 @@ template <int n> __device__ __forceinline__ void wait_loads() {
 
 // Until only the newest `steps` steps' loads are under way.
 template <int kLoads> __device__ __forceinline__ void wait_steps(int steps) {
-  if (steps >= 3)
-    wait_loads<3 * kLoads>();
-  else if (steps == 2)
+  if (steps >= 2)
     wait_loads<2 * kLoads>();
   else if (steps == 1)
     wait_loads<kLoads>();
   else
     wait_loads<0>();
 }
-static_assert(kStages <= 4, "wait_steps");
+static_assert(kStages <= 3, "wait_steps");
 
 // The DMA of one step into the stage at LDS address `to`: at0 and at1 are the page's head that holds
 // each half, place0 and place1 the number of its first token in the page.
@@ -435,9 +431,10 @@ __device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], b
 struct Span {
   uint32_t first, added, rows;  // of its tokens in q; rows a kv head
   int position0, length;        // of its first new token; tokens that may be read
-  __device__ Span(const AttnArgs &a, uint32_t request) {
-    const int begin = max(a.first[request], 0), end = max(a.first[request + 1], 0);
-    const int whole = max(a.length[request], 0);
+  __device__ Span(const AttnArgs &a, uint32_t request)
+      : Span(a, a.first[request], a.first[request + 1], a.length[request]) {}
+  __device__ Span(const AttnArgs &a, int first0, int first1, int length0) {
+    const int begin = max(first0, 0), end = max(first1, 0), whole = max(length0, 0);
     first = static_cast<uint32_t>(begin);
     position0 = whole - max(end - begin, 0);
     added = static_cast<uint32_t>(
@@ -454,8 +451,56 @@ struct Span {
   }
 };
 
+// How the work-groups of the kernel below share out requests of all lengths.  The work is a line of
+// units of 128 tokens (a step of each wave; more, by the power of two unit_shift, where their number
+// would not fit 31 bits), a request's tiles after another's, a tile a kv head; every tile counts kStart
+// more for its beginning and end (a fill and a drain of the loads, a meeting of the waves).  A work-group
+// takes an equal stretch of the line, which may begin and end within a tile: at most two of its tiles are
+// in parts.  Where the line is too short for that, a part of kLeast units or less is a stretch of its own.
+// Against equal parts of the longest request, most of which the others leave empty: 64 requests of 1024
+// to 8192 tokens 99 -> 82 us, of head_dim 256 129 -> 86 (48 requests), f32 and 32 of up to 4096 51 -> 43.
+constexpr uint32_t kStart = 3, kLeast = 2;
+struct Work {
+  uint32_t items, units;  // tiles times kv heads, units of each
+  __device__ Work(const AttnArgs &a, const Span &span) : items(0), units(1) {
+    if (!span.rows || span.rows < a.few_least || span.rows > a.few_most)
+      return;
+    items = (span.rows + kRows - 1) / kRows * (a.heads / a.share);
+    const int seen = span.hi(a, span.added - 1) - begin(a, span);
+    units = seen > 0 ? ((static_cast<uint32_t>(seen) - 1) >> (7 + a.unit_shift)) + 1 : 1;
+  }
+  // where a tile's units begin, for all tiles of a request
+  static __device__ int begin(const AttnArgs &a, const Span &span) { return span.lo(a, 0) & -kStep; }
+  __device__ Work(uint32_t items, uint32_t units) : items(items), units(units) {}
+  // of the line, a tile; the units before its place x
+  __device__ uint32_t parts() const { return (units + kLeast - 1) / kLeast; }
+  __device__ uint32_t weight(bool small) const { return small ? parts() : units + kStart; }
+  __device__ uint32_t before(bool small, uint32_t x) const {
+    return small ? x * units / parts() : max(x, kStart) - kStart;
+  }
+};
+
+template <int kControl, int kLines> __device__ __forceinline__ uint32_t dpp_add(uint32_t x) {
+  return x + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), kControl,
+                                                               kLines, 0xf, false));
+}
+
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ uint32_t lane_sums(uint32_t x) {
+  x = dpp_add<0x111, 0xf>(x);  // the lane 1, 2, 4, 8 before, in a line of 16
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);  // the line before's last
+  return dpp_add<0x143, 0xc>(x);
+}
+
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), lane));
+}
+
 template <int NB, int NP, typename T>
-__global__ __launch_bounds__(kWaves * 64, NB <= 4 ? OCC : 1) void attn_q4_0_rows16(AttnArgs a) {
+__global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16(AttnArgs a) {
   constexpr int D = NB * 32;
   // the waves' rings, and where they meet at the end
   constexpr int kMeet = kWaves * (2 * NB * 16 + 8) * 64;
@@ -463,147 +508,233 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? OCC : 1) void attn_q4_0_rows
   __shared__ __align__(16) uint8_t s_ring[kRing > kMeet ? kRing : kMeet];
   auto s_o = reinterpret_cast<f32x4(*)[2 * NB][64]>(s_ring);
   auto s_ml = reinterpret_cast<float2(*)[64]>(s_ring + kWaves * 2 * NB * 64 * 16);
-  const uint32_t request = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
-  const uint32_t kv_head = blockIdx.y, split = blockIdx.z;
-  const Span span(a, request);
-  if (tile * kRows >= span.rows || span.rows < a.few_least || span.rows > a.few_most)
-    return;
   const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t row_at = tile * kRows + m;
-  const bool valid = row_at < span.rows;
-  const uint32_t i0 = tile * kRows / a.share;
-  const uint32_t i1 = min(tile * kRows + kRows - 1, span.rows - 1) / a.share;
-  // a row past the last one computes what the last one does, and nothing of it is kept
-  const uint32_t mine = min(row_at, span.rows - 1);
-  const uint32_t token = span.first + mine / a.share;
-  const uint32_t head = kv_head * a.share + mine % a.share;
-  // what the tile sees: its first row's first token to its last row's last
-  const int begin = (span.lo(a, i0) & -kStep) + static_cast<int>(split * a.split_tokens);
-  const int end = min(span.hi(a, i1), begin + static_cast<int>(a.split_tokens));
-  if (split && begin >= end)
-    return;
-  const int all_lo = span.lo(a, i1), all_hi = min(span.hi(a, i0), end);  // what every row sees
-  const int my_lo = span.lo(a, mine / a.share), my_hi = min(span.hi(a, mine / a.share), end);
-
-  const PageHead lay(a.page_size, D);
+  // the line's length, and this work-group's stretch [x, line_end) of it
   const uint32_t kv_heads = a.heads / a.share;
-  const int32_t *const table = a.block_table + static_cast<size_t>(request) * a.table_stride;
-  const size_t page_bytes = static_cast<size_t>(lay.bytes()) * kv_heads;
-  const uint8_t *const head_at = a.cache + static_cast<size_t>(kv_head) * lay.bytes();
-
-  // The wave's steps: tokens t_n = begin + 32 (wave + 4 n).  Lane 2 (n % 32) + h holds the page and the
-  // place of step n's half h, for 32 steps at a time.
-  const uint32_t from = static_cast<uint32_t>(begin) + wave * kStep;
-  const uint32_t stop = static_cast<uint32_t>(max(end, begin));
-  const int steps = from < stop ? static_cast<int>((stop - from - 1) / (kWaves * kStep)) + 1 : 0;
-  uint32_t my_page = 0, my_place = 0;
-  const auto look_up = [&](int n) {
-    uint32_t t = from + (n + (lane >> 1)) * (kWaves * kStep) + (lane & 1) * 16;
-    t = t < stop ? t : from;  // past the end the first ones are read again and not seen
-    const uint32_t column = t / a.page_size;
-    my_page = static_cast<uint32_t>(table[column]);
-    my_place = t - column * a.page_size;
+  uint32_t x = blockIdx.x, line_end = x + 1, share = 1;
+  bool small = false;
+  // 64 requests at a time, one a lane: its lengths, its work, and where on the line that begins
+  uint32_t base = 0, line_at = 0, lane_items = 0, lane_units = 0, lane_weight = 0, lane_from = 0;
+  int lane_first0 = 0, lane_first1 = 0, lane_length = 0;
+  const auto look = [&]() __attribute__((always_inline)) {
+    const bool in = base + lane < a.requests;
+    lane_first0 = in ? a.first[base + lane] : 0;
+    lane_first1 = in ? a.first[base + lane + 1] : 0;
+    lane_length = in ? a.length[base + lane] : 0;
+    const Work work(a, Span(a, lane_first0, lane_first1, lane_length));
+    lane_items = work.items;
+    lane_units = work.units;
   };
-  uint8_t *const ring = s_ring + wave * (kStages * Stage<NB>::kBytes);
-  const uint32_t ring_at = static_cast<uint32_t>(
-      __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>(
-          (lds_byte *)ring))));
-  uint32_t there = 0;  // bit 2 (n % 16) + h: whether step n's half h lies in a page
-  const auto load = [&](int n) {
-    if (n % 32 == 0)
-      look_up(n);
-    const int from_lane = 2 * (n % 32);
-    const uint32_t page0 = __builtin_amdgcn_readlane(my_page, from_lane);
-    const uint32_t page1 = __builtin_amdgcn_readlane(my_page, from_lane + 1);
-    const bool in0 = page0 < a.pages, in1 = page1 < a.pages;
-    there = (there & ~(3u << (2 * (n % 16)))) |
-            ((in0 ? 1u : 0u) | (in1 ? 2u : 0u)) << (2 * (n % 16));
-    load_step<NB>(head_at + (in0 ? page0 : 0) * page_bytes,
-                  head_at + (in1 ? page1 : 0) * page_bytes,
-                  __builtin_amdgcn_readlane(my_place, from_lane),
-                  __builtin_amdgcn_readlane(my_place, from_lane + 1), lay,
-                  ring_at + (n % kStages) * Stage<NB>::kBytes, lane);
+  const auto lay_out = [&]() __attribute__((always_inline)) {
+    lane_weight = lane_items * Work(lane_items, lane_units).weight(small);
+    const uint32_t sum = lane_sums(lane_weight);
+    lane_from = line_at + sum - lane_weight;
+    line_at += lane_of(sum, 63);
   };
-  for (int n = 0; n < kStages - 1; ++n)
-    if (n < steps)
-      load(n);
-  Row<NB, NP> row;  // its loads behind those of the first steps, which take longer
-  load_row<NB, NP, T>(row,
-                      static_cast<const T *>(a.q) + static_cast<size_t>(token) * a.q_token +
-                          static_cast<size_t>(head) * a.q_head,
-                      valid, a.q_vec, g, a.scale);
-  for (int n = 0; n < steps; ++n) {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage before this one is read
-    if (n + kStages - 1 < steps)
-      load(n + kStages - 1);
-    wait_steps<Stage<NB>::kLoads>(min(steps - 1 - n, kStages - 1));
-    Tokens16<NB> t[2];
-    read_step<NB>(t, ring + (n % kStages) * Stage<NB>::kBytes, m, g);
-    const int t0 = static_cast<int>(from) + n * (kWaves * kStep);
-    const uint32_t both = there >> (2 * (n % 16)) & 3u;
-    const bool edge = t0 < all_lo || t0 + kStep > all_hi || both != 3u;
-    uint32_t seen = 0;
-    if (edge) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int at = t0 + 16 * (i >> 2) + 4 * g + (i & 3);
-        seen |= at >= my_lo && at < my_hi && (both >> (i >> 2) & 1u) ? 1u << i : 0u;
-      }
+  if (a.groups) {
+    uint32_t parts = 0, units = 0;
+    for (;;) {
+      look();
+      parts += lane_items * Work(lane_items, lane_units).weight(true);
+      units += lane_items * Work(lane_items, lane_units).weight(false);
+      base += 64;
+      if (base >= a.requests)
+        break;
     }
-    attend<NB, NP>(row, t, edge, seen);
+    parts = lane_of(lane_sums(parts), 63);
+    units = lane_of(lane_sums(units), 63);
+    small = parts <= a.groups;
+    share = small ? 1 : (units + a.groups - 1) / a.groups;
+    x = blockIdx.x * share;
+    line_end = min(x + share, small ? parts : units);
+    base = 0;
+    if (a.requests > 64)
+      look();
+    lay_out();
   }
+  uint4 begun{};  // the tile that begins here and not ends: request, item, where it ends
+  while (x < line_end) {
+    Work work(0, 1);
+    uint32_t request, item, at = 0;
+    int first0, first1, length;
+    if (a.groups) {
+      const uint64_t here = __ballot(x - lane_from < lane_weight);
+      if (!here) {
+        base += 64;
+        if (base >= a.requests)
+          break;
+        look();
+        lay_out();
+        continue;
+      }
+      const int owner = __builtin_ctzll(here);
+      request = base + owner;
+      first0 = static_cast<int>(lane_of(static_cast<uint32_t>(lane_first0), owner));
+      first1 = static_cast<int>(lane_of(static_cast<uint32_t>(lane_first1), owner));
+      length = static_cast<int>(lane_of(static_cast<uint32_t>(lane_length), owner));
+      work.units = lane_of(lane_units, owner);
+      const uint32_t place = x - lane_of(lane_from, owner);
+      item = place / work.weight(small);
+      at = place - item * work.weight(small);
+    } else {
+      request = x / (a.tiles * kv_heads);
+      item = x - request * (a.tiles * kv_heads);
+      first0 = a.first[request];
+      first1 = a.first[request + 1];
+      length = a.length[request];
+    }
+    const Span span(a, first0, first1, length);
+    if (!a.groups) {
+      work = Work(a, span);
+      if (item >= work.items)
+        return;
+    }
+    const uint32_t weight = work.weight(small);
+    const uint32_t to = a.groups ? min(weight, at + line_end - x) : weight;
+    const bool whole = at == 0 && to == weight;
+    if (at == 0 && to != weight)
+      begun = make_uint4(request, item, (x + weight - 1) / share, 0);
+    x += to - at;
+    const uint32_t tile = item / kv_heads, kv_head = item - tile * kv_heads;
+    const uint32_t row_at = tile * kRows + m;
+    const bool valid = row_at < span.rows;
+    const uint32_t i0 = tile * kRows / a.share;
+    const uint32_t i1 = min(tile * kRows + kRows - 1, span.rows - 1) / a.share;
+    // a row past the last one computes what the last one does, and nothing of it is kept
+    const uint32_t mine = min(row_at, span.rows - 1);
+    const uint32_t token = span.first + mine / a.share;
+    const uint32_t head = kv_head * a.share + mine % a.share;
+    // the stretch's units, of what the request's first row's first token to its last row's last
+    const uint32_t unit0 = work.before(small, at), unit1 = work.before(small, to);
+    const int all = Work::begin(a, span), seen_end = span.hi(a, i1);
+    const int begin = all + static_cast<int>(unit0 << (7 + a.unit_shift));
+    const int end = whole ? seen_end
+                          : min(seen_end, all + static_cast<int>(unit1 << (7 + a.unit_shift)));
+    const int all_lo = span.lo(a, i1), all_hi = min(span.hi(a, i0), end);  // what every row sees
+    const int my_lo = span.lo(a, mine / a.share), my_hi = min(span.hi(a, mine / a.share), end);
 
-  // to plain units, then the waves' parts together, a share of the elements a wave
-  row.l = row_sum(row.l);
-  if constexpr (NP == 1) {
+    const PageHead lay(a.page_size, D);
+    const int32_t *const table = a.block_table + static_cast<size_t>(request) * a.table_stride;
+    const size_t page_bytes = static_cast<size_t>(lay.bytes()) * kv_heads;
+    const uint8_t *const head_at = a.cache + static_cast<size_t>(kv_head) * lay.bytes();
+
+    // The wave's steps: tokens t_n = begin + 32 (wave + 4 n).  Lane 2 (n % 32) + h holds the page and the
+    // place of step n's half h, for 32 steps at a time.
+    const uint32_t from = static_cast<uint32_t>(begin) + wave * kStep;
+    const uint32_t stop = static_cast<uint32_t>(max(end, begin));
+    const int steps = from < stop ? static_cast<int>((stop - from - 1) / (kWaves * kStep)) + 1 : 0;
+    uint32_t my_page = 0, my_place = 0;
+    const auto look_up = [&](int n) {
+      uint32_t t = from + (n + (lane >> 1)) * (kWaves * kStep) + (lane & 1) * 16;
+      t = t < stop ? t : from;  // past the end the first ones are read again and not seen
+      const uint32_t column = t / a.page_size;
+      my_page = static_cast<uint32_t>(table[column]);
+      my_place = t - column * a.page_size;
+    };
+    uint8_t *const ring = s_ring + wave * (kStages * Stage<NB>::kBytes);
+    const uint32_t ring_at = static_cast<uint32_t>(
+        __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>(
+            (lds_byte *)ring))));
+    uint32_t there = 0;  // bit 2 (n % 16) + h: whether step n's half h lies in a page
+    const auto load = [&](int n) {
+      if (n % 32 == 0)
+        look_up(n);
+      const int from_lane = 2 * (n % 32);
+      const uint32_t page0 = __builtin_amdgcn_readlane(my_page, from_lane);
+      const uint32_t page1 = __builtin_amdgcn_readlane(my_page, from_lane + 1);
+      const bool in0 = page0 < a.pages, in1 = page1 < a.pages;
+      there = (there & ~(3u << (2 * (n % 16)))) |
+              ((in0 ? 1u : 0u) | (in1 ? 2u : 0u)) << (2 * (n % 16));
+      load_step<NB>(head_at + (in0 ? page0 : 0) * page_bytes,
+                    head_at + (in1 ? page1 : 0) * page_bytes,
+                    __builtin_amdgcn_readlane(my_place, from_lane),
+                    __builtin_amdgcn_readlane(my_place, from_lane + 1), lay,
+                    ring_at + (n % kStages) * Stage<NB>::kBytes, lane);
+    };
+    for (int n = 0; n < kStages - 1; ++n)
+      if (n < steps)
+        load(n);
+    Row<NB, NP> row;  // its loads behind those of the first steps, which take longer
+    load_row<NB, NP, T>(row,
+                        static_cast<const T *>(a.q) + static_cast<size_t>(token) * a.q_token +
+                            static_cast<size_t>(head) * a.q_head,
+                        valid, a.q_vec, g, a.scale);
+    for (int n = 0; n < steps; ++n) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage before this one is read
+      if (n + kStages - 1 < steps)
+        load(n + kStages - 1);
+      wait_steps<Stage<NB>::kLoads>(min(steps - 1 - n, kStages - 1));
+      Tokens16<NB> t[2];
+      read_step<NB>(t, ring + (n % kStages) * Stage<NB>::kBytes, m, g);
+      const int t0 = static_cast<int>(from) + n * (kWaves * kStep);
+      const uint32_t both = there >> (2 * (n % 16)) & 3u;
+      const bool edge = t0 < all_lo || t0 + kStep > all_hi || both != 3u;
+      uint32_t seen = 0;
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int at = t0 + 16 * (i >> 2) + 4 * g + (i & 3);
+          seen |= at >= my_lo && at < my_hi && (both >> (i >> 2) & 1u) ? 1u << i : 0u;
+        }
+      }
+      attend<NB, NP>(row, t, edge, seen);
+    }
+
+    // to plain units, then the waves' parts together, a share of the elements a wave
+    row.l = row_sum(row.l);
+    if constexpr (NP == 1) {
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i)
+        row.o[i] = row.o[i] * 0x1p24f - 8.0f * row.weights[i / 2];
+    }
+    rescale(row, exp2_fast(-shift_of(row.level)));
+    __syncthreads();  // all have read their rings
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i)
-      row.o[i] = row.o[i] * 0x1p24f - 8.0f * row.weights[i / 2];
-  }
-  rescale(row, exp2_fast(-shift_of(row.level)));
-  __syncthreads();  // all have read their rings
-#pragma unroll
-  for (int i = 0; i < 2 * NB; ++i)
-    s_o[wave][i][lane] = row.o[i];
-  s_ml[wave][lane] = make_float2(row.m, row.l);
-  __syncthreads();
-  if (!valid)
-    return;
-  float top = kNone, l = 0.0f, f[kWaves];
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w)
-    top = fmaxf(top, s_ml[w][lane].x);
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const float2 x = s_ml[w][lane];
-    f[w] = x.x == top ? 1.0f : exp2_fast(x.x - top);
-    l += x.y * f[w];
-  }
-  const float inverse = a.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-  const size_t at = (static_cast<size_t>(split) * a.tokens + token) * a.heads + head;
-  T *const out = static_cast<T *>(a.out) + static_cast<size_t>(token) * a.out_token +
-                 static_cast<size_t>(head) * a.out_head;
-#pragma unroll
-  for (int k = 0; k < 2 * NB / kWaves; ++k) {
-    const int i = wave * (2 * NB / kWaves) + k;
-    f32x4 o{};
+      s_o[wave][i][lane] = row.o[i];
+    s_ml[wave][lane] = make_float2(row.m, row.l);
+    __syncthreads();
+    float top = kNone, l = 0.0f, f[kWaves];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
-      o += s_o[w][i][lane] * f[w];
-    float v[4];
+      top = fmaxf(top, s_ml[w][lane].x);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      v[r] = o[r] * inverse;
-    if (a.splits > 1)
-      store_values<4>(a.parts + at * D + 16 * i + 4 * g, v, true);
-    else
-      store_values<4>(out + 16 * i + 4 * g, v, a.out_vec);
+    for (int w = 0; w < kWaves; ++w) {
+      const float2 x = s_ml[w][lane];
+      f[w] = x.x == top ? 1.0f : exp2_fast(x.x - top);
+      l += x.y * f[w];
+    }
+    const float inverse = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    const size_t part = (2 * blockIdx.x + (at == 0 ? 1 : 0)) * kRows + m;
+    T *const out = static_cast<T *>(a.out) + static_cast<size_t>(token) * a.out_token +
+                   static_cast<size_t>(head) * a.out_head;
+#pragma unroll
+    for (int k = 0; k < 2 * NB / kWaves; ++k) {
+      const int i = wave * (2 * NB / kWaves) + k;
+      f32x4 o{};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w)
+        o += s_o[w][i][lane] * f[w];
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        v[r] = o[r] * inverse;
+      if (!valid)
+        continue;
+      if (!whole)
+        store_values<4>(a.parts + part * D + 16 * i + 4 * g, v, true);
+      else
+        store_values<4>(out + 16 * i + 4 * g, v, a.out_vec);
+    }
+    if (!whole && valid && g == 0 && wave == 0) {
+      const size_t all_parts = static_cast<size_t>(a.groups) * (2 * kRows);
+      *reinterpret_cast<float2 *>(a.parts + all_parts * D + 2 * part) = make_float2(top, l);
+    }
+    __syncthreads();  // before the next stretch's steps are loaded over these
   }
-  if (a.splits > 1 && g == 0 && wave == 0) {
-    const size_t all = static_cast<size_t>(a.splits) * a.tokens * a.heads;
-    *reinterpret_cast<float2 *>(a.parts + all * D + 2 * at) = make_float2(top, l);
-  }
+  if (a.groups && threadIdx.x == 0)
+    a.plan[blockIdx.x] = begun;
 }
 
 // ---------------------------------------------------------------------------
@@ -1113,19 +1244,83 @@ attn_q4_0_tiles(AttnArgs a) {
   }
 }
 
-// The parts of a row together, 4 elements a thread; one launch joins both kernels' rows, a Cut each: how
-// the kernel had cut them.  Of few parts a group of head_dim / 4 threads takes a head, and the groups of
-// a work-group heads side by side; from kManyParts on the groups share out one head's parts.
-struct Cut {
-  const float *parts;
-  uint32_t tile_rows, split_tokens, splits;
-};
-constexpr int kJoinThreads = 256, kManyParts = 8;
+// The stretches of a tile of attn_q4_0_rows16 together: a work-group takes a row of the tile that one
+// of the kernel's work-groups has begun, 4 elements a thread, and groups of head_dim / 4 threads share
+// out the stretches.
+constexpr int kJoinThreads = 256;
+
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join_few(AttnArgs a, uint32_t head_dim) {
+  __shared__ f32x4 s_o[kJoinThreads];
+  __shared__ float2 s_ml[kJoinThreads];
+  const uint4 begun = a.plan[blockIdx.x];
+  if (begun.z == 0)
+    return;
+  const uint32_t stretches = begun.z - blockIdx.x + 1;
+  const uint32_t kv_heads = a.heads / a.share, tile = begun.y / kv_heads;
+  const Span span(a, begun.x);
+  const uint32_t row = tile * kRows + blockIdx.y;
+  if (row >= span.rows)
+    return;
+  const uint32_t per_head = head_dim / 4, groups = kJoinThreads / per_head;
+  const uint32_t e = 4 * (threadIdx.x % per_head), group = threadIdx.x / per_head;
+  // the first one's part is its work-group's second, the others' their first
+  const auto at = [&](uint32_t s) {
+    return (2 * (blockIdx.x + s) + (s == 0 ? 1 : 0)) * static_cast<size_t>(kRows) + blockIdx.y;
+  };
+  const float2 *const ml = reinterpret_cast<const float2 *>(
+      a.parts + static_cast<size_t>(a.groups) * (2 * kRows) * head_dim);
+  float m = kNone, l = 0.0f;
+  f32x4 o{};
+  if (group < groups) {
+#pragma unroll 4
+    for (uint32_t s = group; s < stretches; s += groups) {
+      // as they come: 16 bytes of output and 8 of its maximum and sum in one turn
+      const float2 x = ml[at(s)];
+      const f32x4 v = *reinterpret_cast<const f32x4 *>(a.parts + at(s) * head_dim + e);
+      const float top = fmaxf(m, x.x);
+      const float f = m == top ? 1.0f : exp2_fast(m - top), h = x.x == top ? 1.0f : exp2_fast(x.x - top);
+      l = l * f + x.y * h;
+      o = o * f + v * h;
+      m = top;
+    }
+  }
+  s_o[threadIdx.x] = o;
+  s_ml[threadIdx.x] = make_float2(m, l);
+  __syncthreads();
+  if (group != 0)
+    return;
+  float top = kNone;
+  for (uint32_t k = 0; k < groups; ++k)
+    top = fmaxf(top, s_ml[k * per_head + threadIdx.x].x);
+  o = f32x4{};
+  l = 0.0f;
+  for (uint32_t k = 0; k < groups; ++k) {
+    const float2 x = s_ml[k * per_head + threadIdx.x];
+    const float f = x.x == top ? 1.0f : exp2_fast(x.x - top);
+    l += x.y * f;
+    o += s_o[k * per_head + threadIdx.x] * f;
+  }
+  float v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    v[k] = l == 0.0f ? 0.0f : o[k] / l;
+  const uint32_t token = span.first + row / a.share;
+  const uint32_t head = (begun.y - tile * kv_heads) * a.share + row % a.share;
+  store_values<4>(static_cast<T *>(a.out) + static_cast<size_t>(token) * a.out_token +
+                      static_cast<size_t>(head) * a.out_head + e,
+                  v, a.out_vec);
+}
+
+// The parts of a row of attn_q4_0_tiles together, 4 elements a thread.  Of few parts a group of
+// head_dim / 4 threads takes a head, and the groups of a work-group heads side by side; from kManyParts
+// on the groups share out one head's parts.
+constexpr int kManyParts = 8;
 
 template <typename T, bool kShared>
 __global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join(AttnArgs a, uint32_t requests,
-                                                               uint32_t head_dim, Cut few,
-                                                               Cut many) {
+                                                               uint32_t head_dim,
+                                                               uint32_t tile_rows) {
   __shared__ f32x4 s_o[kJoinThreads];
   __shared__ float2 s_ml[kJoinThreads];
   const uint32_t token = blockIdx.x, lane = threadIdx.x & 63;
@@ -1140,26 +1335,23 @@ __global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join(AttnArgs a, uint3
     n = min(step, n - skip);
   }
   const Span span(a, request);
-  if (token < span.first || token - span.first >= span.added)
-    return;
-  const Cut cut = span.rows <= a.few_most ? few : many;
-  if (cut.splits <= 1)
+  if (token < span.first || token - span.first >= span.added || span.rows < a.few_least)
     return;
   const uint32_t per_head = head_dim / 4, groups = kJoinThreads / per_head;
   const uint32_t e = 4 * (threadIdx.x % per_head), group = threadIdx.x / per_head;
   const uint32_t head = kShared ? blockIdx.y : blockIdx.y * groups + group;
   const bool works = head < a.heads && group < groups;
-  // the tile's own range, as the kernels above cut it
+  // the tile's own range, as the kernel cut it
   const uint32_t i = token - span.first;
-  const uint32_t row0 = (i * a.share + head % a.share) / cut.tile_rows * cut.tile_rows;
-  const uint32_t i0 = row0 / a.share, i1 = min(row0 + cut.tile_rows - 1, span.rows - 1) / a.share;
+  const uint32_t row0 = (i * a.share + head % a.share) / tile_rows * tile_rows;
+  const uint32_t i0 = row0 / a.share, i1 = min(row0 + tile_rows - 1, span.rows - 1) / a.share;
   const int tokens = max(span.hi(a, i1) - (span.lo(a, i0) & -kStep), 1);
-  const uint32_t splits = min((tokens + cut.split_tokens - 1) / cut.split_tokens, cut.splits);
+  const uint32_t splits = min((tokens + a.split_tokens - 1) / a.split_tokens, a.splits);
   const size_t row = static_cast<size_t>(token) * a.heads + head;
   const size_t stride = static_cast<size_t>(a.tokens) * a.heads;
   const float2 *const ml =
-      reinterpret_cast<const float2 *>(cut.parts + cut.splits * stride * head_dim) + row;
-  const float *const part = cut.parts + row * head_dim + e;
+      reinterpret_cast<const float2 *>(a.parts + a.splits * stride * head_dim) + row;
+  const float *const part = a.parts + row * head_dim + e;
   const uint32_t s0 = kShared ? group : 0, by = kShared ? groups : 1;
   float m = kNone, l = 0.0f;
   f32x4 o{};
@@ -1231,22 +1423,63 @@ size_t many_rows(int elem, size_t head_dim) {
                            : TileStep<8, 1>::kRows;
 }
 
+// Work-groups of the kernel of few rows that the card runs at a time, by their registers and LDS: the
+// shares of its work (64 requests of 1024 to 8192 tokens, f16, 32 query and 8 kv heads of 128: 112 us in
+// 256 shares, 86 in 512, 96 in 768).
+size_t most_groups(size_t head_dim) { return head_dim <= 128 ? 512 : 256; }
+
+// Requests so short that a work-group a tile serves them sooner, where the tiles fill the card (us, whole
+// tiles / shares, contexts from an eighth of the longest up: 64 requests of up to 1024 tokens 21 / 29,
+// 2048 31 / 35, 4096 54 / 52, 8192 99 / 82; 128 of 2048 56 / 59, of 8192 155 / 146), in
+// proportion where they do not (32 of 1024 17 / 23; f32, 32 of 4096 68 / 51; one of 531 15 / 14).
+constexpr size_t kWholeTokens = 2560;
+
 struct Plan {
-  size_t tile_rows, tiles, splits, split_tokens, workspace;
+  size_t tile_rows, tiles, workspace;
+  size_t splits, split_tokens;        // many rows
+  size_t groups, unit_shift, launch;  // few rows: shares (0: a tile a work-group), work-groups
 };
 
-// Work-groups of one tile each, as many as the card runs at a time; the tokens of fewer tiles are
-// split into parts of at least 256 tokens.  More parts cost more in work-groups' beginnings than they
-// even out: decode over two contexts of 131072 75 us in 512 parts, 81 in 1024, 86 in 1536.
-Plan plan_of(bool few, int elem, size_t requests, size_t tokens, size_t max_added,
-             size_t max_length, size_t window, size_t heads, size_t kv_heads, size_t head_dim) {
+size_t parts_bytes(size_t parts, size_t head_dim) {
+  return parts * (head_dim + 2) * sizeof(float);
+}
+
+// The shares of the kernel of few rows, for lengths up to max_length; none where no tile has enough
+// tokens to be cut.
+Plan few_plan(size_t requests, size_t max_added, size_t max_length, size_t window, size_t heads,
+              size_t kv_heads, size_t head_dim) {
+  Plan p{};
   const size_t share = heads / kv_heads;
-  Plan p;
-  p.tile_rows = few ? tcrv::kRows : many_rows(elem, head_dim);
-  size_t rows = max_added * share;
-  if (few)
-    rows = std::min(rows, few_rows_of(requests, rows, kv_heads));
+  const size_t rows = std::min(max_added * share, few_rows_of(requests, max_added * share, kv_heads));
+  p.tile_rows = tcrv::kRows;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+  const size_t items = requests * p.tiles * kv_heads;
+  // what is seen begins at a multiple of 32; `window` is 0 where it does not bound that
+  size_t seen = max_length + 31;
+  if (window && window < seen)
+    seen = std::min(seen, window + max_added + 31);
+  const auto units = [&] { return std::max((seen - 1) >> (7 + p.unit_shift), size_t{0}) + 1; };
+  while (items * (units() + tcrv::kStart) > 0x7fffffffu && units() > 1)
+    ++p.unit_shift;
+  const size_t parts = (units() + tcrv::kLeast - 1) / tcrv::kLeast;
+  p.launch = items;
+  const size_t most = most_groups(head_dim);
+  if (parts > 1 && seen - 31 > kWholeTokens * std::min(items, most) / most) {
+    p.launch = p.groups = std::min(items * parts, most);
+    p.workspace = parts_bytes(p.groups * 2 * tcrv::kRows, head_dim) +
+                  p.groups * sizeof(uint4);
+  }
+  return p;
+}
+
+// Work-groups of one tile each, as many as the card runs at a time; the tokens of fewer tiles are
+// split into parts of at least 512 tokens.
+Plan many_plan(int elem, size_t requests, size_t tokens, size_t max_added, size_t max_length,
+               size_t window, size_t heads, size_t kv_heads, size_t head_dim) {
+  const size_t share = heads / kv_heads;
+  Plan p{};
+  p.tile_rows = many_rows(elem, head_dim);
+  p.tiles = (max_added * share + p.tile_rows - 1) / p.tile_rows;
   const size_t groups = requests * p.tiles * kv_heads;
   const auto parts_of = [&](size_t seen) {
     const size_t most = std::max((seen + 511) / 512, size_t{1});
@@ -1261,7 +1494,7 @@ Plan plan_of(bool few, int elem, size_t requests, size_t tokens, size_t max_adde
   p.splits = (seen + p.split_tokens - 1) / p.split_tokens;
   // for any window: a smaller one has no more parts
   const size_t most = parts_of(max_length + 31);
-  p.workspace = most == 1 ? 0 : most * tokens * heads * (head_dim + 2) * sizeof(float);
+  p.workspace = most == 1 ? 0 : parts_bytes(most * tokens * heads, head_dim);
   return p;
 }
 
@@ -1279,8 +1512,8 @@ Kernels kernels_of(size_t requests, size_t tokens, size_t max_added, size_t head
 }
 
 template <int NP, typename T>
-void launch_rows16(const AttnArgs &a, size_t head_dim, dim3 grid, hipStream_t st) {
-  const dim3 block(tcrv::kWaves * 64);
+void launch_rows16(const AttnArgs &a, size_t head_dim, unsigned groups, hipStream_t st) {
+  const dim3 grid(groups), block(tcrv::kWaves * 64);
   switch (head_dim) {
   case 64:
     tcrv::attn_q4_0_rows16<2, NP, T><<<grid, block, 0, st>>>(a);
@@ -1325,39 +1558,45 @@ void launch_all(AttnArgs a, Kernels k, const Plan &few, const Plan &many, size_t
                 size_t requests, hipStream_t st) {
   const unsigned kv_heads = a.heads / a.share, n = static_cast<unsigned>(requests);
   float *const workspace = a.parts;
-  const auto set = [&](const Plan &p, float *parts) {
-    a.parts = parts;
-    a.tiles = static_cast<uint32_t>(p.tiles);
-    a.split_tokens = static_cast<uint32_t>(p.split_tokens);
-    a.splits = static_cast<uint32_t>(p.splits);
-    return tcrv::Cut{parts, static_cast<uint32_t>(p.tile_rows), a.split_tokens, a.splits};
-  };
-  tcrv::Cut cut_few{nullptr, 1, 1, 0}, cut_many{nullptr, 1, 1, 0};
   const uint32_t few_most = !k.few ? 0 : k.many ? static_cast<uint32_t>(k.few_rows) : 0xffffffffu;
+  const uint32_t dim = static_cast<uint32_t>(head_dim);
+  const dim3 join_block(tcrv::kJoinThreads);
+  a.requests = n;
   if (k.few) {
-    cut_few = set(few, workspace);
+    a.groups = static_cast<uint32_t>(few.groups);
+    a.unit_shift = static_cast<uint32_t>(few.unit_shift);
+    a.tiles = static_cast<uint32_t>(few.tiles);
+    a.plan = reinterpret_cast<uint4 *>(workspace);
+    a.parts = workspace + few.groups * (sizeof(uint4) / sizeof(float));
     a.few_least = 0;
     a.few_most = few_most;
-    launch_rows16<NP, T>(a, head_dim, dim3(n * a.tiles, kv_heads, a.splits), st);
+    launch_rows16<NP, T>(a, head_dim, static_cast<unsigned>(few.launch), st);
+    if (few.groups) {
+      const size_t rows = std::min(static_cast<size_t>(a.max_added) * a.share, few.tile_rows);
+      tcrv::attn_q4_0_join_few<T>
+          <<<dim3(a.groups, static_cast<unsigned>(rows)), join_block, 0, st>>>(a, dim);
+    }
   }
   if (k.many) {
-    cut_many = set(many, workspace + (k.few ? few.workspace / sizeof(float) : 0));
+    a.parts = workspace + (k.few ? few.workspace / sizeof(float) : 0);
+    a.tiles = static_cast<uint32_t>(many.tiles);
+    a.split_tokens = static_cast<uint32_t>(many.split_tokens);
+    a.splits = static_cast<uint32_t>(many.splits);
     a.few_least = few_most ? few_most + 1 : 0;
     a.few_most = 0xffffffffu;
     launch_tiles<NP, T>(a, head_dim, dim3(n * kv_heads, a.tiles, a.splits), st);
-  }
-  const uint32_t parts = std::max(cut_few.splits, cut_many.splits);
-  if (parts > 1) {
-    a.few_most = few_most;
-    const uint32_t dim = static_cast<uint32_t>(head_dim), groups = tcrv::kJoinThreads / (dim / 4);
-    const dim3 block(tcrv::kJoinThreads);
-    // shared out while the rows alone are few work-groups
-    if (parts >= tcrv::kManyParts && static_cast<size_t>(a.tokens) * a.heads <= 4096)
-      tcrv::attn_q4_0_join<T, true>
-          <<<dim3(a.tokens, a.heads), block, 0, st>>>(a, n, dim, cut_few, cut_many);
-    else
-      tcrv::attn_q4_0_join<T, false><<<dim3(a.tokens, (a.heads + groups - 1) / groups), block, 0, st>>>(
-          a, n, dim, cut_few, cut_many);
+    if (many.splits > 1) {
+      const uint32_t tile_rows = static_cast<uint32_t>(many.tile_rows);
+      const uint32_t groups = tcrv::kJoinThreads / (dim / 4);
+      // shared out while the rows alone are few work-groups
+      if (many.splits >= tcrv::kManyParts && static_cast<size_t>(a.tokens) * a.heads <= 4096)
+        tcrv::attn_q4_0_join<T, true>
+            <<<dim3(a.tokens, a.heads), join_block, 0, st>>>(a, n, dim, tile_rows);
+      else
+        tcrv::attn_q4_0_join<T, false>
+            <<<dim3(a.tokens, (a.heads + groups - 1) / groups), join_block, 0, st>>>(a, n, dim,
+                                                                                    tile_rows);
+    }
   }
 }
 
@@ -1389,7 +1628,8 @@ size_t tcrv_hip_attn_q4_0_workspace_bytes(int elem, size_t requests, size_t toke
   size_t need = 0;
   for (const bool few : {true, false})
     if (few ? k.few : k.many)
-      need += plan_of(few, elem, requests, tokens, max_added, max_length, 0, heads, kv_heads, head_dim)
+      need += (few ? few_plan(requests, max_added, max_length, 0, heads, kv_heads, head_dim)
+                   : many_plan(elem, requests, tokens, max_added, max_length, 0, heads, kv_heads, head_dim))
                   .workspace;
   return need;
 }
@@ -1422,12 +1662,12 @@ int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
   if (pages == 0)
     max_length = 0;  // nothing to read
   const Kernels k = kernels_of(requests, tokens, max_added, heads, kv_heads);
-  const Plan few = plan_of(true, elem, requests, tokens, max_added, max_length, causal ? window : 0, heads,
-                            kv_heads, head_dim);
+  const size_t bound = causal ? window : 0;
+  const Plan few = few_plan(requests, max_added, max_length, bound, heads, kv_heads, head_dim);
   const Plan many =
-      plan_of(false, elem, requests, tokens, max_added, max_length, causal ? window : 0, heads, kv_heads, head_dim);
-  if (requests * few.tiles > 0x7fffffffu || few.splits > 65535u || many.splits > 65535u ||
-      (k.many && (many.tiles > 65535u || requests * kv_heads > 0x7fffffffu)))
+      many_plan(elem, requests, tokens, max_added, max_length, bound, heads, kv_heads, head_dim);
+  if ((k.few && requests * few.tiles * kv_heads > 0x7fffffffu) ||
+      (k.many && (many.splits > 65535u || many.tiles > 65535u || requests * kv_heads > 0x7fffffffu)))
     return TCRV_HIP_ERR_TOO_LARGE;
   const size_t need = (k.few ? few.workspace : 0) + (k.many ? many.workspace : 0);
   if (need) {
@@ -1445,6 +1685,7 @@ int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
              first,
              length,
              static_cast<float *>(workspace),
+             nullptr,
              q_token,
              q_head,
              out_token,
@@ -1458,9 +1699,12 @@ int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
              static_cast<uint32_t>(tokens),
              static_cast<uint32_t>(heads),
              static_cast<uint32_t>(heads / kv_heads),
-             0,  // the plan's: launch_attn
+             0,  // the plans': launch_all
              static_cast<uint32_t>(max_added),
              static_cast<uint32_t>(max_length),
+             0,
+             0,
+             0,
              0,
              0,
              0,
