@@ -89,20 +89,30 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Four dwords, each with a quant in the lowest bits of its halves, as an operand: n - 8 for two parts,
-// n 2^-24 for one.
+// Quants from the halves of dwords, as operands: n - 8 for two parts, n 2^-24 for one; kFours: of their
+// bits 4 .. 7, which are left where they are, 16 times that.
 template <int NP> struct Quants {
   uint32_t bits;  // of 1024.0, kept in a register: an instruction takes one constant
   __device__ Quants() : bits(0x64006400u) { asm("" : "+v"(bits)); }
-  __device__ __forceinline__ uint32_t pair(uint32_t w) const {
+  template <bool kFours> __device__ __forceinline__ uint32_t pair(uint32_t w) const {
+    constexpr uint32_t kMask = kFours ? 0x00f000f0u : 0x000f000fu;
     if constexpr (NP == 1)
-      return w & 0x000f000fu;
-    const f16x2 v = __builtin_bit_cast(f16x2, (w & 0x000f000fu) | bits);
-    return __builtin_bit_cast(uint32_t, v + f16x2{-1032, -1032});
+      return w & kMask;
+    constexpr int kOff = kFours ? -1152 : -1032;
+    const f16x2 v = __builtin_bit_cast(f16x2, (w & kMask) | bits);
+    return __builtin_bit_cast(uint32_t, v + f16x2{kOff, kOff});
   }
-  __device__ __forceinline__ f16x8 operator()(uint32_t a, uint32_t b, uint32_t c,
-                                              uint32_t d) const {
-    u32x4 v = {pair(a), pair(b), pair(c), pair(d)};
+  // the keys of a dword; of one part the second and the fourth pair 16 times, which their queries make
+  // up for: 5 instructions a dword for 7, 64 requests as above 87 -> 86 us
+  __device__ __forceinline__ f16x8 keys(uint32_t w) const {
+    u32x4 v = {pair<false>(w), pair<NP == 1>(NP == 1 ? w : w >> 4), pair<false>(w >> 8),
+               pair<NP == 1>(w >> (NP == 1 ? 8 : 12))};
+    return __builtin_bit_cast(f16x8, v);
+  }
+  // a pair of each of four dwords
+  template <bool kFours>
+  __device__ __forceinline__ f16x8 values(uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {
+    u32x4 v = {pair<kFours>(a), pair<kFours>(b), pair<kFours>(c), pair<kFours>(d)};
     return __builtin_bit_cast(f16x8, v);
   }
 };
@@ -123,6 +133,19 @@ __device__ __forceinline__ void split_pair(float x0, float x1, f16x8 (&part)[kPa
     part[1][i] = static_cast<_Float16>(x0 - static_cast<float>(h[0]));
     part[1][i + 1] = static_cast<_Float16>(x1 - static_cast<float>(h[1]));
   }
+}
+
+// Two f32 values times two fp16 ones, rounded once, to f16: the instructions that widen and narrow on the
+// way, which the compiler does not form here (64 requests of 1024 to 8192 tokens, f16: 89 us by its own, 87
+// so; 82 with the weight rounded first and the product again, which made the output's error 3.2e-4 of it
+// where one rounding leaves 2.8e-4, its own 2.1e-4 among them).
+__device__ __forceinline__ f16x2 times_pair(float x0, float x1, uint32_t d) {
+  uint32_t r;
+  asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(r) : "v"(x0), "v"(d));
+  asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]"
+      : "+v"(r)
+      : "v"(x1), "v"(d));
+  return __builtin_bit_cast(f16x2, r);
 }
 
 // A lane's own value and that of lane ^ 32 (lane ^ 16), in an order that both lanes share.
@@ -242,7 +265,7 @@ template <int NB, int NP> struct Row {
   f16x8 q[NB][NP];      // the block's elements in the order in which the keys' nibbles come
   Quants<NP> quants;
   float unit;           // from the products' units to scores in powers of 2
-  f32x4 o[2 * NB];      // 16 elements each: block o / 2, half o % 2
+  f32x4 o[2 * NB];      // 16 elements each: block o / 2, half o % 2, the second ones 16 times
   // for one part, whose quants lack the -8: the keys' products start at -8 sum q, and the values'
   // take 8 times these sums of the weights off at the end
   f32x4 start[NP == 1 ? NB : 1], weights[NP == 1 ? NB : 1];
@@ -292,8 +315,10 @@ __device__ __forceinline__ void load_row(Row<NB, NP> &row, const T *q, bool vali
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-      split_pair<NP>(x[b][i] * into, x[b][i + 1] * into, row.q[b], i);
-      sum += static_cast<float>(row.q[b][0][i]) + static_cast<float>(row.q[b][0][i + 1]);
+      // Quants::keys: a sixteenth, whose own range still ends 2^-20 below the largest
+      const float fours = NP == 1 && (i & 2) ? 0x1p-4f : 1.0f;
+      split_pair<NP>(x[b][i] * (into * fours), x[b][i + 1] * (into * fours), row.q[b], i);
+      sum += (static_cast<float>(row.q[b][0][i]) + static_cast<float>(row.q[b][0][i + 1])) / fours;
     }
     if constexpr (NP == 1) {
       const float c = row_sum(sum) * -0x1p-21f;
@@ -334,7 +359,7 @@ __device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], b
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const uint32_t w = t[h].k.v[b];
-      const f16x8 keys = row.quants(w, w >> 4, w >> 8, w >> 12);
+      const f16x8 keys = row.quants.keys(w);
       f32x4 s;
       if constexpr (NP == 1) {
         s = mfma(keys, row.q[b][0], row.start[b]);
@@ -395,10 +420,6 @@ __device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], b
     p[i] = exp2_fast(fmaf(z[i], row.unit, row.base));
     row.l += p[i];
   }
-  f16x2 ph[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    ph[i] = f16x2{static_cast<_Float16>(p[2 * i]), static_cast<_Float16>(p[2 * i + 1])};
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     f16x8 w[NP];
@@ -406,7 +427,7 @@ __device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], b
     for (int i = 0; i < 8; i += 2) {
       const uint32_t *d = t[i >> 2].vs.v + 2 * b;
       if constexpr (NP == 1) {
-        const f16x2 x = ph[i / 2] * __builtin_bit_cast(f16x2, d[(i & 3) / 2]);
+        const f16x2 x = times_pair(p[i], p[i + 1], d[(i & 3) / 2]);
         w[0][i] = x[0];
         w[0][i + 1] = x[1];
       } else {
@@ -415,14 +436,15 @@ __device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], b
     }
     if constexpr (NP == 1)
       row.weights[b] = mfma(f16x8{1, 1, 1, 1, 1, 1, 1, 1}, w[0], row.weights[b]);
+    const int at = 8 * (b & 1);
+    const uint32_t *v0 = t[0].v.v + (b & ~1), *v1 = t[1].v.v + (b & ~1);
+    const uint32_t v[4] = {v0[0] >> at, v0[1] >> at, v1[0] >> at, v1[1] >> at};
+    const f16x8 low = row.quants.template values<false>(v[0], v[1], v[2], v[3]);
+    const f16x8 high = row.quants.template values<true>(v[0], v[1], v[2], v[3]);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int at = 4 * (2 * (b & 1) + half);
-      const uint32_t *v0 = t[0].v.v + (b & ~1), *v1 = t[1].v.v + (b & ~1);
-      const f16x8 values = row.quants(v0[0] >> at, v0[1] >> at, v1[0] >> at, v1[1] >> at);
-#pragma unroll
-      for (int s = 0; s < NP; ++s)
-        row.o[2 * b + half] = mfma(values, w[s], row.o[2 * b + half]);
+    for (int s = 0; s < NP; ++s) {
+      row.o[2 * b] = mfma(low, w[s], row.o[2 * b]);
+      row.o[2 * b + 1] = mfma(high, w[s], row.o[2 * b + 1]);
     }
   }
 }
@@ -683,10 +705,11 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16
 
     // to plain units, then the waves' parts together, a share of the elements a wave
     row.l = row_sum(row.l);
-    if constexpr (NP == 1) {
 #pragma unroll
-      for (int i = 0; i < 2 * NB; ++i)
-        row.o[i] = row.o[i] * 0x1p24f - 8.0f * row.weights[i / 2];
+    for (int i = 0; i < 2 * NB; ++i) {
+      row.o[i] *= (NP == 1 ? 0x1p24f : 1.0f) * (i & 1 ? 0x1p-4f : 1.0f);
+      if constexpr (NP == 1)
+        row.o[i] -= 8.0f * row.weights[i / 2];
     }
     rescale(row, exp2_fast(-shift_of(row.level)));
     __syncthreads();  // all have read their rings
@@ -1127,8 +1150,15 @@ attn_q4_0_tiles(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
           const float p0 = exp2_fast(fmaf(z[i], u, base)), p1 = exp2_fast(fmaf(z[i + 1], u, base));
-          l += p0 + p1;
           split_pair<NP>(p0, p1, w[i >> 3], i & 7);
+          // one part: the sum of the rounded weights, so that a row of few tokens divides by what its
+          // values were multiplied with
+          if constexpr (NP == 1) {
+            const f16x8 &x = w[i >> 3][0];
+            l = __builtin_amdgcn_fdot2(f16x2{x[i & 7], x[(i & 7) + 1]}, f16x2{1, 1}, l, false);
+          } else {
+            l += p0 + p1;
+          }
         }
       };
       const auto add_values = [&](const f16x8 (&w)[2][NP], int sub) {
