@@ -114,3 +114,27 @@ def test_value_scales_that_are_not_finite(hip, dev, elem, dim, bad):
     got[at:, :, hit] = want[at:, :, hit]
     # a step that holds such a scale takes its values by another way: their own rounding at most
     assert (np.abs(got - want) <= 2 * s.tolerance(want)).all()
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+def test_many_prompts(hip, dev, elem):
+    """More requests than a wave has lanes, their tiles from none to several."""
+    n = 140
+    rng = np.random.default_rng(14)
+    added = [int(x) for x in rng.integers(0, 60, n)]
+    added[::9] = [0] * len(added[::9])
+    added[70], added[130] = 150, 1
+    lengths = [a + int(x) for a, x in zip(added, rng.integers(0, 120, n))]
+    s = Setup(dev, elem, lengths, added, 4, 1, 64, 16, seed=15)
+    s.check(hip)
+    s.check(hip, window=50)
+
+
+@pytest.mark.parametrize("requests", [3, 70])
+def test_chunks_in_parts_beside_short_ones(hip, dev, requests):
+    """Parts by the longest request, which the others have fewer of."""
+    lengths = [2100] + [30 + 7 * r for r in range(requests - 1)]
+    added = [64] + [20] * (requests - 1)
+    s = Setup(dev, "f32", lengths, added, 2, 1, 64, 16, seed=16)
+    s.check(hip)
+    s.check(hip, causal=False)

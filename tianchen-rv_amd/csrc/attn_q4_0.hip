@@ -49,13 +49,15 @@ struct AttnArgs {
   // workspace: outputs of parts of rows, [part][head_dim], then their maxima and sums, [part][2]; for
   // the kernel of many rows part [split][token][head], for that of few [work-group][2][row of a tile]
   float *parts;
-  uint4 *plan;  // workspace, for the kernel of few rows: a work-group's tile that others end
+  // workspace; for the kernel of few rows a work-group's tile that others end, for that of many the
+  // tokens of a part
+  uint4 *plan;
   size_t q_token, q_head, out_token, out_head;
   size_t table_stride;
   uint32_t table_tokens, window;  // tokens of a table's row; 0: no window
   uint32_t pages, page_size, tokens, heads, share, tiles, max_added, max_length;
   uint32_t few_least, few_most;  // the kernel at hand serves requests of so many rows a kv head
-  uint32_t split_tokens, splits;
+  uint32_t splits;  // many rows: parts of a tile, at most
   uint32_t requests, groups, unit_shift;  // few rows: work-groups that share out the work, 0: one a tile
   float scale;
   int causal;
@@ -481,7 +483,7 @@ struct Span {
 // in parts.  Where the line is too short for that, a part of kLeast units or less is a stretch of its own.
 // Against equal parts of the longest request, most of which the others leave empty: 64 requests of 1024
 // to 8192 tokens 99 -> 82 us, of head_dim 256 129 -> 86 (48 requests), f32 and 32 of up to 4096 51 -> 43.
-constexpr uint32_t kStart = 3, kLeast = 2;
+constexpr uint32_t kCus = 256, kStart = 3, kLeast = 2;
 struct Work {
   uint32_t items, units;  // tiles times kv heads, units of each
   __device__ Work(const AttnArgs &a, const Span &span) : items(0), units(1) {
@@ -515,6 +517,21 @@ __device__ __forceinline__ uint32_t lane_sums(uint32_t x) {
   x = dpp_add<0x118, 0xf>(x);
   x = dpp_add<0x142, 0xa>(x);  // the line before's last
   return dpp_add<0x143, 0xc>(x);
+}
+
+template <int kControl, int kLines> __device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
+  return max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), kControl,
+                                                                  kLines, 0xf, false)));
+}
+
+// The largest so far; the last lane has that of all.
+__device__ __forceinline__ uint32_t lane_maxima(uint32_t x) {
+  x = dpp_max<0x111, 0xf>(x);
+  x = dpp_max<0x112, 0xf>(x);
+  x = dpp_max<0x114, 0xf>(x);
+  x = dpp_max<0x118, 0xf>(x);
+  x = dpp_max<0x142, 0xa>(x);
+  return dpp_max<0x143, 0xc>(x);
 }
 
 __device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) {
@@ -813,6 +830,110 @@ template <int NP> __device__ __forceinline__ void scaled(uint32_t w, f16x2 d, ui
     part[1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, d, -hi));
 }
 
+// What a work-group of the kernel below takes: a part of the steps of a tile.
+struct Piece {
+  uint32_t request, tile, kv_head, split;
+  int part_tokens;  // 0: all of the tile's
+};
+
+// The w-th piece of the requests' work; false past the last.  Pieces have no gaps, since consecutive
+// work-groups go to the XCDs and then to the groups of CUs in turn: where those of a request with fewer
+// tiles than the longest one has ended at once, the working ones kept meeting in the same CUs.  The parts'
+// length goes by the lengths of all requests: of the ways to cut the longest one into up to a.splits parts
+// the one whose work-groups are done first, one a CU at a time; a part takes kPartFill steps' time more
+// than its steps (a work-group's beginning and end, 9 us beside 3.4 a step), and the joining of parts
+// kPartJoin.  Both together (us, f16, 8 kv heads of 128, against a grid of all tiles that there might be
+// in equal parts of the longest request): 4 requests with up to 512 new tokens on up to 4096 224 -> 178, 20
+// with up to 400 on 1000 147 -> 120, one with 256 on 8192 98 -> 83; 16 of 200 on 2000 with a window, f32,
+// 2 kv heads of 64, 72 -> 50; one of 2048 alone, whose tiles see 1 to 32 steps, 100 -> 101.
+constexpr uint32_t kPartFill = 5, kPartJoin = 2;
+
+template <uint32_t kTileRows, uint32_t kTokens>
+__device__ __forceinline__ bool find_piece(const AttnArgs &a, uint32_t w, int lane, Piece &piece) {
+  const uint32_t kv_heads = a.heads / a.share;
+  // of the lane's request: tiles times kv heads, the last tile's steps and the first one's
+  uint32_t items = 0, steps = 1, steps0 = 1;
+  const auto look = [&](uint32_t base) __attribute__((always_inline)) {
+    items = 0;
+    steps = steps0 = 1;
+    if (base + lane < a.requests) {
+      const Span span(a, base + lane);
+      if (span.rows >= max(a.few_least, 1u) && span.rows <= a.few_most) {
+        items = (span.rows + kTileRows - 1) / kTileRows * kv_heads;
+        const int low = span.lo(a, 0) & -kStep, seen = span.hi(a, span.added - 1) - low;
+        const int seen0 = span.hi(a, min(kTileRows - 1, span.rows - 1) / a.share) - low;
+        steps = seen > 0 ? (seen - 1) / kTokens + 1 : 1;
+        steps0 = seen0 > 0 ? (seen0 - 1) / kTokens + 1 : 1;
+      }
+    }
+  };
+  look(0);
+  uint32_t part = 0;
+  if (a.splits > 1) {
+    uint32_t longest = 1;
+    for (uint32_t base = 0;;) {
+      longest = max(longest, items ? steps : 1);
+      base += 64;
+      if (base >= a.requests)
+        break;
+      look(base);
+    }
+    longest = lane_of(lane_maxima(longest), 63);
+    // a way a lane: the longest in lane + 1 parts.  Numbers of work-groups as floats, near enough.
+    part = (longest + lane) / (lane + 1);
+    const float parts = 1.0f / static_cast<float>(part);
+    float groups = 0.0f, work = 0.0f;
+    bool alike = true;  // the tiles of each request, but for a quarter
+    for (uint32_t base = 0; base < a.requests; base += 64) {
+      if (a.requests > 64)
+        look(base);
+      for (uint32_t r = 0; r < min(a.requests - base, 64u); ++r) {
+        const uint32_t last = lane_of(steps, r), first = lane_of(steps0, r);
+        const float n = lane_of(items, r), mean = 0.5f * (last + first);
+        const bool even = 4 * first >= 3 * last;
+        alike = alike && (even || n == 0.0f);
+        work += n * mean;
+        groups += n * (even ? ceilf(last * parts - 0x1p-10f) : fmaxf(mean * parts + 0.5f, 1.0f));
+      }
+    }
+    // alike they run in rounds of the CUs, else one after the other with the longest at the end
+    const float one = static_cast<float>(part + kPartFill);
+    const float cost = (lane ? kPartJoin : 0) +
+                       (alike ? ceilf(groups * (1.0f / kCus)) * one
+                              : fmaxf((work + kPartFill * groups) * (1.0f / kCus) + 0.4f * one, one));
+    // the least of them, and of equal ones the fewest parts; costs are not negative: their bits order
+    const uint32_t order =
+        lane < static_cast<int>(a.splits) ? ~__builtin_bit_cast(uint32_t, cost) : 0;
+    const uint64_t best = __ballot(order == lane_of(lane_maxima(order), 63));
+    part = lane_of(part, __builtin_ctzll(best));
+    if (a.requests > 64)
+      look(0);
+  }
+  uint32_t before = 0;
+  for (uint32_t base = 0;;) {
+    const uint32_t pieces = items * (part ? (steps - 1) / part + 1 : 1);
+    const uint32_t sum = lane_sums(pieces), from = before + sum - pieces;
+    const uint64_t here = __ballot(w - from < pieces);
+    if (here) {
+      const int owner = __builtin_ctzll(here);
+      const uint32_t of_tile = lane_of(items, owner), at = w - lane_of(from, owner);
+      piece.request = base + owner;
+      piece.split = at / of_tile;
+      const uint32_t rest = at - piece.split * of_tile;
+      // the last tiles of a prompt see the most tokens: they go first
+      piece.tile = of_tile / kv_heads - 1 - rest / kv_heads;
+      piece.kv_head = rest % kv_heads;
+      piece.part_tokens = static_cast<int>(part * kTokens);
+      return true;
+    }
+    before += lane_of(sum, 63);
+    base += 64;
+    if (base >= a.requests)
+      return false;
+    look(base);
+  }
+}
+
 template <int NB, int NP, typename T>
 __global__ __launch_bounds__((TileStep<NB, NP>::kThreads), (TileStep<NB, NP>::kWaves / 4)) void
 attn_q4_0_tiles(AttnArgs a) {
@@ -821,22 +942,29 @@ attn_q4_0_tiles(AttnArgs a) {
   __shared__ __align__(16) uint8_t s_step[2][S::kBytes];
   __shared__ uint32_t s_flags[2][S::kWaves];
   __shared__ uint32_t s_bad[2][NB][kTokens / 32];
-  // the last tiles of a prompt see the most tokens: they go first
-  const uint32_t kv_heads = a.heads / a.share, kv_head = blockIdx.x % kv_heads;
-  const uint32_t tile = a.tiles - 1 - blockIdx.y, split = blockIdx.z;
-  const uint32_t request = blockIdx.x / kv_heads;
-  const Span span(a, request);
-  if (tile * S::kRows >= span.rows || span.rows < a.few_least || span.rows > a.few_most)
+  Piece mine;
+  if (!find_piece<S::kRows, kTokens>(a, blockIdx.x, threadIdx.x & 63, mine))
     return;
+  const uint32_t kv_heads = a.heads / a.share, kv_head = mine.kv_head;
+  const uint32_t tile = mine.tile, split = mine.split, request = mine.request;
+  const Span span(a, request);
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t last = span.rows - 1;
   const uint32_t i0 = tile * S::kRows / a.share;
   const uint32_t i1 = min(tile * S::kRows + S::kRows - 1, last) / a.share;
-  const int begin = (span.lo(a, i0) & -kStep) + static_cast<int>(split * a.split_tokens);
-  const int end = min(span.hi(a, i1), begin + static_cast<int>(a.split_tokens));
-  if (split && begin >= end)
-    return;
+  int begin = span.lo(a, i0) & -kStep, end = span.hi(a, i1);
+  bool cut = false;
+  if (mine.part_tokens) {
+    const int part = mine.part_tokens;
+    if (threadIdx.x == 0)
+      a.plan[0].x = static_cast<uint32_t>(part);  // the same from all
+    cut = end - begin > part;
+    if (split && (!cut || (end - begin - 1) / part < static_cast<int>(split)))
+      return;
+    begin += static_cast<int>(split) * part;
+    end = min(end, begin + part);
+  }
   const int steps = begin < end ? (end - begin + kTokens - 1) / kTokens : 0;
 
   // the wave's rows, and what they see
@@ -1221,11 +1349,11 @@ attn_q4_0_tiles(AttnArgs a) {
       next_step(n);
   }
 
-  if (row0 > last && a.splits > 1)
+  if (row0 > last && cut)
     return;
   const float sum = sum_of(with_lane32(l));
   const float out_unit = exp2_fast(was_big ? 4.0f : -11.0f);
-  if (a.splits > 1) {
+  if (cut) {
     if (!valid)
       return;
     const size_t at = (static_cast<size_t>(split) * a.tokens + token) * a.heads + head;
@@ -1257,19 +1385,25 @@ attn_q4_0_tiles(AttnArgs a) {
     }
   }
   const int rows = static_cast<int>(min(last + 1 - min(row0, last + 1), 32u));
-#pragma unroll 4
-  for (int i = lane; i < rows * (D / 4); i += 64) {
-    const uint32_t at = row0 + i / (D / 4), e = 4 * (i % (D / 4));
-    T *p = static_cast<T *>(a.out) + static_cast<size_t>(span.first + at / a.share) * a.out_token +
-           static_cast<size_t>(kv_head * a.share + at % a.share) * a.out_head + e;
-    const Values<T, 4> x = *reinterpret_cast<const Values<T, 4> *>(
-        rows_at + i / (D / 4) * kRowBytes + e * sizeof(T));
-    if (a.out_vec) {
-      *reinterpret_cast<Values<T, 4> *>(p) = x;
-    } else {
+  // where a row goes, from the lane that has had it
+  const size_t out_at = static_cast<size_t>(token) * a.out_token + static_cast<size_t>(head) * a.out_head;
+  const int out_low = static_cast<int>(out_at), out_high = static_cast<int>(out_at >> 32);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        p[k] = x.v[k];
+  for (int first = 0; first < 32 * (D / 4); first += 64) {
+    const int i = first + lane, at = i / (D / 4), e = 4 * (i % (D / 4));
+    const uint32_t low = static_cast<uint32_t>(__shfl(out_low, at & 31));
+    const uint32_t high = static_cast<uint32_t>(__shfl(out_high, at & 31));
+    if (at < rows) {
+      T *p = static_cast<T *>(a.out) + (static_cast<size_t>(high) << 32 | low) + e;
+      const Values<T, 4> x =
+          *reinterpret_cast<const Values<T, 4> *>(rows_at + at * kRowBytes + e * sizeof(T));
+      if (a.out_vec) {
+        *reinterpret_cast<Values<T, 4> *>(p) = x;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          p[k] = x.v[k];
+      }
     }
   }
 }
@@ -1376,7 +1510,10 @@ __global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join(AttnArgs a, uint3
   const uint32_t row0 = (i * a.share + head % a.share) / tile_rows * tile_rows;
   const uint32_t i0 = row0 / a.share, i1 = min(row0 + tile_rows - 1, span.rows - 1) / a.share;
   const int tokens = max(span.hi(a, i1) - (span.lo(a, i0) & -kStep), 1);
-  const uint32_t splits = min((tokens + a.split_tokens - 1) / a.split_tokens, a.splits);
+  const uint32_t part_tokens = a.plan[0].x;
+  const uint32_t splits = min((tokens + part_tokens - 1) / part_tokens, a.splits);
+  if (splits == 1)
+    return;  // whole, of all rows of the tile
   const size_t row = static_cast<size_t>(token) * a.heads + head;
   const size_t stride = static_cast<size_t>(a.tokens) * a.heads;
   const float2 *const ml =
@@ -1466,8 +1603,9 @@ constexpr size_t kWholeTokens = 2560;
 
 struct Plan {
   size_t tile_rows, tiles, workspace;
-  size_t splits, split_tokens;        // many rows
-  size_t groups, unit_shift, launch;  // few rows: shares (0: a tile a work-group), work-groups
+  size_t splits;                      // many rows
+  size_t groups, unit_shift;          // few rows: shares (0: a tile a work-group)
+  size_t launch;                      // work-groups
 };
 
 size_t parts_bytes(size_t parts, size_t head_dim) {
@@ -1502,29 +1640,32 @@ Plan few_plan(size_t requests, size_t max_added, size_t max_length, size_t windo
   return p;
 }
 
-// Work-groups of one tile each, as many as the card runs at a time; the tokens of fewer tiles are
-// split into parts of at least 512 tokens.
+// Tiles that may be fewer than kMostParts work-groups are cut into parts of 256 tokens and more, which the
+// kernel chooses by the requests' lengths.
+constexpr size_t kMostParts = 768, kLeastPart = 256;
+
 Plan many_plan(int elem, size_t requests, size_t tokens, size_t max_added, size_t max_length,
                size_t window, size_t heads, size_t kv_heads, size_t head_dim) {
   const size_t share = heads / kv_heads;
   Plan p{};
   p.tile_rows = many_rows(elem, head_dim);
   p.tiles = (max_added * share + p.tile_rows - 1) / p.tile_rows;
-  const size_t groups = requests * p.tiles * kv_heads;
+  // as many tiles as full ones, and one that is not a request
+  const size_t groups =
+      std::min(requests * p.tiles, tokens * share / p.tile_rows + requests) * kv_heads;
   const auto parts_of = [&](size_t seen) {
-    const size_t most = std::max((seen + 511) / 512, size_t{1});
-    return std::min(std::max((512 + groups - 1) / groups, size_t{1}), most);
+    const size_t most = std::max((seen + kLeastPart - 1) / kLeastPart, size_t{1});
+    return std::min(std::min(std::max(kMostParts / groups, size_t{1}), most), size_t{64});
   };
   // what a tile sees begins at a multiple of 32; `window` is 0 where it does not bound that
   size_t seen = max_length + 31;
   if (window && window < seen)
     seen = std::min(seen, window + p.tile_rows / share + 34);
-  const size_t parts = parts_of(seen);
-  p.split_tokens = parts == 1 ? seen : ((seen + parts - 1) / parts + 127) / 128 * 128;
-  p.splits = (seen + p.split_tokens - 1) / p.split_tokens;
+  p.splits = parts_of(seen);
+  p.launch = groups * p.splits;
   // for any window: a smaller one has no more parts
   const size_t most = parts_of(max_length + 31);
-  p.workspace = most == 1 ? 0 : parts_bytes(most * tokens * heads, head_dim);
+  p.workspace = most == 1 ? 0 : sizeof(uint4) + parts_bytes(most * tokens * heads, head_dim);
   return p;
 }
 
@@ -1586,7 +1727,7 @@ void launch_tiles(const AttnArgs &a, size_t head_dim, dim3 grid, hipStream_t st)
 template <int NP, typename T>
 void launch_all(AttnArgs a, Kernels k, const Plan &few, const Plan &many, size_t head_dim,
                 size_t requests, hipStream_t st) {
-  const unsigned kv_heads = a.heads / a.share, n = static_cast<unsigned>(requests);
+  const unsigned n = static_cast<unsigned>(requests);
   float *const workspace = a.parts;
   const uint32_t few_most = !k.few ? 0 : k.many ? static_cast<uint32_t>(k.few_rows) : 0xffffffffu;
   const uint32_t dim = static_cast<uint32_t>(head_dim);
@@ -1608,13 +1749,13 @@ void launch_all(AttnArgs a, Kernels k, const Plan &few, const Plan &many, size_t
     }
   }
   if (k.many) {
-    a.parts = workspace + (k.few ? few.workspace / sizeof(float) : 0);
+    a.plan = reinterpret_cast<uint4 *>(workspace + (k.few ? few.workspace / sizeof(float) : 0));
+    a.parts = reinterpret_cast<float *>(a.plan + 1);
     a.tiles = static_cast<uint32_t>(many.tiles);
-    a.split_tokens = static_cast<uint32_t>(many.split_tokens);
     a.splits = static_cast<uint32_t>(many.splits);
     a.few_least = few_most ? few_most + 1 : 0;
     a.few_most = 0xffffffffu;
-    launch_tiles<NP, T>(a, head_dim, dim3(n * kv_heads, a.tiles, a.splits), st);
+    launch_tiles<NP, T>(a, head_dim, dim3(static_cast<unsigned>(many.launch)), st);
     if (many.splits > 1) {
       const uint32_t tile_rows = static_cast<uint32_t>(many.tile_rows);
       const uint32_t groups = tcrv::kJoinThreads / (dim / 4);
@@ -1697,7 +1838,7 @@ int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
   const Plan many =
       many_plan(elem, requests, tokens, max_added, max_length, bound, heads, kv_heads, head_dim);
   if ((k.few && requests * few.tiles * kv_heads > 0x7fffffffu) ||
-      (k.many && (many.splits > 65535u || many.tiles > 65535u || requests * kv_heads > 0x7fffffffu)))
+      (k.many && many.launch > 0x7fffffffu))
     return TCRV_HIP_ERR_TOO_LARGE;
   const size_t need = (k.few ? few.workspace : 0) + (k.many ? many.workspace : 0);
   if (need) {
@@ -1732,7 +1873,6 @@ int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
              0,  // the plans': launch_all
              static_cast<uint32_t>(max_added),
              static_cast<uint32_t>(max_length),
-             0,
              0,
              0,
              0,
