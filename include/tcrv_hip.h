@@ -508,15 +508,21 @@ TCRV_HIP_API int tcrv_hip_kv_load_q4_0(int elem, const uint8_t *cache, size_t pa
  * A row that sees no token is zero.  What the cache holds in places that a row
  * does not see (tokens past the length, infinities and NaN among them) does not
  * reach it; a page outside 0 .. pages - 1 holds no token.  Rows that hold a NaN
- * or infinity are NaN.  f32 rows: queries and weights enter the matrix cores as
- * two f16 parts each (22 bits); f16 and bf16 rows: queries exactly, weights as
- * f16.  out's rows past first[requests] are not written; out must not overlap q.
- * max_added and max_length are the caller's bounds on added tokens and lengths
- * (they size the launch): further rows are not written, further tokens not read.
+ * or infinity are NaN; a row that sees a value scale which is not finite is not
+ * finite in that block.  f32 rows: queries and weights, and values of prompts,
+ * enter the matrix cores as two f16 parts each (22 bits).  f16 and bf16 rows:
+ * queries down to 2^-20 of the row's largest, weights as f16, in prompts values
+ * as f16; keys always with all of their bits.  out's rows past first[requests]
+ * are not written; out must not overlap q.
+ * max_added and max_length (at most 2^30, else TCRV_HIP_ERR_TOO_LARGE) are the
+ * caller's bounds on added tokens and lengths (they size the launch): further
+ * rows are not written, further tokens not read.  How contexts are cut over
+ * work-groups, and with it the results' last bits, follows the lengths of all
+ * requests; the same call gives the same bits.
  * The workspace (device, 16-byte aligned, at least ..._workspace_bytes of the same
- * arguments) joins the parts of long contexts; 0 bytes where none is needed, when
- * `workspace` may be NULL.  What it holds after a call is unspecified; calls that
- * share one must be ordered (one stream). */
+ * arguments) holds the parts of what is cut until they are joined; 0 bytes where
+ * nothing is, when `workspace` may be NULL.  What it holds after a call is
+ * unspecified; calls that share one must be ordered (one stream). */
 TCRV_HIP_API size_t tcrv_hip_attn_q4_0_workspace_bytes(int elem, size_t requests, size_t tokens,
                                                        size_t max_added, size_t max_length,
                                                        size_t heads, size_t kv_heads,

@@ -10,10 +10,16 @@
 // register each.
 //
 // A dword of 8 quants becomes four operand registers.  4 bits n at the bottom of a half are the f16
-// denormal n 2^-24: three shifts and four ands, and the offset -8 comes in with the keys' start value
-// and goes out with the sums of the values' weights.  The product aligns denormals by their exponent
-// field, which costs it 3 bits of 24: nothing beside 16-bit rows (one part), but f32 rows (two parts)
-// take n over the bits of 1024.0, which is 1024 + n, and subtract 1032.
+// denormal n 2^-24, those above them 16 n 2^-24: a shift and four ands, and the offset -8 comes in with
+// the keys' start value and goes out with the sums of the values' weights.  The product aligns denormals by
+// their exponent field, which costs it 3 bits of 24: nothing beside 16-bit rows (one part), but f32 rows
+// (two parts) take n over the bits of 1024.0, which is 1024 + n, and subtract 1032.
+//
+// Few rows are bound by the read of the cache, 9/8 byte an element of a kv head and token, and the
+// instructions that make operands of it: two contexts of 131072 tokens, bf16, 32 query and 8 kv heads of
+// 128, 54 us and 6.6 for the join (264 MB, 4.9 TB/s without it); 64 requests of 1024 to 8192, f16, 77 and
+// 5.3 (334 MB, 4.3 TB/s).  A wave reads its steps through an LDS ring of its own, so that
+// no register waits for them.
 #include <algorithm>
 
 #include "kv_cache.h"
@@ -786,6 +792,10 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16
 // A key is two f16 parts, which hold all of its 15 bits: a score's error would grow with the score.
 // f16 and bf16 rows take values and weights as one part each; for f32 rows queries, values and weights
 // are two parts as well, and a product three: the larger parts', and the mixed ones.
+// A prompt of 4096, f16, 32 query and 8 kv heads of 128: 223 us, 620 TFLOP/s, a step of 64 tokens 3.4 us, of
+// which the matrix instructions are 1.6 and the others and LDS as much each: eight waves, two a SIMD, meet at
+// every step and overlap no more.  Of head_dim 64 and f32 a step is 5 us; two work-groups a CU there (128
+// registers) spilled and took 74 us in 9 chunks where one takes 74.
 // ---------------------------------------------------------------------------
 using f32x16 = float __attribute__((ext_vector_type(16)));
 

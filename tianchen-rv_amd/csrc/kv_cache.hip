@@ -10,7 +10,8 @@ namespace {
 // the sums.  All work-groups form the sums of all requests for themselves, kTableThreads requests
 // at a time, and share out the tokens and the new pages: one launch, no order between work-groups.
 // A slot in a new page is formed from free_pages itself, so that it does not wait for the table's
-// entry, which another work-group writes.
+// entry, which another work-group writes.  64 requests of a token each 4.5 us, 301 of up to 700 tokens
+// 6.8: a launch and four loads that follow one another.
 // ---------------------------------------------------------------------------
 constexpr int kTableThreads = 256;
 constexpr int kTableWaves = kTableThreads / 64;
@@ -131,6 +132,10 @@ __global__ __launch_bounds__(kTableThreads) void kv_tables(TablesArgs a) {
 // The store.  Bound by memory: keys and values read once, 9/16 byte an element written.  A block
 // of 32 elements is 8 lanes of 4 (as in quantize_q8_0), a row of 16 lanes two blocks: the nibbles
 // of a byte meet by a move of 4 lanes, and the two bytes of a unit of the values by one of 8.
+// A work-group takes a token: 8191 tokens x 8 heads x 128, f32, 26 us (77 MB, 2.9 TB/s), what is left
+// being the slot's, the position's and the table row's latency before 9 KB of work.  Four tokens a
+// work-group, whose bytes leave 8 at a time, took 32 to 35 us, an item's loads sent before the one before
+// it is worked on 33.
 // ---------------------------------------------------------------------------
 struct StoreArgs {
   const void *k, *v;
@@ -305,7 +310,8 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_q4_0(StoreArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// The reading back: (q - 8) d is exact in f32.  The lanes' places as in the store.
+// The reading back: (q - 8) d is exact in f32.  The lanes' places as in the store; 8191 tokens as there
+// 27 us (77 MB).
 // ---------------------------------------------------------------------------
 struct LoadArgs {
   const uint8_t *cache;
