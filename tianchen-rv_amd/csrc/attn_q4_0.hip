@@ -1139,12 +1139,15 @@ attn_q4_0_tiles(AttnArgs a) {
   static_assert(S::kWaves * 32 * kRowBytes <= 2 * S::kBytes, "");
   uint8_t *const rows_at = &s_step[0][0] + wave * 32 * kRowBytes;
   if (row0 <= last) {
-#pragma unroll 4
-    for (int i = lane; i < 32 * (D / 4); i += 64) {
-      const uint32_t at = min(row0 + i / (D / 4), last), e = 4 * (i % (D / 4));
-      const T *p = static_cast<const T *>(a.q) +
-                   static_cast<size_t>(span.first + at / a.share) * a.q_token +
-                   static_cast<size_t>(kv_head * a.share + at % a.share) * a.q_head + e;
+    // where a row lies, from the lane that has it
+    const size_t q_at = static_cast<size_t>(token) * a.q_token + static_cast<size_t>(head) * a.q_head;
+    const int q_low = static_cast<int>(q_at), q_high = static_cast<int>(q_at >> 32);
+#pragma unroll 8
+    for (int first = 0; first < 32 * (D / 4); first += 64) {
+      const int at = (first + lane) / (D / 4), e = 4 * ((first + lane) % (D / 4));
+      const uint32_t low = static_cast<uint32_t>(__shfl(q_low, at));
+      const uint32_t high = static_cast<uint32_t>(__shfl(q_high, at));
+      const T *p = static_cast<const T *>(a.q) + (static_cast<size_t>(high) << 32 | low) + e;
       Values<T, 4> x;
       if (a.q_vec) {
         x = *reinterpret_cast<const Values<T, 4> *>(p);
@@ -1153,7 +1156,7 @@ attn_q4_0_tiles(AttnArgs a) {
         for (int k = 0; k < 4; ++k)
           x.v[k] = p[k];
       }
-      *reinterpret_cast<Values<T, 4> *>(rows_at + i / (D / 4) * kRowBytes + e * sizeof(T)) = x;
+      *reinterpret_cast<Values<T, 4> *>(rows_at + at * kRowBytes + e * sizeof(T)) = x;
     }
   }
   // a wave reads only what it wrote
