@@ -57,7 +57,7 @@ def test_nothing_to_do_launches_nothing(elem):
 
 @pytest.mark.parametrize("requests,tokens,added,heads,kv,dim", [
     (1, 1, 1, 32, 8, 128), (64, 64, 1, 32, 8, 128), (5, 700, 300, 14, 2, 64), (3, 90, 30, 16, 4, 256),
-    (200, 200, 1, 16, 2, 192), (1, 2000, 2000, 8, 8, 128),
+    (200, 200, 1, 10, 2, 192), (1, 2000, 2000, 8, 8, 128),
 ])
 @pytest.mark.parametrize("length", [1, 257, 4000, 131072, 1 << 30])
 def test_workspace_serves_every_window(requests, tokens, added, heads, kv, dim, length):
