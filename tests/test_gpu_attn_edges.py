@@ -1,0 +1,62 @@
+"""attn_q4_0 where a row sees little or what it sees is uneven.  Oracle and, where not said otherwise,
+tolerances: those of test_gpu_kv_cache.Setup (float64)."""
+import numpy as np
+import pytest
+
+from test_gpu_kv_cache import ELEMS, Setup, wide
+
+pytestmark = pytest.mark.gpu
+
+
+# ----------------------------------------------------------- missing pages ---
+
+def attend_there(q, keys, vals, position0, scale, causal, window, there):
+    """kv_plain.attend with the tokens alone that `there` holds, for all rows of a head at once."""
+    added, heads, dim = q.shape
+    length, kv, _ = keys.shape
+    at, t = position0 + np.arange(added)[:, None], np.arange(length)[None]
+    seen = np.broadcast_to(there, (added, length)).copy()
+    if causal:
+        seen &= t <= at
+    if window:
+        seen &= t > at - window
+    out = np.zeros((added, heads, dim))
+    some = seen.any(1)
+    for h in range(heads):
+        z = scale * (q[:, h].astype(np.float64) @ keys[:, h * kv // heads].T)
+        z = np.where(seen, z, -np.inf)[some]
+        w = np.exp(z - z.max(1, keepdims=True))
+        out[some, h] = w @ vals[:, h * kv // heads] / w.sum(1, keepdims=True)
+    return out, some
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("lengths,added,heads,kv,page,holes", [
+    # whole tiles; the last page in part, and a request of nothing else
+    ([150, 70, 33], [150, 70, 33], 12, 2, 16, [(0, 3, 4, 9), range(5), ()]),
+    # pages of three halves of a step
+    ([400], [130], 8, 1, 48, [(0, 2, 5, 8)]),
+    # parts of a context
+    ([4500], [20], 2, 1, 16, [(0, 7, *range(100, 121), 130, 281)]),
+    # beside requests of few rows
+    ([2000, 1500, 900, 40], [1, 300, 2, 40], 8, 2, 32, [(1, 2), (0, 30, 46), (5,), (1,)]),
+])
+def test_prompts_with_missing_pages(hip, dev, elem, dim, lengths, added, heads, kv, page, holes):
+    """Tokens of a page outside the cache are not there, in prompts as in single tokens."""
+    s = Setup(dev, elem, lengths, added, heads, kv, dim, page, seed=21)
+    table = s.table.copy()
+    for r, pages in enumerate(holes):
+        for i, page_at in enumerate(pages):
+            table[r, page_at] = -1 if i % 2 == 0 else s.pages
+    for causal, window in ((True, 0), (False, 0), (True, 90), (True, 9)):
+        out = wide(s.run(hip, table=table, causal=causal, window=window))
+        want, some = zip(*(
+            attend_there(s.q[s.first[r]:s.first[r + 1]], s.k[r], s.v[r], lengths[r] - added[r],
+                         np.float64(np.float32(dim ** -0.5)), causal, window,
+                         ~np.isin(np.arange(lengths[r]) // page, list(holes[r])))
+            for r in range(len(lengths))))
+        want, some = np.concatenate(want), np.concatenate(some)
+        off = np.abs(out - want)
+        assert (off <= s.tolerance(want)).all(), (causal, window, off.max())
+        assert (out[~some] == 0.0).all()

@@ -805,6 +805,8 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
 
 constexpr float kTileShift = 10.0f;       // weights: 2^4 2^10, within f16
 constexpr uint32_t kKeyBig = 1, kValueBig = 2, kValueBad = 4;  // a step's scales
+// bit kAbsentAt + i: the page of a step's i-th 16 tokens is not in the cache
+constexpr uint32_t kAbsentAt = 8, kAbsent = 0xfu << kAbsentAt;
 
 template <int NB, int NP> struct TileStep {
   // eight waves, two a SIMD, while a wave's queries and output fit 256 registers; a thread brings a
@@ -1007,6 +1009,7 @@ attn_q4_0_tiles(AttnArgs a) {
                  static_cast<uint32_t>(t) - column * a.page_size};
   };
   Raw<NB> raw;
+  bool absent = false;  // a wave of keys' pieces holds 16 tokens, which lie in one page
   const auto bring = [&](int n, const Place &p) __attribute__((always_inline)) {
     const bool in = p.page < a.pages;
     const uint8_t *at = head_at + (in ? p.page : 0) * page_bytes;
@@ -1019,9 +1022,12 @@ attn_q4_0_tiles(AttnArgs a) {
       raw.q = load_dwords<NB>(at + lay.value(NB, p.token, m, 0));
       raw.d = load_dwords<2 * NB>(at + lay.value_scale(NB, p.token, 0));
     }
-    // tokens that are not there: scales of 0
+    // tokens that are not there: scales of 0, and no scores where it is their page that is missing (those
+    // past the length are hidden by it)
     const int t0 = begin + n * kTokens;
+    absent = false;
     if (t0 + kTokens > span.length || !__all(in)) {
+      absent = __any(!in && t0 + piece_token < span.length);
       const int left = in ? span.length - (t0 + piece_token) : 0;
       if (keys_piece) {
 #pragma unroll
@@ -1039,14 +1045,14 @@ attn_q4_0_tiles(AttnArgs a) {
       }
     }
   };
-  // what the step's scales are, a word a wave
+  // what the step's scales are and which of its pages are missing, a word a wave
   const auto tell = [&](int n) __attribute__((always_inline)) {
     uint32_t any = 0, said = 0;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
       any |= raw.d.v[i];
     if (keys_piece) {
-      said = __any(any & 0x4000u) ? kKeyBig : 0;
+      said = (__any(any & 0x4000u) ? kKeyBig : 0) | (absent ? 1u << (kAbsentAt + wave) : 0);
     } else {
 #pragma unroll
       for (int i = NB; i < 2 * NB; ++i)
@@ -1238,7 +1244,7 @@ attn_q4_0_tiles(AttnArgs a) {
     const float u = unit * (mine & kKeyBig ? 1.0f : 0x1p-15f);
     const int t0 = begin + n * kTokens;
     if (t0 < wave_hi && t0 + kTokens > wave_lo) {
-      const bool edge = t0 < all_lo || t0 + kTokens > all_hi;
+      const bool edge = t0 < all_lo || t0 + kTokens > all_hi || (mine & kAbsent) != 0;
       // 32 tokens' scores
       const auto scores = [&](int sub) __attribute__((always_inline)) {
         __builtin_amdgcn_s_setprio(1);
@@ -1264,7 +1270,8 @@ attn_q4_0_tiles(AttnArgs a) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int at = 8 * (i >> 2) + (i & 3);
-            z[i] = at >= lo_at && at < hi_at ? z[i] : kNone;
+            const bool there = !(mine >> (kAbsentAt + 2 * sub + (i >> 3)) & 1u);
+            z[i] = there && at >= lo_at && at < hi_at ? z[i] : kNone;
           }
         }
         float high = z[0];
