@@ -60,3 +60,30 @@ def test_prompts_with_missing_pages(hip, dev, elem, dim, lengths, added, heads, 
         off = np.abs(out - want)
         assert (off <= s.tolerance(want)).all(), (causal, window, off.max())
         assert (out[~some] == 0.0).all()
+
+
+# ------------------------------------------------- rows that are not finite ---
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("length,added", [(90, 90), (20, 30), (9, 4)])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_bad_rows(hip, dev, elem, dim, length, added, bad):
+    """A row that holds an infinity or a NaN is NaN whatever it sees, one token or many, and zero
+    where it sees none; the other rows keep their bits."""
+    s = Setup(dev, elem, [length], [added], 4, 1, dim, 16, seed=22)
+    clean = s.q.copy()
+    place = np.zeros((added, 4), bool)
+    for i in range(added):
+        for h in (1, 3) if i % 3 else (0, 1, 2):
+            s.q[i, h, (11 * i + 17 * h) % dim] = bad
+            place[i, h] = True
+    sees = length - added + np.arange(added) >= 0
+    for window in (0, 1):
+        got = wide(s.run(hip, window=window))
+        kept, s.q = s.q, clean
+        fine = wide(s.run(hip, window=window))
+        s.q = kept
+        assert np.isnan(got[place & sees[:, None]]).all()
+        assert (got[~sees] == 0.0).all()
+        assert np.array_equal(got[~place], fine[~place])

@@ -1177,7 +1177,9 @@ attn_q4_0_tiles(AttnArgs a) {
       if (most > 0.0f && most < __builtin_inff())
         (void)frexpf(most, &e);
       e = min(max(e - 1, -100), 100);
-      sign = ldexpf(sign, -e);
+      // an infinity makes the whole row NaN: its products with a key's two parts may be infinities of
+      // one sign, a score that looks like that of a hidden token
+      sign = most < __builtin_inff() ? ldexpf(sign, -e) : __builtin_nanf("");
       unit = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, e + 4), 0x1p-100f);
     }
 #pragma unroll
