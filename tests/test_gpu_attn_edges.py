@@ -87,3 +87,14 @@ def test_bad_rows(hip, dev, elem, dim, length, added, bad):
         assert np.isnan(got[place & sees[:, None]]).all()
         assert (got[~sees] == 0.0).all()
         assert np.array_equal(got[~place], fine[~place])
+
+
+# -------------------------------------------------------- query magnitudes ---
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+@pytest.mark.parametrize("power", [-122, -105, 105, 122])
+@pytest.mark.parametrize("added", [3, 60])
+def test_queries_of_any_power(hip, dev, elem, power, added):
+    """Rows near either end of the type's range, with the scale that brings their scores back."""
+    s = Setup(dev, elem, [200], [added], 4, 1, 64, 16, seed=23, spread=2.0 ** power)
+    s.check(hip, scale=0.1 * 2.0 ** -power)

@@ -281,6 +281,24 @@ template <int NB, int NP> struct Row {
   int level;            // of the shift
 };
 
+// An exact power of two, 2^-e, brings a row's largest element to 1 .. 2 (to 4 at the range's upper end,
+// to less among f32's subnormals): no f16 part overflows, and what falls below f16's range is 2^-24 of the
+// largest.  The sign of `scale` goes into the queries, so that the unit of the scores is positive and a
+// maximum of products one of scores.
+__device__ __forceinline__ int exponent_of(float top) {
+  int e = 0;
+  if (top > 0.0f && top < __builtin_inff())
+    (void)frexpf(top, &e);
+  return min(max(e - 1, -126), 126);  // either power is a normal f32
+}
+
+// |scale| log2 e 2^e.  Not 0, so that a hidden token's score stays what it is; nor infinite, where the
+// scores may not be: products that differ do so by 2^-72 or more, and a unit of 2^126 as any larger one
+// leaves a weight to the greatest alone.
+__device__ __forceinline__ float unit_of(float scale, int e) {
+  return fminf(fmaxf(ldexpf(fabsf(scale) * kLog2e, e), 0x1p-100f), 0x1p126f);
+}
+
 template <int NB, int NP, typename T>
 __device__ __forceinline__ void load_row(Row<NB, NP> &row, const T *q, bool valid, bool vec, int g,
                                          float scale) {
@@ -308,16 +326,9 @@ __device__ __forceinline__ void load_row(Row<NB, NP> &row, const T *q, bool vali
     }
   }
   top = row_max(top);
-  // an exact power of two brings the largest to 1 .. 2: no f16 part overflows, and what falls below
-  // f16's range is 2^-24 of the largest.  The sign of `scale` goes into the queries, so that unit
-  // >= 0 and a maximum of products is one of scores.
-  int e = 0;
-  if (top > 0.0f && top < __builtin_inff())
-    (void)frexpf(top, &e);
-  e = min(max(e - 1, -100), 100);
+  const int e = exponent_of(top);
   const float into = ldexpf(scale < 0.0f ? -1.0f : 1.0f, -e);
-  // not 0, so that a hidden token's score stays what it is
-  row.unit = fmaxf(ldexpf(fabsf(scale) * kLog2e, NP == 1 ? e + 24 : e), 0x1p-100f);
+  row.unit = unit_of(scale, NP == 1 ? e + 24 : e);
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     float sum = 0.0f;
@@ -325,7 +336,7 @@ __device__ __forceinline__ void load_row(Row<NB, NP> &row, const T *q, bool vali
     for (int i = 0; i < 8; i += 2) {
       // Quants::keys: a sixteenth, whose own range still ends 2^-20 below the largest
       const float fours = NP == 1 && (i & 2) ? 0x1p-4f : 1.0f;
-      split_pair<NP>(x[b][i] * (into * fours), x[b][i + 1] * (into * fours), row.q[b], i);
+      split_pair<NP>(x[b][i] * into * fours, x[b][i + 1] * into * fours, row.q[b], i);
       sum += (static_cast<float>(row.q[b][0][i]) + static_cast<float>(row.q[b][0][i + 1])) / fours;
     }
     if constexpr (NP == 1) {
@@ -1172,15 +1183,12 @@ attn_q4_0_tiles(AttnArgs a) {
 #pragma unroll
   for (int pass = 0; pass < 2; ++pass) {  // the largest first, then the parts
     if (pass) {
-      int e = 0;
       most = max_of(with_lane32(most));
-      if (most > 0.0f && most < __builtin_inff())
-        (void)frexpf(most, &e);
-      e = min(max(e - 1, -100), 100);
+      const int e = exponent_of(most);
       // an infinity makes the whole row NaN: its products with a key's two parts may be infinities of
       // one sign, a score that looks like that of a hidden token
       sign = most < __builtin_inff() ? ldexpf(sign, -e) : __builtin_nanf("");
-      unit = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, e + 4), 0x1p-100f);
+      unit = unit_of(a.scale, e + 4);
     }
 #pragma unroll
     for (int s = 0; s < 2 * NB; ++s) {
