@@ -3,6 +3,7 @@ tolerances: those of test_gpu_kv_cache.Setup (float64)."""
 import numpy as np
 import pytest
 
+import kv_plain
 from test_gpu_kv_cache import ELEMS, Setup, wide
 
 pytestmark = pytest.mark.gpu
@@ -98,3 +99,67 @@ def test_queries_of_any_power(hip, dev, elem, power, added):
     """Rows near either end of the type's range, with the scale that brings their scores back."""
     s = Setup(dev, elem, [200], [added], 4, 1, 64, 16, seed=23, spread=2.0 ** power)
     s.check(hip, scale=0.1 * 2.0 ** -power)
+
+
+# ------------------------------------------------------- loud beside quiet ---
+
+class Shared(Setup):
+    """Requests that share one run of cached tokens, a new token and one query head each: so many
+    that a work-group takes a whole context and one wave a quarter of it."""
+
+    def __init__(self, dev, elem, k, v, q, requests=512, page=64):
+        length, kv, dim = k.shape
+        super().__init__(dev, elem, [length], [1], 1, kv, dim, page)
+        kq, vq = kv_plain.quantize(k.astype(np.float32)), kv_plain.quantize(v.astype(np.float32))
+        self._put(self.cache, self.slots, kq, vq)
+        self.one = kv_plain.values(*kq)[:, 0], kv_plain.values(*vq)[:, 0]
+        self.lengths, self.added = (np.full(requests, n, np.int32) for n in (length, 1))
+        self.table = np.repeat(self.table, requests, 0)
+        self.first, self.tokens = np.arange(requests + 1, dtype=np.int32), requests
+        self.q = kv_plain.round_to(np.broadcast_to(q, (requests, 1, dim)).copy(), elem)
+
+    def weights(self):
+        """The softmax over the tokens, float64."""
+        z = self.one[0] @ self.q[0, 0].astype(np.float64) * np.float64(np.float32(self.dim ** -0.5))
+        w = np.exp(z - z.max())
+        return w / w.sum()
+
+
+def sink(dev, elem, dim, at, value_of, tail):
+    """2560 tokens, all of a weight of 2^-19 but the one at `at`, which has nearly all of it.
+    tail: magnitudes of the values of elements 32 .. 63; value_of: loud ones, {token: value}, of
+    element 0."""
+    rng = np.random.default_rng(24)
+    k = np.zeros((2560, 1, dim))
+    k[at, 0, 0] = 4.0
+    v = np.zeros((2560, 1, dim))
+    v[:, 0, 32:64] = tail * rng.uniform(0.5, 1.0, (2560, 32))
+    v[at, 0, 32:64] = 0.0
+    for token, value in value_of.items():
+        v[token, 0, 0] = value
+    q = np.zeros(dim)
+    q[0] = 19.0 * np.log(2.0) * dim ** 0.5 / 4.0
+    return Shared(dev, elem, k, v, q)
+
+
+def check_tail(hip, s, top_scale):
+    """Elements 32 .. 63.  A weight is off by twice 2^-21 |z| (z up to 13.2 here) and 2^-20 of it; a
+    weight times a scale is rounded to 11 bits for 16-bit rows, to 22 for f32, and at 2^-25 of what
+    brings weight and largest scale to 2^15 at most and over 2^10: to 2^-35 of that scale.  Eight
+    times that a token at most."""
+    out = wide(s.run(hip))[:, 0, 32:64]
+    w, v = s.weights(), s.one[1][:, 32:64]
+    want, mass = w @ v, w @ np.abs(v)
+    tol = mass * (2.0 ** -22 if s.elem == "f32" else 2.0 ** -11)
+    tol += mass * 2 * (2.0 ** -21 * 13.2 + 2.0 ** -20) + 8 * len(w) * top_scale * 2.0 ** -35
+    tol += np.abs(want) * {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[s.elem]
+    off = np.abs(out - want)
+    assert (off <= tol).all(), (off.max(), tol.min(), want.mean())
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("at", [0, 1300])
+def test_tail_of_small_values(hip, dev, elem, dim, at):
+    """Values of 2^-14 and less under weights that are small together and not alone."""
+    check_tail(hip, sink(dev, elem, dim, at, {}, 2.0 ** -14), 2.0 ** -12)  # scales below 2^-11 alike

@@ -38,13 +38,18 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // value scale within f16's range and as high in it as the value scales seen so far let it be, by the
 // top bits of their exponents: below 2^-11, 2^-7, 2, and whatever fp16 holds.
 constexpr float kSlack = 4.0f;
-constexpr int kLevels = 4;
-__device__ __forceinline__ float shift_of(int level) {  // 2^4 2^shift scale <= 2^15
-  return level == 0 ? 22.0f : level == 1 ? 18.0f : level == 2 ? 10.0f : -4.0f;
+constexpr float kMostShift = 22.0f;
+// `any` holds the bits of all scales: 2^4 2^shift scale <= 2^15
+__device__ __forceinline__ float shift_of(uint32_t any) {
+  float shift = any & 0x70007000u ? 18.0f : kMostShift;
+  shift = any & 0x60006000u ? 10.0f : shift;
+  return any & 0x40004000u ? -4.0f : shift;
 }
-// the exponent bits that a scale of the level's range does not have
-__device__ __forceinline__ uint32_t bits_over(int level) {
-  return level == 0 ? 0x70007000u : level == 1 ? 0x60006000u : level == 2 ? 0x40004000u : 0u;
+// the exponent bits that no scale of the shift's range has
+__device__ __forceinline__ uint32_t bits_over(float shift) {
+  uint32_t over = shift > -4.0f ? 0x40004000u : 0u;
+  over = shift > 10.0f ? 0x60006000u : over;
+  return shift > 18.0f ? 0x70007000u : over;
 }
 
 struct AttnArgs {
@@ -278,7 +283,8 @@ template <int NB, int NP> struct Row {
   // take 8 times these sums of the weights off at the end
   f32x4 start[NP == 1 ? NB : 1], weights[NP == 1 ? NB : 1];
   float m, base, l;     // maximum so far; shift - maximum; this lane's sum of weights
-  int level;            // of the shift
+  float shift;
+  uint32_t over;        // bits_over(shift)
 };
 
 // An exact power of two, 2^-e, brings a row's largest element to 1 .. 2 (to 4 at the range's upper end,
@@ -349,8 +355,8 @@ __device__ __forceinline__ void load_row(Row<NB, NP> &row, const T *q, bool vali
   for (int i = 0; i < 2 * NB; ++i)
     row.o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   row.m = kNone;
-  row.level = NP == 1 ? 2 : 0;
-  row.base = shift_of(row.level);
+  row.shift = row.base = kMostShift;
+  row.over = bits_over(kMostShift);
   row.l = 0.0f;
 }
 
@@ -417,21 +423,19 @@ __device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], b
   for (int i = 1; i < 8; ++i)
     top = fmaxf(top, z[i]);
   top = row_max(top) * row.unit;
-  if (__any(top > row.m + kSlack || (any & bits_over(row.level)) != 0)) {
+  if (__any(top > row.m + kSlack || (any & row.over) != 0)) {
     any |= __shfl_xor(any, 16);
     any |= __shfl_xor(any, 32);
-    int level = row.level;
-#pragma unroll
-    for (int i = NP == 1 ? 2 : 0; i + 1 < kLevels; ++i)
-      level = max(level, any & bits_over(i) ? i + 1 : 0);
+    const float shift = fminf(row.shift, shift_of(any));
     const float m = top > row.m + kSlack ? top : row.m;
-    float f = exp2_fast(shift_of(level) - shift_of(row.level));
+    float f = exp2_fast(shift - row.shift);
     if (m != row.m)
       f *= exp2_fast(row.m - m);  // by 0 from no token to the first
     rescale(row, f);
-    row.level = level;
+    row.shift = shift;
+    row.over = bits_over(shift);
     row.m = m;
-    row.base = shift_of(level) - (m == kNone ? 0.0f : m);
+    row.base = shift - (m == kNone ? 0.0f : m);
   }
   float p[8];
 #pragma unroll
@@ -745,7 +749,7 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16
       if constexpr (NP == 1)
         row.o[i] -= 8.0f * row.weights[i / 2];
     }
-    rescale(row, exp2_fast(-shift_of(row.level)));
+    rescale(row, exp2_fast(-row.shift));
     __syncthreads();  // all have read their rings
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i)
