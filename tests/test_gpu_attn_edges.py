@@ -163,3 +163,14 @@ def check_tail(hip, s, top_scale):
 def test_tail_of_small_values(hip, dev, elem, dim, at):
     """Values of 2^-14 and less under weights that are small together and not alone."""
     check_tail(hip, sink(dev, elem, dim, at, {}, 2.0 ** -14), 2.0 ** -12)  # scales below 2^-11 alike
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("at,loud", [
+    (0, {0: 32.0}), (1300, {1300: 32.0}), (1300, {100: 32.0, 1300: -512.0}), (40, {41: 20.0}),
+])
+def test_tail_beside_loud_values(hip, dev, elem, dim, at, loud):
+    """Values of 1 in one block where another has some of 20 to 512."""
+    top = max(abs(x) for x in loud.values()) / 8
+    check_tail(hip, sink(dev, elem, dim, at, loud, 1.0), top)

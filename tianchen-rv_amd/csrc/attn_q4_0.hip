@@ -35,20 +35,24 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 // Weights are 2^(z - m + shift).  m follows the row's maximum only when that has risen by kSlack
 // (2^4): a rescale of the output costs as much as the tile's products.  The shift keeps weight times
-// value scale within f16's range and as high in it as the value scales seen so far let it be, by the
-// top bits of their exponents: below 2^-11, 2^-7, 2, and whatever fp16 holds.
+// value scale within f16's range and as high in it as the value scales seen so far let it be: by the top
+// bits of their exponents, which an OR of them all shows, below 2^-11, 2^-7 and 2, and from 2 on by the
+// largest exponent itself.  One shift for all blocks of a row: beside a scale of 2^e, e >= 1, what a
+// weight times a scale keeps ends at 2^(e - 35) of the largest weight.
 constexpr float kSlack = 4.0f;
 constexpr float kMostShift = 22.0f;
-// `any` holds the bits of all scales: 2^4 2^shift scale <= 2^15
+// 2^4 2^shift scale <= 2^15, for scales with the bits that `any` has, but for those of 2 and more
 __device__ __forceinline__ float shift_of(uint32_t any) {
-  float shift = any & 0x70007000u ? 18.0f : kMostShift;
-  shift = any & 0x60006000u ? 10.0f : shift;
-  return any & 0x40004000u ? -4.0f : shift;
+  const float shift = any & 0x70007000u ? 18.0f : kMostShift;
+  return any & 0x60006000u ? 10.0f : shift;
 }
-// the exponent bits that no scale of the shift's range has
+// for those, by the field of the largest one's exponent (fp16's 2^0 is 15; what is not finite is left out)
+__device__ __forceinline__ float shift_of_exponent(uint32_t e) {
+  return e < 16 ? kMostShift : 25.0f - static_cast<float>(min(e, 30u));
+}
+// the exponent bits that no scale of the shift's range has, or has to be looked at for
 __device__ __forceinline__ uint32_t bits_over(float shift) {
-  uint32_t over = shift > -4.0f ? 0x40004000u : 0u;
-  over = shift > 10.0f ? 0x60006000u : over;
+  const uint32_t over = shift > 10.0f ? 0x60006000u : 0x40004000u;
   return shift > 18.0f ? 0x70007000u : over;
 }
 
@@ -418,6 +422,19 @@ __device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], b
 #pragma unroll
   for (int i = 0; i < 2 * NB; ++i)
     any |= t[0].vs.v[i] | t[1].vs.v[i];
+  float room = kMostShift;
+  if (__any((any & 0x40004000u) != 0)) {
+    using u16x2 = uint16_t __attribute__((ext_vector_type(2)));
+    u16x2 most{};
+#pragma unroll
+    for (int i = 0; i < 4 * NB; ++i) {
+      const uint32_t e = t[i / (2 * NB)].vs.v[i % (2 * NB)] & 0x7c007c00u;
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, e));
+    }
+    room = shift_of_exponent(static_cast<uint32_t>(max(most[0], most[1])) >> 10);
+    if (room >= row.shift)
+      any &= ~0x40004000u;  // the shift is theirs already
+  }
   float top = z[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i)
@@ -426,7 +443,7 @@ __device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], b
   if (__any(top > row.m + kSlack || (any & row.over) != 0)) {
     any |= __shfl_xor(any, 16);
     any |= __shfl_xor(any, 32);
-    const float shift = fminf(row.shift, shift_of(any));
+    const float shift = fminf(fminf(row.shift, shift_of(any)), -row_max(-room));
     const float m = top > row.m + kSlack ? top : row.m;
     float f = exp2_fast(shift - row.shift);
     if (m != row.m)
