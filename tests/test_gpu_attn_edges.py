@@ -174,3 +174,50 @@ def test_tail_beside_loud_values(hip, dev, elem, dim, at, loud):
     """Values of 1 in one block where another has some of 20 to 512."""
     top = max(abs(x) for x in loud.values()) / 8
     check_tail(hip, sink(dev, elem, dim, at, loud, 1.0), top)
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+def test_prompt_keys_beside_a_loud_one(hip, dev, elem, dim):
+    """Small keys under a large scale of the scores, and after them one key of 2^6: the rows before
+    it do not see it, and keep all bits of theirs."""
+    s = Setup(dev, elem, [100], [100], 4, 1, dim, 16, seed=25)
+    rng = np.random.default_rng(25)
+    k = rng.standard_normal((100, 1, dim)) * 2.0 ** -12
+    k[99] *= 2.0 ** 18
+    kq, vq = kv_plain.quantize(k.astype(np.float32)), kv_plain.quantize(s.v[0].astype(np.float32))
+    s._put(s.cache, s.slots, kq, vq)
+    s.k, s.v = [kv_plain.values(*kq)], [kv_plain.values(*vq)]
+    scale = 2.0 ** 9
+    out, want = wide(s.run(hip, scale=scale))[:99], s.want(scale=scale)[:99]
+    s.k = [s.k[0][:99]]  # those whose norm counts
+    off = np.abs(out - want)
+    assert (off <= s.tolerance(want, scale)).all(), off.max()
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("loud", [{3: 64.0}, {70: 64.0}, {99: 64.0}, {3: 64.0, 70: 40000.0},
+                                  {70: 40000.0}])
+@pytest.mark.parametrize("length,added", [(100, 100), (1100, 20)])
+def test_prompt_values_beside_loud_ones(hip, dev, elem, dim, loud, length, added):
+    """Values of 2^-12 in block 1, in a prompt whose block 0 has single large ones; each block by
+    its own values.  Past scales of 4096 a value ends at 2^-21."""
+    s = Setup(dev, elem, [length], [added], 8, 1, dim, 16, seed=26)
+    rng = np.random.default_rng(26)
+    v = rng.standard_normal((length, 1, dim))
+    v[:, :, 32:64] *= 2.0 ** -12
+    for token, value in loud.items():
+        v[token, 0, 5] = value
+    kq, vq = kv_plain.quantize(s.k[0].astype(np.float32)), kv_plain.quantize(v.astype(np.float32))
+    s._put(s.cache, s.slots, kq, vq)
+    s.k, s.v = [kv_plain.values(*kq)], [kv_plain.values(*vq)]
+    out, want = wide(s.run(hip)), s.want()
+    whole = s.v[0]
+    for b in range(dim // 32):
+        block = slice(32 * b, 32 * b + 32)
+        s.v = [whole[:, :, block]]
+        tol = s.tolerance(want[..., block]) + (2.0 ** -25 if elem == "f16" else 0.0)
+        tol += 2.0 ** -21 if max(loud.values()) > 32768 else 0.0
+        off = np.abs(out - want)[..., block]
+        assert (off <= tol).all(), (b, off.max())

@@ -27,6 +27,8 @@
 namespace tcrv {
 namespace {
 
+using u16x2 = uint16_t __attribute__((ext_vector_type(2)));
+
 constexpr int kRows = 16;          // rows of a tile
 constexpr int kWaves = 4;          // waves of a work-group, which share out a tile's tokens
 constexpr int kStep = 32;          // tokens that a wave takes at a time
@@ -424,7 +426,6 @@ __device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], b
     any |= t[0].vs.v[i] | t[1].vs.v[i];
   float room = kMostShift;
   if (__any((any & 0x40004000u) != 0)) {
-    using u16x2 = uint16_t __attribute__((ext_vector_type(2)));
     u16x2 most{};
 #pragma unroll
     for (int i = 0; i < 4 * NB; ++i) {
@@ -836,7 +837,34 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
 }
 
 constexpr float kTileShift = 10.0f;       // weights: 2^4 2^10, within f16
-constexpr uint32_t kKeyBig = 1, kValueBig = 2, kValueBad = 4;  // a step's scales
+// A step's scales: some are 2 or more, finite ones 4096 or more, not finite.
+constexpr uint32_t kKeyBig = 1, kValueBig = 2, kValueBad = 4, kKeyHuge = 16, kValueHuge = 32;
+// The power of two that scales are multiplied with as they become operands, so that neither they nor the
+// products with sixteenths leave f16's range: 15, 4 or 0.  With the first two a key's two parts hold all of
+// it, whatever the other scales; without any they end at 2^-21 of an element.
+__device__ __forceinline__ int up_of(uint32_t flags, uint32_t big, uint32_t huge) {
+  const int up = flags & big ? 4 : 15;
+  return flags & huge ? 0 : up;
+}
+// 2^e by its bits: in scalar registers where e is
+__device__ __forceinline__ _Float16 power16(int e) {
+  return __builtin_bit_cast(_Float16, static_cast<uint16_t>((15 + e) << 10));
+}
+__device__ __forceinline__ float power32(int e) {
+  return __builtin_bit_cast(float, static_cast<uint32_t>(127 + e) << 23);
+}
+// Scales by the fields of their exponents: the largest field, and the least that one is over 4096's (fields
+// below that wrap past the others; infinity's and NaN's is 0x1000 over)
+struct Exponents {
+  u16x2 most{}, over{0xffff, 0xffff};
+  __device__ __forceinline__ void add(uint32_t scales) {
+    const u16x2 e = __builtin_bit_cast(u16x2, scales & 0x7c007c00u);
+    most = __builtin_elementwise_max(most, e);
+    over = __builtin_elementwise_min(over, static_cast<u16x2>(e - u16x2{0x6c00, 0x6c00}));
+  }
+  __device__ __forceinline__ bool bad() const { return max(most[0], most[1]) == 0x7c00; }
+  __device__ __forceinline__ bool huge() const { return min(over[0], over[1]) < 0x1000; }
+};
 // bit kAbsentAt + i: the page of a step's i-th 16 tokens is not in the cache
 constexpr uint32_t kAbsentAt = 8, kAbsent = 0xfu << kAbsentAt;
 
@@ -1084,17 +1112,24 @@ attn_q4_0_tiles(AttnArgs a) {
     for (int i = 0; i < NB; ++i)
       any |= raw.d.v[i];
     if (keys_piece) {
-      said = (__any(any & 0x4000u) ? kKeyBig : 0) | (absent ? 1u << (kAbsentAt + wave) : 0);
+      if (__any((any & 0x4000u) != 0)) {
+        Exponents e;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          e.add(raw.d.v[b]);
+        said = kKeyBig | (__any(e.huge()) ? kKeyHuge : 0);
+      }
+      said |= absent ? 1u << (kAbsentAt + wave) : 0;
     } else {
 #pragma unroll
       for (int i = NB; i < 2 * NB; ++i)
         any |= raw.d.v[i];
       if (__any((any & 0x40004000u) != 0)) {
-        bool bad = false;
+        Exponents e;
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i)
-          bad |= (raw.d.v[i] & 0x7c00u) == 0x7c00u || (raw.d.v[i] >> 16 & 0x7c00u) == 0x7c00u;
-        said = kValueBig | (__any(bad) ? kValueBad : 0);
+          e.add(raw.d.v[i]);
+        said = kValueBig | (__any(e.bad()) ? kValueBad : 0) | (__any(e.huge()) ? kValueHuge : 0);
       }
     }
     if (lane == 0)
@@ -1107,7 +1142,7 @@ attn_q4_0_tiles(AttnArgs a) {
       f |= s_flags[n & 1][w];
     return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(f)));
   };
-  const auto lay_out = [&](int n, uint32_t flags, bool v_big) __attribute__((always_inline)) {
+  const auto lay_out = [&](int n, uint32_t flags, int v_up) __attribute__((always_inline)) {
     if (flags & kValueBad) {  // infinite and NaN scales: noted, and taken out of the product
       if (tid < NB * (kTokens / 32))
         s_bad[n & 1][tid / (kTokens / 32)][tid % (kTokens / 32)] = 0;
@@ -1125,9 +1160,8 @@ attn_q4_0_tiles(AttnArgs a) {
       }
     }
     uint8_t *const keys = s_step[n & 1], *const values = keys + 2 * S::kKeys;
-    const _Float16 up = static_cast<_Float16>(32768.0f), one = static_cast<_Float16>(1.0f);
     if (keys_piece) {
-      const _Float16 f = flags & kKeyBig ? one : up;
+      const _Float16 f = power16(up_of(flags, kKeyBig, kKeyHuge));
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const _Float16 d = __builtin_bit_cast(_Float16, static_cast<uint16_t>(raw.d.v[b])) * f;
@@ -1140,7 +1174,7 @@ attn_q4_0_tiles(AttnArgs a) {
         *reinterpret_cast<u32x4 *>(to) = u32x4{x[0][0], x[1][0], x[2][0], x[3][0]};
       }
     } else {
-      const _Float16 f = v_big ? one : up;
+      const _Float16 f = power16(v_up);
       // tokens in the order in which the weights lie: 4 of a lane's half, 4 of the other half's,
       // then 4 and 4 again
       const int at = 16 * (value_group >> 2) + 8 * (value_group & 1) + 2 * (value_group & 2);
@@ -1235,44 +1269,45 @@ attn_q4_0_tiles(AttnArgs a) {
     o[b] = f32x16{};
 
   uint32_t flags = 0;
-  bool v_big = false;
+  int v_up = 15;  // the least of the steps so far
   if (steps > 0) {
     tell(0);
     __syncthreads();  // and all have their queries
     flags = told(0);
-    v_big = flags & kValueBig;
-    lay_out(0, flags, v_big);
+    v_up = up_of(flags, kValueBig, kValueHuge);
+    lay_out(0, flags, v_up);
     bring(1, place);
     place = find(2);
   }
-  bool was_big = v_big;
+  int was_up = v_up;
   // The keys' threads bring the next step in before they compute, the values' afterwards: of the two
   // waves of a SIMD one is at its matrix products while the other is not.
   const auto next_step = [&](int n) __attribute__((always_inline)) {
-    lay_out(n + 1, flags, v_big);
+    lay_out(n + 1, flags, v_up);
     bring(n + 2, place);
     place = find(n + 3);
   };
   for (int n = 0; n < steps; ++n) {
     const uint32_t mine = flags;
-    const bool mine_big = v_big;
+    const int mine_up = v_up;
     if (n + 1 < steps)
       tell(n + 1);
     __syncthreads();  // this step is laid out, and the one before it read
     if (n + 1 < steps) {
       flags = told(n + 1);
-      v_big = v_big || (flags & kValueBig);
+      v_up = min(v_up, up_of(flags, kValueBig, kValueHuge));
       if (keys_piece)
         next_step(n);
     }
     const uint8_t *const keys = s_step[n & 1], *const values = keys + 2 * S::kKeys;
-    if (mine_big && !was_big) {
-      was_big = true;
+    if (mine_up != was_up) {
+      const float f = power32(mine_up - was_up);
 #pragma unroll
       for (int b = 0; b < NB; ++b)
-        o[b] *= 0x1p-15f;
+        o[b] *= f;
+      was_up = mine_up;
     }
-    const float u = unit * (mine & kKeyBig ? 1.0f : 0x1p-15f);
+    const float u = unit * power32(-up_of(mine, kKeyBig, kKeyHuge));
     const int t0 = begin + n * kTokens;
     if (t0 < wave_hi && t0 + kTokens > wave_lo) {
       const bool edge = t0 < all_lo || t0 + kTokens > all_hi || (mine & kAbsent) != 0;
@@ -1403,7 +1438,7 @@ attn_q4_0_tiles(AttnArgs a) {
   if (row0 > last && cut)
     return;
   const float sum = sum_of(with_lane32(l));
-  const float out_unit = exp2_fast(was_big ? 4.0f : -11.0f);
+  const float out_unit = power32(4 - was_up);
   if (cut) {
     if (!valid)
       return;
