@@ -1332,12 +1332,15 @@ attn_q4_0_tiles(AttnArgs a) {
       const auto settle = [&](f32x16 &z, int sub) __attribute__((always_inline)) {
         if (edge) {
           // register i: token 8 (i / 4) + 4 hh + i % 4
-          const int lo_at = lo - t0 - 32 * sub - 4 * hh, hi_at = hi - t0 - 32 * sub - 4 * hh;
+          const int lo_at = lo - t0 - 32 * sub - 4 * hh;
+          int hi_at[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            hi_at[i] = mine >> (kAbsentAt + 2 * sub + i) & 1u ? 0 : hi - t0 - 32 * sub - 4 * hh;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int at = 8 * (i >> 2) + (i & 3);
-            const bool there = !(mine >> (kAbsentAt + 2 * sub + (i >> 3)) & 1u);
-            z[i] = there && at >= lo_at && at < hi_at ? z[i] : kNone;
+            z[i] = at >= lo_at && at < hi_at[i >> 3] ? z[i] : kNone;
           }
         }
         float high = z[0];
