@@ -390,7 +390,9 @@ TCRV_HIP_API int tcrv_hip_gemv_q4_0_soa_q8_0(size_t n, float *s, const uint8_t *
  * Activations are f32, f16 or bf16 (`elem`: TCRV_HIP_ELEM_F32, _F16, _BF16) as
  * [token][head][head_dim] with the last dimension dense and the strides of a
  * token and of a head given in elements (the columns of one fused projection
- * serve as they are); pointers need the element's alignment.  Sums, softmax
+ * serve as they are); pointers need the element's alignment.  No two rows that an
+ * entry writes may overlap; rows that it reads may, but for those of neighbouring
+ * heads and neighbouring tokens: else TCRV_HIP_ERR_BAD_SIZE.  Sums, softmax
  * statistics and rotations are computed in f32 for every `elem`.
  *
  * The cache of one layer is `pages` pages of page_size tokens (a multiple of

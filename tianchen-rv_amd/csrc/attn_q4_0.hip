@@ -1919,6 +1919,8 @@ int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
   if (attn_too_large(requests, tokens, max_added, max_length, heads) || pages > 0x7fffffffu ||
       table_stride > 0x7fffffffu)
     return TCRV_HIP_ERR_TOO_LARGE;
+  if (!rows_apart(out_token, out_head, tokens, heads, head_dim))
+    return TCRV_HIP_ERR_BAD_SIZE;
   if (pages == 0)
     max_length = 0;  // nothing to read
   const Kernels k = kernels_of(requests, tokens, max_added, heads, kv_heads);

@@ -126,10 +126,32 @@ inline bool groups_of_4(const void *p, size_t token, size_t head, size_t size) {
   return aligned_to(p, 4 * size) && token % 4 == 0 && head % 4 == 0;
 }
 
-// Rows of `heads` heads: a head lies beside the next, and a token's heads before the next
-// token's or interleaved with them; only what would make two rows overlap in part is refused.
+// Rows that are read: a head's row begins past the one before it, and a token's likewise.  In other
+// pairs they may overlap.
 inline bool strides_ok(size_t token, size_t head, size_t tokens, size_t heads, size_t dim) {
   return (heads <= 1 || head >= dim) && (tokens <= 1 || token >= dim);
+}
+
+// Rows that are written: no two of them overlap.  Token t's head h lies t * token + h * head on, so that
+// i > 0 heads on and j > 0 tokens back must be a row away either way: looked at for the two j next to where
+// these meet.
+inline bool rows_apart(size_t token, size_t head, size_t tokens, size_t heads, size_t dim) {
+  using Wide = unsigned __int128;
+  if (!strides_ok(token, head, tokens, heads, dim))
+    return false;
+  if (tokens <= 1 || heads <= 1 || Wide{token} >= Wide{head} * (heads - 1) + dim ||
+      Wide{head} >= Wide{token} * (tokens - 1) + dim)
+    return true;
+  if (token == 0)
+    return dim == 0;
+  for (size_t i = 1; i < heads; ++i) {
+    const Wide on = Wide{head} * i, j = on / token;
+    if (j >= 1 && j < tokens && on - j * token < dim)
+      return false;
+    if (j + 1 < tokens && (j + 1) * token - on < dim)
+      return false;
+  }
+  return true;
 }
 
 }  // namespace tcrv_host

@@ -493,6 +493,9 @@ int tcrv_hip_kv_load_q4_0(int elem, const uint8_t *cache, size_t pages, size_t p
     return TCRV_HIP_ERR_MISALIGNED;
   if (tokens > 0x7fffffffu || pages > 0x7fffffffu)
     return TCRV_HIP_ERR_TOO_LARGE;
+  if (!rows_apart(k_token, k_head, tokens, kv_heads, head_dim) ||
+      !rows_apart(v_token, v_head, tokens, kv_heads, head_dim))
+    return TCRV_HIP_ERR_BAD_SIZE;
   const uint32_t nb = static_cast<uint32_t>(head_dim / 32);
   tcrv::LoadArgs a{cache,   slots,  k, v, k_token, k_head, v_token, v_head, pages * page_size,
                    static_cast<uint32_t>(page_size), static_cast<uint32_t>(kv_heads), nb,

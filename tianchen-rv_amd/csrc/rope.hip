@@ -225,6 +225,8 @@ int tcrv_hip_rope(int elem, int layout, const void *x, size_t x_token, size_t x_
     return TCRV_HIP_ERR_MISALIGNED;
   if (tokens > 0x7fffffffu || heads > 0xffffu || head_dim > 65536u)
     return TCRV_HIP_ERR_TOO_LARGE;
+  if (!rows_apart(y_token, y_head, tokens, heads, head_dim))
+    return TCRV_HIP_ERR_BAD_SIZE;
   const auto whole = [&](const void *p, size_t token, size_t head) {
     // the loads of 4 or 8 elements: 16 bytes of f32, 8 or 16 of 16-bit types
     return aligned16(p) && token * size % 16 == 0 && head * size % 16 == 0;
