@@ -392,8 +392,10 @@ TCRV_HIP_API int tcrv_hip_gemv_q4_0_soa_q8_0(size_t n, float *s, const uint8_t *
  * token and of a head given in elements (the columns of one fused projection
  * serve as they are); pointers need the element's alignment.  No two rows that an
  * entry writes may overlap; rows that it reads may, but for those of neighbouring
- * heads and neighbouring tokens: else TCRV_HIP_ERR_BAD_SIZE.  Sums, softmax
- * statistics and rotations are computed in f32 for every `elem`.
+ * heads and neighbouring tokens: else TCRV_HIP_ERR_BAD_SIZE.  A call takes less than
+ * 2^24 tokens (tcrv_hip_kv_tables 2^31), a table up to 2^28 - 16 rows, else
+ * TCRV_HIP_ERR_TOO_LARGE.  Sums, softmax statistics and rotations are computed in
+ * f32 for every `elem`.
  *
  * The cache of one layer is `pages` pages of page_size tokens (a multiple of
  * 16) for `kv_heads` heads of head_dim 64, 128, 192 or 256; a page is

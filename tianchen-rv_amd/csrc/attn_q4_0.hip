@@ -1868,7 +1868,8 @@ bool attn_sizes_ok(size_t heads, size_t kv_heads, size_t head_dim) {
 bool attn_too_large(size_t requests, size_t tokens, size_t max_added, size_t max_length,
                     size_t heads) {
   const size_t most = 0x7fffffffu;
-  return requests > most || tokens > most || max_added > most || max_length > (size_t{1} << 30) ||
+  return requests > most || tokens > tcrv_host::kMostTokens || max_added > most ||
+         max_length > (size_t{1} << 30) ||
          max_added * heads > most || requests * max_added > most ||
          requests * max_added * heads > (size_t{1} << 40);
 }
@@ -1928,8 +1929,9 @@ int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
   const Plan few = few_plan(requests, max_added, max_length, bound, heads, kv_heads, head_dim);
   const Plan many =
       many_plan(elem, requests, tokens, max_added, max_length, bound, heads, kv_heads, head_dim);
-  if ((k.few && requests * few.tiles * kv_heads > 0x7fffffffu) ||
-      (k.many && many.launch > 0x7fffffffu))
+  // rows16 numbers its tiles in 32 bits; a work-group of the other kernel has two threads a row
+  if ((k.few && (requests * few.tiles * kv_heads > 0x7fffffffu || few.launch > kMostGroups)) ||
+      (k.many && many.launch > 0xffffffffu / (2 * many.tile_rows)))
     return TCRV_HIP_ERR_TOO_LARGE;
   const size_t need = (k.few ? few.workspace : 0) + (k.many ? many.workspace : 0);
   if (need) {

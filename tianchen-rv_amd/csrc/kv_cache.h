@@ -114,6 +114,8 @@ inline bool aligned_to(const void *p, size_t bytes) {
 // A page's bytes have to fit the kernels' 32-bit offsets within a page's head, and heads a grid.
 constexpr size_t kMostPageSize = 65536;
 constexpr size_t kMostHeads = 65535;
+// A launch holds less than 2^32 threads along an axis: work-groups of 256, one a token.
+constexpr size_t kMostGroups = 0xffffffu, kMostTokens = kMostGroups;
 
 inline bool cache_sizes_ok(size_t page_size, size_t kv_heads, size_t head_dim) {
   return page_size != 0 && page_size % 16 == 0 && page_size <= kMostPageSize && kv_heads != 0 &&

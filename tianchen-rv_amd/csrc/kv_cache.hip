@@ -443,7 +443,7 @@ int tcrv_hip_kv_store_q4_0(int elem, const void *k, size_t k_token, size_t k_hea
   if (!aligned_to(k, size) || !aligned_to(v, size) || !aligned_to(slots, 8) || !aligned16(cache) ||
       (n_dims && (!aligned4(positions) || !aligned4(table))))
     return TCRV_HIP_ERR_MISALIGNED;
-  if (tokens > 0x7fffffffu || pages > 0x7fffffffu)
+  if (tokens > kMostTokens || pages > 0x7fffffffu)
     return TCRV_HIP_ERR_TOO_LARGE;
   const uint32_t nb = static_cast<uint32_t>(head_dim / 32);
   tcrv::StoreArgs a{k,       v,       positions, table,      slots,
@@ -491,7 +491,7 @@ int tcrv_hip_kv_load_q4_0(int elem, const uint8_t *cache, size_t pages, size_t p
     return TCRV_HIP_ERR_NULL_POINTER;
   if (!aligned_to(k, size) || !aligned_to(v, size) || !aligned_to(slots, 8) || !aligned16(cache))
     return TCRV_HIP_ERR_MISALIGNED;
-  if (tokens > 0x7fffffffu || pages > 0x7fffffffu)
+  if (tokens > kMostTokens || pages > 0x7fffffffu)
     return TCRV_HIP_ERR_TOO_LARGE;
   if (!rows_apart(k_token, k_head, tokens, kv_heads, head_dim) ||
       !rows_apart(v_token, v_head, tokens, kv_heads, head_dim))

@@ -178,7 +178,7 @@ int tcrv_hip_rope_table(int scaling, size_t n_dims, double base, double factor,
   const size_t pairs = n_dims / 2;
   const size_t gx = (count - 1) / tcrv::kTableRows + 1;
   const size_t gy = (pairs + tcrv::kTableThreads - 1) / tcrv::kTableThreads;
-  if (gx > 0x7fffffffu || gy > 65535u || first > (1ull << 52) || count > (1ull << 52))
+  if (gx > kMostGroups || gy > 65535u || first > (1ull << 52) || count > (1ull << 52))
     return TCRV_HIP_ERR_TOO_LARGE;
   const double n = static_cast<double>(n_dims);
   tcrv::TableForm form{log2(base), 0.0, 0.0, 1.0, amplitude > 0.0 ? amplitude : 1.0, 0};
@@ -223,7 +223,7 @@ int tcrv_hip_rope(int elem, int layout, const void *x, size_t x_token, size_t x_
     return TCRV_HIP_ERR_NULL_POINTER;
   if (!aligned_to(x, size) || !aligned_to(y, size) || !aligned4(positions) || !aligned4(table))
     return TCRV_HIP_ERR_MISALIGNED;
-  if (tokens > 0x7fffffffu || heads > 0xffffu || head_dim > 65536u)
+  if (tokens > kMostTokens || heads > 0xffffu || head_dim > 65536u)
     return TCRV_HIP_ERR_TOO_LARGE;
   if (!rows_apart(y_token, y_head, tokens, heads, head_dim))
     return TCRV_HIP_ERR_BAD_SIZE;
