@@ -471,7 +471,9 @@ TCRV_HIP_API int tcrv_hip_rope(int elem, int layout, const void *x, size_t x_tok
  *   taken        one value: the new pages that the requests need.  Over
  *                free_count: some are missing
  * Sums are 64-bit; what does not fit an int32 output is written as INT32_MAX.
- * Repeating a call with the same inputs gives the same outputs. */
+ * Repeating a call with the same inputs gives the same outputs.  free_pages is not
+ * changed: before the next step, also before a captured one is replayed, the caller
+ * takes its first taken[0] entries off, or that step gives them out again. */
 TCRV_HIP_API int tcrv_hip_kv_tables(const int32_t *context, const int32_t *added,
                                     size_t requests, size_t page_size,
                                     const int32_t *free_pages, size_t free_count,
