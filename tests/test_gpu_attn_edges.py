@@ -221,3 +221,18 @@ def test_prompt_values_beside_loud_ones(hip, dev, elem, dim, loud, length, added
         tol += 2.0 ** -21 if max(loud.values()) > 32768 else 0.0
         off = np.abs(out - want)[..., block]
         assert (off <= tol).all(), (b, off.max())
+
+
+# ------------------------------------------------------------- wide windows ---
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("lengths,added", [([20, 50], [30, 3]), ([3, 1], [6, 1])])
+def test_windows_wider_than_all_positions(hip, dev, elem, lengths, added):
+    """They hide nothing, also from rows before the first position, which see all tokens where a row's
+    own position is no bound."""
+    s = Setup(dev, elem, lengths, added, 4, 2, 64, 16, seed=27)
+    for causal in (False, True):
+        whole = wide(s.run(hip, causal=causal))
+        for window in (2 ** 30, 2 ** 31 - 20, 2 ** 31 - 2, 2 ** 31 - 1, 2 ** 32 + 1):
+            assert np.array_equal(wide(s.run(hip, causal=causal, window=window)), whole), window
+    s.check(hip, causal=False)

@@ -505,9 +505,11 @@ struct Span {
     rows = added * a.share;
     length = min(min(whole, static_cast<int>(a.max_length)), static_cast<int>(a.table_tokens));
   }
-  // tokens lo <= t < hi that the row of the i-th new token sees
+  // tokens lo <= t < hi that the row of the i-th new token sees; a position may lie before the first one,
+  // from which a window of 2^31 - 2 would leave 32 bits
   __device__ int lo(const AttnArgs &a, uint32_t i) const {
-    return a.window ? max(position0 + static_cast<int>(i) + 1 - static_cast<int>(a.window), 0) : 0;
+    const int next = max(position0 + static_cast<int>(i) + 1, 0);
+    return a.window ? max(next - static_cast<int>(a.window), 0) : 0;
   }
   __device__ int hi(const AttnArgs &a, uint32_t i) const {
     return max(a.causal ? min(position0 + static_cast<int>(i) + 1, length) : length, 0);
