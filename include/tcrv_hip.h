@@ -471,6 +471,8 @@ TCRV_HIP_API int tcrv_hip_rope(int elem, int layout, const void *x, size_t x_tok
  *   taken        one value: the new pages that the requests need.  Over
  *                free_count: some are missing
  * Sums are 64-bit; what does not fit an int32 output is written as INT32_MAX.
+ * The outputs overlap neither one another nor the inputs (`length` is copied to
+ * `context` after the call, not written there).
  * Repeating a call with the same inputs gives the same outputs.  free_pages is not
  * changed: before the next step, also before a captured one is replayed, the caller
  * takes its first taken[0] entries off, or that step gives them out again. */

@@ -17,8 +17,8 @@
 //
 // Few rows are bound by the read of the cache, 9/8 byte an element of a kv head and token, and the
 // instructions that make operands of it: two contexts of 131072 tokens, bf16, 32 query and 8 kv heads of
-// 128, 54 us and 6.6 for the join (264 MB, 4.9 TB/s without it); 64 requests of 1024 to 8192, f16, 77 and
-// 5.3 (334 MB, 4.3 TB/s).  A wave reads its steps through an LDS ring of its own, so that
+// 128, 55 us and 6.7 for the join (264 MB, 4.8 TB/s without it); 64 requests of 1024 to 8192, f16, 78 and
+// 5.2 (334 MB, 4.3 TB/s).  A wave reads its steps through an LDS ring of its own, so that
 // no register waits for them.
 #include <algorithm>
 
@@ -827,10 +827,11 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16
 // A key is two f16 parts, which hold all of its 15 bits: a score's error would grow with the score.
 // f16 and bf16 rows take values and weights as one part each; for f32 rows queries, values and weights
 // are two parts as well, and a product three: the larger parts', and the mixed ones.
-// A prompt of 4096, f16, 32 query and 8 kv heads of 128: 223 us, 620 TFLOP/s, a step of 64 tokens 3.4 us, of
-// which the matrix instructions are 1.6 and the others and LDS as much each: eight waves, two a SIMD, meet at
-// every step and overlap no more.  Of head_dim 64 and f32 a step is 5 us; two work-groups a CU there (128
-// registers) spilled and took 74 us in 9 chunks where one takes 74.
+// A prompt of 4096, f16, 32 query and 8 kv heads of 128: 225 us back to back, 611 TFLOP/s (263 after 2 ms
+// without work), a step of 64 tokens 3.4 us, of which the matrix instructions are 1.6 and the others and
+// LDS as much each: eight waves, two a SIMD, meet at every step and overlap no more.  Of head_dim 64 and
+// f32 a step is 5 us; two work-groups a CU there (128 registers) spilled and took 74 us in 9 chunks where
+// one took 74.
 // ---------------------------------------------------------------------------
 using f32x16 = float __attribute__((ext_vector_type(16)));
 
@@ -970,7 +971,11 @@ __device__ __forceinline__ bool find_piece(const AttnArgs &a, uint32_t w, int la
         groups += n * (even ? ceilf(last * parts - 0x1p-10f) : fmaxf(mean * parts + 0.5f, 1.0f));
       }
     }
-    // alike they run in rounds of the CUs, else one after the other with the longest at the end
+    // alike they run in rounds of the CUs, else one after the other with the longest at the end, of which
+    // 0.4 is not hidden (with none of it a prompt of 1024 takes 61 us for 48, 4 of 700 72 for 56; with all
+    // of it the same, and one of 2048 105 for 95).  Alike from 3/4 on: from 9/10 1000 new tokens on 7192
+    // take 279 for 219 and 4 times 512 on 3584 177 for 205; from 1/2 3 times 300 on 2700, f32, 99 for 127,
+    // all else within 8 %
     const float one = static_cast<float>(part + kPartFill);
     const float cost = (lane ? kPartJoin : 0) +
                        (alike ? ceilf(groups * (1.0f / kCus)) * one

@@ -132,10 +132,11 @@ __global__ __launch_bounds__(kTableThreads) void kv_tables(TablesArgs a) {
 // The store.  Bound by memory: keys and values read once, 9/16 byte an element written.  A block
 // of 32 elements is 8 lanes of 4 (as in quantize_q8_0), a row of 16 lanes two blocks: the nibbles
 // of a byte meet by a move of 4 lanes, and the two bytes of a unit of the values by one of 8.
-// A work-group takes a token: 8191 tokens x 8 heads x 128, f32, 26 us (77 MB, 2.9 TB/s), what is left
-// being the slot's, the position's and the table row's latency before 9 KB of work.  Four tokens a
-// work-group, whose bytes leave 8 at a time, took 32 to 35 us, an item's loads sent before the one before
-// it is worked on 33.
+// A work-group takes a token: 8191 tokens x 8 heads x 128, f32, 24 us for 81 MB that have to move.  It moves
+// 98: a token's value bytes are 2 of every 8, beside those of three neighbours whose work-groups run on
+// other XCDs, and 25 MB are written for 9.4.  The slot, the position and the table row come one after the
+// other before 9 KB of work.  Four tokens a work-group, whose bytes leave 8 at a time, took 32 to 35 us, an
+// item's loads sent before the one before it is worked on 33.
 // ---------------------------------------------------------------------------
 struct StoreArgs {
   const void *k, *v;
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_q4_0(StoreArgs a) {
 
 // ---------------------------------------------------------------------------
 // The reading back: (q - 8) d is exact in f32.  The lanes' places as in the store; 8191 tokens as there
-// 27 us (77 MB).
+// 26 us for 77 MB: 102 move, 35 of the cache for the 9.4 that are there, by the neighbours' shared lines.
 // ---------------------------------------------------------------------------
 struct LoadArgs {
   const uint8_t *cache;

@@ -7,7 +7,9 @@ namespace {
 // ---------------------------------------------------------------------------
 // The table.  Angles of a position past 2^17 need more than f32's 24 bits, so they are formed in
 // f64 and reduced there.  A thread makes kTableRows rows of one pair, so that the power is taken
-// once for all of them.
+// once for all of them.  131072 rows of 64 pairs 34 us (67 MB, 14 us at a copy's rate), of 32 pairs 31, 4096
+// rows 5.9: a thread's 16 sines in turn, on one of a work-group's four waves up to 64 pairs.  It runs once, or
+// as contexts grow.
 // ---------------------------------------------------------------------------
 constexpr int kTableThreads = 256;
 constexpr int kTableRows = 16;
