@@ -519,12 +519,13 @@ TCRV_HIP_API int tcrv_hip_kv_load_q4_0(int elem, const uint8_t *cache, size_t pa
  * or infinity are NaN; a row that sees a value scale which is not finite is not
  * finite in that block.  f32 rows: queries and weights, and values of prompts,
  * enter the matrix cores as two f16 parts each (22 bits).  f16 and bf16 rows:
- * queries down to 2^-20 of the row's largest, weights as f16, in prompts values
- * as f16; keys always with all of their bits (in prompts finite scales of 4096 and
- * more end keys and values that lie beside them at 2^-21).  Single tokens and few
- * rows take weight times value scale together, the row's largest weight being about
- * 1: down to 2^-35, and to 2^(e - 35) where the row sees a scale of 2^e, e >= 1.
- * out's rows past first[requests] are not written; out must not overlap q.
+ * queries down to 2^-20 of the row's largest, weights as f16 (in prompts of f16
+ * rows half of them as two parts), in prompts values as f16; keys always with all
+ * of their bits (in prompts finite scales of 4096 and more end keys and values that
+ * lie beside them at 2^-21).  Single tokens and few rows take weight times value
+ * scale together, the row's largest weight being about 1: down to 2^-35, and to
+ * 2^(e - 35) where the row sees a scale of 2^e, e >= 1.  out's rows past
+ * first[requests] are not written; out must not overlap q.
  * max_added and max_length (at most 2^30, else TCRV_HIP_ERR_TOO_LARGE) are the
  * caller's bounds on added tokens and lengths (they size the launch): further
  * rows are not written, further tokens not read.  How contexts are cut over

@@ -236,3 +236,28 @@ def test_windows_wider_than_all_positions(hip, dev, elem, lengths, added):
         for window in (2 ** 30, 2 ** 31 - 20, 2 ** 31 - 2, 2 ** 31 - 1, 2 ** 32 + 1):
             assert np.array_equal(wide(s.run(hip, causal=causal, window=window)), whole), window
     s.check(hip, causal=False)
+
+
+# ------------------------------------------------------- error of 16-bit rows ---
+
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("length,added", [(700, 200), (1500, 90)])
+def test_error_of_f16_prompts(hip, dev, dim, length, added):
+    """The error against float64, as a 2-norm, is that of the roundings that are meant: values to f16,
+    every other 16 tokens' weights to f16, the output to f16.  Their sum is formed here from the same
+    inputs, with weights over the row's own maximum; the kernel's base differs, which shifts which
+    weights round up and which down: 3 % for that, where rounding the others' too adds 7 %."""
+    s = Setup(dev, "f16", [length], [added], 8, 2, dim, 16, seed=28, spread=0.5)
+    out, want = wide(s.run(hip)), s.want()
+    model = np.empty_like(want)
+    at, t = length - added + np.arange(added)[:, None], np.arange(length)[None]
+    half = np.float64(2.0 ** 10)
+    values = (s.v[0] * half).astype(np.float16).astype(np.float64) / half
+    for h in range(8):
+        z = np.float64(np.float32(dim ** -0.5)) * (s.q[:, h].astype(np.float64) @ s.k[0][:, h // 4].T)
+        z = np.where(t <= at, z, -np.inf)
+        w = np.exp(z - z.max(1, keepdims=True)) * half
+        w = np.where(t // 16 % 2 == 0, w.astype(np.float16).astype(np.float64), w)
+        model[:, h] = w @ values[:, h // 4] / w.sum(1, keepdims=True)
+    model = model.astype(np.float16).astype(np.float64)
+    assert np.linalg.norm(out - want) <= 1.03 * np.linalg.norm(model - want)

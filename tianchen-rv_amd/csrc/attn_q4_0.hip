@@ -21,6 +21,7 @@
 // 5.2 (334 MB, 4.3 TB/s).  A wave reads its steps through an LDS ring of its own, so that
 // no register waits for them.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_cache.h"
 
@@ -164,6 +165,17 @@ __device__ __forceinline__ f16x2 times_pair(float x0, float x1, uint32_t d) {
   asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]"
       : "+v"(r)
       : "v"(x1), "v"(d));
+  return __builtin_bit_cast(f16x2, r);
+}
+
+// What rounding two f32 values to f16 left of them, as f16: exact but for f16's range.
+__device__ __forceinline__ f16x2 left_of_pair(float x0, float x1, f16x2 rounded) {
+  const uint32_t hi = __builtin_bit_cast(uint32_t, rounded);
+  uint32_t r;
+  asm("v_fma_mixlo_f16 %0, %1, 1.0, -%2 op_sel_hi:[0,0,1]" : "=v"(r) : "v"(x0), "v"(hi));
+  asm("v_fma_mixhi_f16 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]"
+      : "+v"(r)
+      : "v"(x1), "v"(hi));
   return __builtin_bit_cast(f16x2, r);
 }
 
@@ -826,10 +838,14 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16
 // weights again leave the first one where the second one reads them.
 // A key is two f16 parts, which hold all of its 15 bits: a score's error would grow with the score.
 // f16 and bf16 rows take values and weights as one part each; for f32 rows queries, values and weights
-// are two parts as well, and a product three: the larger parts', and the mixed ones.
-// A prompt of 4096, f16, 32 query and 8 kv heads of 128: 225 us back to back, 611 TFLOP/s (263 after 2 ms
-// without work), a step of 64 tokens 3.4 us, of which the matrix instructions are 1.6 and the others and
-// LDS as much each: eight waves, two a SIMD, meet at every step and overlap no more.  Of head_dim 64 and
+// are two parts as well, and a product three: the larger parts', and the mixed ones.  f16 rows take what the
+// rounding left of every other 16 tokens' weights beside them: without it the prompt below is off by 3.11e-4
+// of its output, more than 1.5 times the output's own rounding of 2.06e-4; with it by 2.90e-4, for 12 % of
+// its time (other prompts 3 to 11 %); with that of all tokens' weights by 2.61e-4, for 24 %.  The rounding
+// of bf16 outputs alone is 1.7e-3.
+// A prompt of 4096, f16, 32 query and 8 kv heads of 128: 248 us back to back, 555 TFLOP/s (289 after 2 ms
+// without work), a step of 64 tokens 3.8 us, of which the matrix instructions are 1.9 and the others and
+// LDS 1.6 each: eight waves, two a SIMD, meet at every step and overlap no more.  Of head_dim 64 and
 // f32 a step is 5 us; two work-groups a CU there (128 registers) spilled and took 74 us in 9 chunks where
 // one took 74.
 // ---------------------------------------------------------------------------
@@ -1370,7 +1386,9 @@ attn_q4_0_tiles(AttnArgs a) {
         }
         return f;
       };
-      const auto weigh = [&](const f32x16 &z, f16x8 (&w)[2][NP]) {
+      // left: of the second 16 tokens' weights, for f16 rows
+      constexpr bool kLeft = std::is_same_v<T, _Float16>;
+      const auto weigh = [&](const f32x16 &z, f16x8 (&w)[2][NP], f16x8 &left) {
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
           const float p0 = exp2_fast(fmaf(z[i], u, base)), p1 = exp2_fast(fmaf(z[i + 1], u, base));
@@ -1379,13 +1397,20 @@ attn_q4_0_tiles(AttnArgs a) {
           // values were multiplied with
           if constexpr (NP == 1) {
             const f16x8 &x = w[i >> 3][0];
-            l = __builtin_amdgcn_fdot2(f16x2{x[i & 7], x[(i & 7) + 1]}, f16x2{1, 1}, l, false);
+            const f16x2 rounded{x[i & 7], x[(i & 7) + 1]};
+            l = __builtin_amdgcn_fdot2(rounded, f16x2{1, 1}, l, false);
+            if (kLeft && i >= 8) {
+              const f16x2 rest = left_of_pair(p0, p1, rounded);
+              l = __builtin_amdgcn_fdot2(rest, f16x2{1, 1}, l, false);
+              left[i & 7] = rest[0];
+              left[(i & 7) + 1] = rest[1];
+            }
           } else {
             l += p0 + p1;
           }
         }
       };
-      const auto add_values = [&](const f16x8 (&w)[2][NP], int sub) {
+      const auto add_values = [&](const f16x8 (&w)[2][NP], const f16x8 &left, int sub) {
         const uint8_t *const value = values + col * S::kValueRow + (32 * sub + 8 * hh) * 2;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -1397,6 +1422,8 @@ attn_q4_0_tiles(AttnArgs a) {
               v[p] = *reinterpret_cast<const f16x8 *>(value + p * S::kValues + b * 32 * S::kValueRow +
                                                       s * 32);
             o[b] = mfma32(v[0], w[s][0], o[b]);
+            if (kLeft && s == 1)
+              o[b] = mfma32(v[0], left, o[b]);
             if constexpr (NP == 2) {
               o[b] = mfma32(v[0], w[s][1], o[b]);
               o[b] = mfma32(v[1], w[s][0], o[b]);
@@ -1409,24 +1436,26 @@ attn_q4_0_tiles(AttnArgs a) {
       // where they alternate.
       f32x16 z0 = scores(0);
       (void)settle(z0, 0);
-      f16x8 w0[2][NP];
+      f16x8 w0[2][NP], left0;
       if constexpr (kTokens == 32) {
-        weigh(z0, w0);
-        add_values(w0, 0);
+        weigh(z0, w0, left0);
+        add_values(w0, left0, 0);
       } else {
         f32x16 z1 = scores(1);
-        weigh(z0, w0);
+        weigh(z0, w0, left0);
         const float f = settle(z1, 1);
         if (__any(f != 1.0f)) {
           const _Float16 h = static_cast<_Float16>(f);
 #pragma unroll
           for (int i = 0; i < 2 * NP; ++i)
             w0[i / NP][i % NP] *= h;
+          if (kLeft)
+            left0 *= h;
         }
-        f16x8 w1[2][NP];
-        weigh(z1, w1);
-        add_values(w0, 0);
-        add_values(w1, 1);
+        f16x8 w1[2][NP], left1;
+        weigh(z1, w1, left1);
+        add_values(w0, left0, 0);
+        add_values(w1, left1, 1);
       }
       if (mine & kValueBad) {
         // a row that sees a value scale that is not finite is NaN in that block
