@@ -177,6 +177,21 @@ def test_tail_beside_loud_values(hip, dev, elem, dim, at, loud):
 
 
 @pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("at,token", [(0, 0), (0, 700), (1300, 1301)])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_tail_beside_a_scale_that_is_not_finite(hip, dev, elem, dim, at, token, bad):
+    """Values of 1 in one block where another has a scale that is not finite: they keep their weights,
+    as beside scales below 2."""
+    s = sink(dev, elem, dim, at, {}, 1.0)
+    lay, (page, t) = s.cache, divmod(int(s.slots[token]), s.page)
+    o = 2 * lay.quants + lay.scales + (t // 4) * lay.nb * 8 + (t % 4) * 2
+    lay.bytes[page, 0, o:o + 2] = np.array([bad], np.float16).view(np.uint8)
+    check_tail(hip, s, 1.0)
+    assert not np.isfinite(wide(s.run(hip))[:, 0, :32]).any()
+
+
+@pytest.mark.parametrize("elem", ELEMS)
 @pytest.mark.parametrize("dim", [64, 128, 192, 256])
 def test_prompt_keys_beside_a_loud_one(hip, dev, elem, dim):
     """Small keys under a large scale of the scores, and after them one key of 2^6: the rows before

@@ -49,9 +49,9 @@ __device__ __forceinline__ float shift_of(uint32_t any) {
   const float shift = any & 0x70007000u ? 18.0f : kMostShift;
   return any & 0x60006000u ? 10.0f : shift;
 }
-// for those, by the field of the largest one's exponent (fp16's 2^0 is 15; what is not finite is left out)
+// for those, by the field of the largest one's exponent (fp16's 2^0 is 15)
 __device__ __forceinline__ float shift_of_exponent(uint32_t e) {
-  return e < 16 ? kMostShift : 25.0f - static_cast<float>(min(e, 30u));
+  return e < 16 ? kMostShift : 25.0f - static_cast<float>(e);
 }
 // the exponent bits that no scale of the shift's range has, or has to be looked at for
 __device__ __forceinline__ uint32_t bits_over(float shift) {
@@ -390,6 +390,23 @@ template <int NB, int NP> __device__ __forceinline__ void rescale(Row<NB, NP> &r
   row.l *= f;
 }
 
+// The largest exponent's field of a lane's value scales, of the finite ones alone where asked for: one more
+// takes the others' to 0.
+template <int NB, bool kFinite>
+__device__ __forceinline__ uint32_t largest_exponent(const Tokens16<NB> (&t)[2]) {
+  u16x2 most{};
+#pragma unroll
+  for (int i = 0; i < 4 * NB; ++i) {
+    const uint32_t bits = t[i / (2 * NB)].vs.v[i % (2 * NB)] & 0x7c007c00u;
+    u16x2 e = __builtin_bit_cast(u16x2, bits);
+    if constexpr (kFinite)
+      e = (e + u16x2{0x400, 0x400}) & u16x2{0x7c00, 0x7c00};
+    most = __builtin_elementwise_max(most, e);
+  }
+  const uint32_t e = static_cast<uint32_t>(max(most[0], most[1])) >> 10;
+  return kFinite ? max(e, 1u) - 1 : e;
+}
+
 // 32 tokens.  edge (the same in all lanes): not all of them are seen by all rows of the tile; token
 // 4 g + r of half h is seen by this lane's row where bit 4 h + r of `seen` is set.
 template <int NB, int NP>
@@ -437,14 +454,11 @@ __device__ __forceinline__ void attend(Row<NB, NP> &row, Tokens16<NB> (&t)[2], b
   for (int i = 0; i < 2 * NB; ++i)
     any |= t[0].vs.v[i] | t[1].vs.v[i];
   float room = kMostShift;
-  if (__any((any & 0x40004000u) != 0)) {
-    u16x2 most{};
-#pragma unroll
-    for (int i = 0; i < 4 * NB; ++i) {
-      const uint32_t e = t[i / (2 * NB)].vs.v[i % (2 * NB)] & 0x7c007c00u;
-      most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, e));
-    }
-    room = shift_of_exponent(static_cast<uint32_t>(max(most[0], most[1])) >> 10);
+  if (__builtin_expect(__any((any & 0x40004000u) != 0), 0)) {
+    uint32_t e = largest_exponent<NB, false>(t);
+    if (__any(e == 31))  // their block is lost, and is no reason to lose small weights in the others
+      e = largest_exponent<NB, true>(t);
+    room = shift_of_exponent(e);
     if (room >= row.shift)
       any &= ~0x40004000u;  // the shift is theirs already
   }
