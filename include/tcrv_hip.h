@@ -549,6 +549,116 @@ TCRV_HIP_API int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, siz
                                     void *out, size_t out_token, size_t out_head,
                                     void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- between the quantized products of a step (no reference counterpart) ---
+ * Rows of activations go from one quantized product to the next as Q8_0 rows:
+ * tcrv_hip_add_rms_norm adds the residual and leaves the norm as such rows (or in
+ * `elem`), tcrv_hip_gated_q4_0_q8_0 takes them through the first half of a gated
+ * feed-forward and leaves what the down projection takes.  `elem`: as above; rows
+ * are dense in their last dimension, the stride of a token in elements (of Q8_0
+ * rows in bytes).  What is written does not overlap, not itself either, nor what is
+ * read (but for the exact places named): else the results are unspecified.  A call
+ * takes less than 2^24 tokens, else TCRV_HIP_ERR_TOO_LARGE. */
+
+/* h = x + residual (NULL: x), per token
+ *   sum  h rounded to `elem` (NULL: not written; may be residual or x)
+ *   y_i = fl(fl(h_i c) weight_i),  c = fl32(1 / sqrt(mean(h^2) + eps))
+ * y rounded to `elem` (NULL: not written; may be x, or residual where that is not
+ * sum), and as the Q8_0 blocks that tcrv_hip_quantize_row_q8_0 makes of it (q8; NULL:
+ * not written; a partial last block is not written).  weight: n floats (NULL: ones).
+ * h is the f32 sum, not rounded to `elem` first; squares, their mean and its root
+ * are computed in f64: c, and with it every quant, does not depend on an order.
+ * eps >= 0 and finite, else TCRV_HIP_ERR_BAD_SIZE. */
+TCRV_HIP_API int tcrv_hip_add_rms_norm(int elem, const void *x, size_t x_token,
+                                       const void *residual, size_t residual_token, void *sum,
+                                       size_t sum_token, const float *weight, double eps, void *y,
+                                       size_t y_token, uint8_t *q8, size_t q8_token,
+                                       size_t tokens, size_t n, void *stream);
+
+/* out[col][ir] = act(g) u,  g = block dot of gate row ir and activation row col, u
+ * of the up row: gate and up Q4_0 weight rows at stride bx, activations Q8_0 rows at
+ * stride by, as tcrv_hip_q4_0_q8_0_gemm takes them (n / 32 blocks a row, 2-byte
+ * aligned; the two matrices may be the halves of one, or its rows in turn).  Token
+ * major: out (in `elem`; NULL: not written) at col * out_token + ir, q8 (Q8_0 blocks
+ * of 32 ir; NULL: not written) at col * q8_token; a partial last block of nr is not
+ * written.  The quants are those of the f32 values, not of those rounded to `elem`.
+ *   SILU       g / (1 + e^-g)
+ *   GELU_TANH  g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2
+ *   GELU       g (1 + erf(g / sqrt(2))) / 2
+ *   RELU       max(g, 0)
+ * Integer sums of a block are exact, the sums of blocks f32 in an order that follows
+ * the sizes (not the one order of the GEMM); the same call gives the same bits.  An
+ * output whose rows hold a scale that is not finite is NaN or infinite.
+ * nr up to 2^28 - 32 and rows up to 2^31 - 1 bytes, else TCRV_HIP_ERR_TOO_LARGE. */
+enum {
+  TCRV_HIP_ACT_SILU = 0,
+  TCRV_HIP_ACT_GELU_TANH = 1,
+  TCRV_HIP_ACT_GELU = 2,
+  TCRV_HIP_ACT_RELU = 3
+};
+TCRV_HIP_API int tcrv_hip_gated_q4_0_q8_0(int elem, int act, size_t n, void *out,
+                                          size_t out_token, uint8_t *q8, size_t q8_token,
+                                          const uint8_t *gate, const uint8_t *up, size_t bx,
+                                          const uint8_t *vy, size_t by, size_t nr, size_t nc,
+                                          void *stream);
+
+/* ---- drafted tokens over the paged Q4_0 cache (no reference counterpart) ---
+ * A step that checks a tree of drafted tokens a request: the tree's nodes are the
+ * request's new tokens (tcrv_hip_kv_tables lays them out, added[r] nodes), stored in
+ * their slots and attended to at once, each seeing its request's cached tokens, its
+ * ancestors and itself; then the accepted path's rows move up to follow the cached
+ * tokens.  Nodes are numbered within their request, parents before their children. */
+
+/* From each token's parent (a node of its request, below its own number; anything
+ * else: the token follows the cached ones):
+ *   ancestors  [max_tokens][words] of 64 bits: bit i of word w is set where node
+ *              64 w + i is the token or an ancestor of it (nodes from 64 words on have
+ *              no bits); 0 past the last token
+ *   positions  max_tokens: length[r] - the request's nodes + the token's depth, 0
+ *              for one that follows the cached tokens; -1 past the last token
+ * first and length as tcrv_hip_kv_tables writes them.  The outputs overlap neither
+ * each other nor the inputs.  Rotary positions of queries and keys go by `positions`. */
+TCRV_HIP_API int tcrv_hip_tree_tables(const int32_t *parents, const int32_t *first,
+                                      const int32_t *length, size_t requests,
+                                      uint64_t *ancestors, size_t words, int32_t *positions,
+                                      size_t max_tokens, void *stream);
+
+/* tcrv_hip_attn_q4_0 (arguments, types, precision, workspace and checks) where a row
+ * sees of its request's new tokens those that its bits name, and of the cached ones,
+ * length[r] - the request's nodes, all: its token's `words` words of `ancestors`
+ * (8-byte aligned; 64 words >= max_added, else TCRV_HIP_ERR_BAD_SIZE).  Bits past
+ * the token's own are not looked at.  window > 0: of positions p - window + 1 .. p,
+ * where p is the cached tokens' number plus the row's bits up to its own less one, and
+ * a new token's position is that of its place among these bits.  A row whose bits
+ * leave nothing, and no cached token, is zero. */
+TCRV_HIP_API size_t tcrv_hip_attn_tree_q4_0_workspace_bytes(int elem, size_t requests,
+                                                            size_t tokens, size_t max_added,
+                                                            size_t max_length, size_t heads,
+                                                            size_t kv_heads, size_t head_dim);
+TCRV_HIP_API int tcrv_hip_attn_tree_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
+                                         const uint8_t *cache, size_t pages, size_t page_size,
+                                         const int32_t *block_table, size_t table_stride,
+                                         const int32_t *first, const int32_t *length,
+                                         const uint64_t *ancestors, size_t words,
+                                         size_t requests, size_t tokens, size_t max_added,
+                                         size_t max_length, size_t heads, size_t kv_heads,
+                                         size_t head_dim, float scale, size_t window, void *out,
+                                         size_t out_token, size_t out_head, void *workspace,
+                                         size_t workspace_bytes, void *stream);
+
+/* The accepted nodes' keys and values, node path[r * path_stride + k] of request r to
+ * the place of its node k, k < count[r], in place: afterwards the request's cached
+ * tokens are followed by the path's.  A path goes down the tree, so that its nodes
+ * ascend; of one that does not, what the nodes' places hold is unspecified.  Nodes
+ * that the request does not have are skipped, as are places without a page.
+ * count[r] is cut to path_stride, and to the request's nodes; at most max_added
+ * nodes of a request are looked at.  The pages past the kept tokens are free again. */
+TCRV_HIP_API int tcrv_hip_kv_keep_q4_0(uint8_t *cache, size_t pages, size_t page_size,
+                                       const int32_t *block_table, size_t table_stride,
+                                       const int32_t *first, const int32_t *length,
+                                       const int32_t *path, size_t path_stride,
+                                       const int32_t *count, size_t requests, size_t max_added,
+                                       size_t kv_heads, size_t head_dim, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -80,6 +80,9 @@ struct AttnArgs {
   float scale;
   int causal;
   bool q_vec, out_vec;  // groups of 4 values lie on aligned places
+  // of a tree of drafted tokens: which of the new ones a token sees, `words` of 64 bits each
+  const uint64_t *ancestors;
+  size_t words;
 };
 
 template <int n> struct Dwords {
@@ -571,6 +574,39 @@ struct Work {
   }
 };
 
+// What the row of a tree's i-th node sees: cached tokens from `lo` on, and of the request's new ones, whose
+// first is token `tree`, those from `lo` on whose bits are set.
+struct Branch {
+  const uint64_t *bits;
+  int tree, lo;
+  __device__ Branch() {}
+  __device__ Branch(const AttnArgs &a, const Span &span, uint32_t i)
+      : bits(a.ancestors + static_cast<size_t>(span.first + i) * a.words), tree(span.position0), lo(0) {
+    if (!a.window)
+      return;
+    // of the bits up to the row's own, those that the window leaves: the last a.window
+    uint32_t left = a.window;
+    for (int w = static_cast<int>(i >> 6); w >= 0; --w) {
+      uint64_t x = bits[w];
+      if (w == static_cast<int>(i >> 6))
+        x &= ~0ull >> (63 - (i & 63));
+      const uint32_t n = __popcll(x);
+      if (n >= left) {
+        for (uint32_t drop = n - left; drop > 0; --drop)
+          x &= x - 1;
+        lo = tree + 64 * w + __builtin_ctzll(x);
+        return;
+      }
+      left -= n;
+    }
+    // the others are cached tokens; a row without bits takes its own as one
+    lo = max(tree - static_cast<int>(min(left, a.window - 1)), 0);
+  }
+  __device__ bool sees(int t) const {
+    return t < tree || (bits[(t - tree) >> 6] >> ((t - tree) & 63) & 1u);
+  }
+};
+
 template <int kControl, int kLines> __device__ __forceinline__ uint32_t dpp_add(uint32_t x) {
   return x + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), kControl,
                                                                kLines, 0xf, false));
@@ -605,7 +641,8 @@ __device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) {
   return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), lane));
 }
 
-template <int NB, int NP, typename T>
+// kTree: a row sees of its request's new tokens its ancestors, by their bits, in the place of those before it.
+template <int NB, int NP, typename T, bool kTree = false>
 __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16(AttnArgs a) {
   constexpr int D = NB * 32;
   // the waves' rings, and where they meet at the end
@@ -717,8 +754,17 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16
     const int begin = all + static_cast<int>(unit0 << (7 + a.unit_shift));
     const int end = whole ? seen_end
                           : min(seen_end, all + static_cast<int>(unit1 << (7 + a.unit_shift)));
-    const int all_lo = span.lo(a, i1), all_hi = min(span.hi(a, i0), end);  // what every row sees
-    const int my_lo = span.lo(a, mine / a.share), my_hi = min(span.hi(a, mine / a.share), end);
+    // what every row sees: of a tree cached tokens only, whatever the rows' depths, which are no more than
+    // their numbers
+    const int all_lo = span.lo(a, i1);
+    const int all_hi = min(kTree ? span.position0 : span.hi(a, i0), end);
+    Branch branch;
+    int my_lo = span.lo(a, mine / a.share);
+    if constexpr (kTree) {
+      branch = Branch(a, span, mine / a.share);
+      my_lo = branch.lo;
+    }
+    const int my_hi = min(span.hi(a, mine / a.share), end);
 
     const PageHead lay(a.page_size, D);
     const int32_t *const table = a.block_table + static_cast<size_t>(request) * a.table_stride;
@@ -781,7 +827,10 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int at = t0 + 16 * (i >> 2) + 4 * g + (i & 3);
-          seen |= at >= my_lo && at < my_hi && (both >> (i >> 2) & 1u) ? 1u << i : 0u;
+          bool sees = at >= my_lo && at < my_hi && (both >> (i >> 2) & 1u);
+          if constexpr (kTree)
+            sees = sees && branch.sees(at);
+          seen |= sees ? 1u << i : 0u;
         }
       }
       attend<NB, NP>(row, t, edge, seen);
@@ -1754,10 +1803,10 @@ size_t parts_bytes(size_t parts, size_t head_dim) {
 // The shares of the kernel of few rows, for lengths up to max_length; none where no tile has enough
 // tokens to be cut.
 Plan few_plan(size_t requests, size_t max_added, size_t max_length, size_t window, size_t heads,
-              size_t kv_heads, size_t head_dim) {
+              size_t kv_heads, size_t head_dim, size_t most_rows) {
   Plan p{};
   const size_t share = heads / kv_heads;
-  const size_t rows = std::min(max_added * share, few_rows_of(requests, max_added * share, kv_heads));
+  const size_t rows = std::min(max_added * share, most_rows);
   p.tile_rows = tcrv::kRows;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const size_t items = requests * p.tiles * kv_heads;
@@ -1808,34 +1857,38 @@ Plan many_plan(int elem, size_t requests, size_t tokens, size_t max_added, size_
   return p;
 }
 
-// Which of the two kernels a call launches, and the rows up to which the first serves.
+// Which of the two kernels a call launches, and the rows up to which the first serves: all of them of trees.
 struct Kernels {
   bool few, many;
   size_t few_rows;
 };
-Kernels kernels_of(size_t requests, size_t tokens, size_t max_added, size_t heads, size_t kv_heads) {
-  const size_t rows = max_added * (heads / kv_heads), few = few_rows_of(requests, rows, kv_heads);
+Kernels kernels_of(bool tree, size_t requests, size_t tokens, size_t max_added, size_t heads,
+                   size_t kv_heads) {
+  const size_t rows = max_added * (heads / kv_heads);
+  if (tree)
+    return {true, false, rows};
+  const size_t few = few_rows_of(requests, rows, kv_heads);
   if (rows <= few)
     return {true, false, few};
   // one request, or all as long as the longest: none is short
   return {requests > 1 && tokens < requests * max_added, true, few};
 }
 
-template <int NP, typename T>
+template <int NP, typename T, bool kTree>
 void launch_rows16(const AttnArgs &a, size_t head_dim, unsigned groups, hipStream_t st) {
   const dim3 grid(groups), block(tcrv::kWaves * 64);
   switch (head_dim) {
   case 64:
-    tcrv::attn_q4_0_rows16<2, NP, T><<<grid, block, 0, st>>>(a);
+    tcrv::attn_q4_0_rows16<2, NP, T, kTree><<<grid, block, 0, st>>>(a);
     break;
   case 128:
-    tcrv::attn_q4_0_rows16<4, NP, T><<<grid, block, 0, st>>>(a);
+    tcrv::attn_q4_0_rows16<4, NP, T, kTree><<<grid, block, 0, st>>>(a);
     break;
   case 192:
-    tcrv::attn_q4_0_rows16<6, NP, T><<<grid, block, 0, st>>>(a);
+    tcrv::attn_q4_0_rows16<6, NP, T, kTree><<<grid, block, 0, st>>>(a);
     break;
   default:
-    tcrv::attn_q4_0_rows16<8, NP, T><<<grid, block, 0, st>>>(a);
+    tcrv::attn_q4_0_rows16<8, NP, T, kTree><<<grid, block, 0, st>>>(a);
     break;
   }
 }
@@ -1863,7 +1916,7 @@ void launch_tiles(const AttnArgs &a, size_t head_dim, dim3 grid, hipStream_t st)
   }
 }
 
-template <int NP, typename T>
+template <int NP, typename T, bool kTree>
 void launch_all(AttnArgs a, Kernels k, const Plan &few, const Plan &many, size_t head_dim,
                 size_t requests, hipStream_t st) {
   const unsigned n = static_cast<unsigned>(requests);
@@ -1880,14 +1933,14 @@ void launch_all(AttnArgs a, Kernels k, const Plan &few, const Plan &many, size_t
     a.parts = workspace + few.groups * (sizeof(uint4) / sizeof(float));
     a.few_least = 0;
     a.few_most = few_most;
-    launch_rows16<NP, T>(a, head_dim, static_cast<unsigned>(few.launch), st);
+    launch_rows16<NP, T, kTree>(a, head_dim, static_cast<unsigned>(few.launch), st);
     if (few.groups) {
       const size_t rows = std::min(static_cast<size_t>(a.max_added) * a.share, few.tile_rows);
       tcrv::attn_q4_0_join_few<T>
           <<<dim3(a.groups, static_cast<unsigned>(rows)), join_block, 0, st>>>(a, dim);
     }
   }
-  if (k.many) {
+  if (!kTree && k.many) {
     a.plan = reinterpret_cast<uint4 *>(workspace + (k.few ? few.workspace / sizeof(float) : 0));
     a.parts = reinterpret_cast<float *>(a.plan + 1);
     a.tiles = static_cast<uint32_t>(many.tiles);
@@ -1924,34 +1977,31 @@ bool attn_too_large(size_t requests, size_t tokens, size_t max_added, size_t max
          requests * max_added * heads > (size_t{1} << 40);
 }
 
-}  // namespace
-
-extern "C" {
-
-size_t tcrv_hip_attn_q4_0_workspace_bytes(int elem, size_t requests, size_t tokens,
-                                          size_t max_added, size_t max_length, size_t heads,
-                                          size_t kv_heads, size_t head_dim) {
+size_t workspace_bytes_of(bool tree, int elem, size_t requests, size_t tokens, size_t max_added,
+                          size_t max_length, size_t heads, size_t kv_heads, size_t head_dim) {
   if (!tcrv_host::float_elem_bytes(elem) || !attn_sizes_ok(heads, kv_heads, head_dim) ||
       attn_too_large(requests, tokens, max_added, max_length, heads) || !requests || !tokens ||
       !max_added)
     return 0;
-  const Kernels k = kernels_of(requests, tokens, max_added, heads, kv_heads);
+  const Kernels k = kernels_of(tree, requests, tokens, max_added, heads, kv_heads);
   size_t need = 0;
   for (const bool few : {true, false})
     if (few ? k.few : k.many)
-      need += (few ? few_plan(requests, max_added, max_length, 0, heads, kv_heads, head_dim)
+      need += (few ? few_plan(requests, max_added, max_length, 0, heads, kv_heads, head_dim, k.few_rows)
                    : many_plan(elem, requests, tokens, max_added, max_length, 0, heads, kv_heads, head_dim))
                   .workspace;
   return need;
 }
 
-int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
-                       const uint8_t *cache, size_t pages, size_t page_size,
-                       const int32_t *block_table, size_t table_stride, const int32_t *first,
-                       const int32_t *length, size_t requests, size_t tokens, size_t max_added,
-                       size_t max_length, size_t heads, size_t kv_heads, size_t head_dim,
-                       float scale, int causal, size_t window, void *out, size_t out_token,
-                       size_t out_head, void *workspace, size_t workspace_bytes, void *stream) {
+// kTree: the entry of drafted tokens.
+template <bool kTree>
+int attend(int elem, const void *q, size_t q_token, size_t q_head, const uint8_t *cache, size_t pages,
+           size_t page_size, const int32_t *block_table, size_t table_stride, const int32_t *first,
+           const int32_t *length, const uint64_t *ancestors, size_t words, size_t requests,
+           size_t tokens, size_t max_added, size_t max_length, size_t heads, size_t kv_heads,
+           size_t head_dim, float scale, int causal, size_t window, void *out, size_t out_token,
+           size_t out_head, void *workspace, size_t workspace_bytes, void *stream) {
+  constexpr bool tree = kTree;
   using namespace tcrv_host;
   const size_t size = float_elem_bytes(elem);
   if (!size)
@@ -1962,21 +2012,24 @@ int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
     return TCRV_HIP_ERR_BAD_SIZE;
   if (tokens == 0 || requests == 0 || max_added == 0)
     return TCRV_HIP_OK;
-  if (!q || !out || !first || !length || (!cache && pages) || (!block_table && table_stride))
+  if (!q || !out || !first || !length || (!cache && pages) || (!block_table && table_stride) ||
+      (tree && !ancestors))
     return TCRV_HIP_ERR_NULL_POINTER;
-  if (!aligned_to(q, size) || !aligned_to(out, size) || !aligned16(cache) ||
+  if (!aligned_to(ancestors, 8) || !aligned_to(q, size) || !aligned_to(out, size) || !aligned16(cache) ||
       !aligned4(block_table) || !aligned4(first) || !aligned4(length))
     return TCRV_HIP_ERR_MISALIGNED;
   if (attn_too_large(requests, tokens, max_added, max_length, heads) || pages > 0x7fffffffu ||
       table_stride > 0x7fffffffu)
     return TCRV_HIP_ERR_TOO_LARGE;
-  if (!rows_apart(out_token, out_head, tokens, heads, head_dim))
+  if (!rows_apart(out_token, out_head, tokens, heads, head_dim) ||
+      (tree && words < (max_added + 63) / 64))
     return TCRV_HIP_ERR_BAD_SIZE;
   if (pages == 0)
     max_length = 0;  // nothing to read
-  const Kernels k = kernels_of(requests, tokens, max_added, heads, kv_heads);
+  const Kernels k = kernels_of(tree, requests, tokens, max_added, heads, kv_heads);
   const size_t bound = causal ? window : 0;
-  const Plan few = few_plan(requests, max_added, max_length, bound, heads, kv_heads, head_dim);
+  const Plan few =
+      few_plan(requests, max_added, max_length, bound, heads, kv_heads, head_dim, k.few_rows);
   const Plan many =
       many_plan(elem, requests, tokens, max_added, max_length, bound, heads, kv_heads, head_dim);
   // rows16 numbers its tiles in 32 bits; a work-group of the other kernel has two threads a row
@@ -2025,20 +2078,67 @@ int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
              scale,
              causal,
              groups_of_4(q, q_token, q_head, size),
-             groups_of_4(out, out_token, out_head, size)};
+             groups_of_4(out, out_token, out_head, size),
+             ancestors,
+             words};
   hipStream_t st = as_stream(stream);
   switch (elem) {
   case TCRV_HIP_ELEM_F32:
-    launch_all<2, float>(a, k, few, many, head_dim, requests, st);
+    launch_all<2, float, kTree>(a, k, few, many, head_dim, requests, st);
     break;
   case TCRV_HIP_ELEM_F16:
-    launch_all<1, _Float16>(a, k, few, many, head_dim, requests, st);
+    launch_all<1, _Float16, kTree>(a, k, few, many, head_dim, requests, st);
     break;
   default:
-    launch_all<1, tcrv::Bf16>(a, k, few, many, head_dim, requests, st);
+    launch_all<1, tcrv::Bf16, kTree>(a, k, few, many, head_dim, requests, st);
     break;
   }
   return launch_status();
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tcrv_hip_attn_q4_0_workspace_bytes(int elem, size_t requests, size_t tokens,
+                                          size_t max_added, size_t max_length, size_t heads,
+                                          size_t kv_heads, size_t head_dim) {
+  return workspace_bytes_of(false, elem, requests, tokens, max_added, max_length, heads, kv_heads,
+                            head_dim);
+}
+
+size_t tcrv_hip_attn_tree_q4_0_workspace_bytes(int elem, size_t requests, size_t tokens,
+                                               size_t max_added, size_t max_length, size_t heads,
+                                               size_t kv_heads, size_t head_dim) {
+  return workspace_bytes_of(true, elem, requests, tokens, max_added, max_length, heads, kv_heads,
+                            head_dim);
+}
+
+int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
+                       const uint8_t *cache, size_t pages, size_t page_size,
+                       const int32_t *block_table, size_t table_stride, const int32_t *first,
+                       const int32_t *length, size_t requests, size_t tokens, size_t max_added,
+                       size_t max_length, size_t heads, size_t kv_heads, size_t head_dim,
+                       float scale, int causal, size_t window, void *out, size_t out_token,
+                       size_t out_head, void *workspace, size_t workspace_bytes, void *stream) {
+  return attend<false>(elem, q, q_token, q_head, cache, pages, page_size, block_table, table_stride,
+                       first, length, nullptr, 0, requests, tokens, max_added, max_length, heads,
+                       kv_heads, head_dim, scale, causal, window, out, out_token, out_head, workspace,
+                       workspace_bytes, stream);
+}
+
+int tcrv_hip_attn_tree_q4_0(int elem, const void *q, size_t q_token, size_t q_head,
+                            const uint8_t *cache, size_t pages, size_t page_size,
+                            const int32_t *block_table, size_t table_stride, const int32_t *first,
+                            const int32_t *length, const uint64_t *ancestors, size_t words,
+                            size_t requests, size_t tokens, size_t max_added, size_t max_length,
+                            size_t heads, size_t kv_heads, size_t head_dim, float scale,
+                            size_t window, void *out, size_t out_token, size_t out_head,
+                            void *workspace, size_t workspace_bytes, void *stream) {
+  return attend<true>(elem, q, q_token, q_head, cache, pages, page_size, block_table, table_stride,
+                      first, length, ancestors, words, requests, tokens, max_added, max_length, heads,
+                      kv_heads, head_dim, scale, 1, window, out, out_token, out_head, workspace,
+                      workspace_bytes, stream);
 }
 
 }  // extern "C"

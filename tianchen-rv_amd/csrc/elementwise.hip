@@ -4,7 +4,7 @@
 //   a3b dequantize_row_q4_0    (ggml block dequant)
 //   a10 quantize_row_q8_0      (tcrv_rvv.quantize_row_q8_0)
 // plus the library's status/version/synchronize entry points.
-#include "tcrv_hip_internal.h"
+#include "q8_block.h"
 
 namespace {
 
@@ -206,31 +206,6 @@ constexpr int kQzThreads = 256;
 // threads with 2 15.64, 512 slower also without streaming)
 constexpr int kQzPer = 2;
 constexpr int kQzBlocks = kQzPer * kQzThreads / 8;
-
-// Branch-free: the clamp to the i16 range (v_med3_f32) commutes with the
-// rounding, as both bounds are integers; NaN is selected afterwards, since the
-// clamp would map it to a bound.  (Written with branches the compiler gave
-// every element its own exec-mask block: 340 instructions against 271.)
-__device__ __forceinline__ uint32_t quant_byte(float x, float id) {
-  const float v = x * id;
-  const float r = fminf(fmaxf(__builtin_rintf(v), -32768.0f), 32767.0f);  // rint: nearest-even
-  // RVV float->int conversion of NaN gives the largest value
-  const int w = v != v ? 32767 : static_cast<int>(r);
-  return static_cast<uint32_t>(w) & 0xffu;  // narrowing keeps the low byte
-}
-
-// max of v over the 8 lanes of its group: quad_perm [1,0,3,2] and [2,3,0,1]
-// give each quad's max, row_half_mirror pairs lane i with lane 7-i of the
-// other quad (fmaxf is exact and order-free)
-__device__ __forceinline__ float max8(float v) {
-  v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v),
-                                                                  0xB1, 0xf, 0xf, false)));
-  v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v),
-                                                                  0x4E, 0xf, 0xf, false)));
-  v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v),
-                                                                  0x141, 0xf, 0xf, false)));
-  return v;
-}
 
 // kVec: x is 16-byte aligned (128-bit loads); otherwise 4-byte loads.  Each
 // thread quantizes kQzPer blocks' parts; all its loads are issued first

@@ -1,0 +1,221 @@
+// tree.hip -- drafted tokens as a tree: what each of them sees of the others and its position, and the
+// accepted path's rows of the paged Q4_0 cache to the places after the cached tokens.
+#include <algorithm>
+
+#include "kv_cache.h"
+
+namespace tcrv {
+namespace {
+
+// A request's new tokens: where they begin in its step's rows, how many, and the tokens cached before.
+struct Nodes {
+  int first, count, cached;
+  __device__ Nodes(const int32_t *begins, const int32_t *length, uint32_t request, uint32_t most) {
+    const int begin = max(begins[request], 0), end = max(begins[request + 1], 0);
+    first = begin;
+    count = max(min(end, static_cast<int>(most)) - begin, 0);
+    cached = max(length[request], 0) - max(end - begin, 0);
+  }
+};
+
+constexpr int kTreeThreads = 256;
+constexpr int kTreeHeld = 8192;  // parents in LDS
+
+// A work-group a request, a thread a node, which walks up its ancestors: their numbers go down, so that
+// the words of its bits are made one after the other.  Parents are fetched once, into LDS: a walk is a
+// chain of reads.  The last work-group fills what lies past the last token.
+__global__ __launch_bounds__(kTreeThreads) void tree_tables(const int32_t *parents,
+                                                            const int32_t *first,
+                                                            const int32_t *length,
+                                                            uint32_t requests, uint64_t *ancestors,
+                                                            size_t words, int32_t *positions,
+                                                            uint32_t tokens) {
+  __shared__ int32_t s_parent[kTreeHeld];
+  if (blockIdx.x == requests) {
+    const uint32_t end = requests ? max(first[requests], 0) : 0;
+    for (uint32_t i = end + threadIdx.x; i < tokens; i += kTreeThreads) {
+      positions[i] = -1;
+      for (size_t w = 0; w < words; ++w)
+        ancestors[i * words + w] = 0;
+    }
+    return;
+  }
+  const Nodes nodes(first, length, blockIdx.x, tokens);
+  const int32_t *const mine = parents + nodes.first;
+  const int held = min(nodes.count, kTreeHeld);
+  for (int i = threadIdx.x; i < held; i += kTreeThreads)
+    s_parent[i] = mine[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < nodes.count; i += kTreeThreads) {
+    uint64_t *const row = ancestors + (static_cast<size_t>(nodes.first) + i) * words;
+    int at = i, depth = -1;
+    size_t word = words;  // those from here on are written
+    uint64_t bits = 0;
+    while (at >= 0) {
+      ++depth;
+      const size_t w = static_cast<size_t>(at) >> 6;
+      while (word > w) {  // down to this node's
+        if (word < words)
+          row[word] = bits;
+        bits = 0;
+        --word;
+        if (word > w)
+          row[word] = 0;
+      }
+      if (w == word)
+        bits |= 1ull << (at & 63);
+      const int up = at < held ? s_parent[at] : mine[at];
+      at = up < at ? up : -1;
+    }
+    if (word < words)
+      row[word] = bits;
+    while (word > 0) {
+      --word;
+      row[word] = 0;
+    }
+    positions[nodes.first + i] = nodes.cached + depth;
+  }
+}
+
+// A row's bytes of one head in units of 16 bits: keys' quants lie side by side, the others 8 bytes apart.
+struct RowUnits {
+  uint32_t nb, keys, all;
+  __device__ explicit RowUnits(uint32_t head_dim)
+      : nb(head_dim / kQK), keys(head_dim / 4), all(2 * (keys + nb)) {}
+  __device__ uint32_t at(const PageHead &lay, uint32_t token, uint32_t unit) const {
+    if (unit < keys)
+      return lay.key(nb, token, 0, 0) + 2 * unit;
+    unit -= keys;
+    if (unit < nb)
+      return lay.key_scale(nb, token, unit);
+    unit -= nb;
+    if (unit < keys)
+      return lay.value(nb, token, unit / (nb / 2), unit % (nb / 2));
+    return lay.value_scale(nb, token, unit - keys);
+  }
+};
+
+struct KeepArgs {
+  uint8_t *cache;
+  const int32_t *block_table, *first, *length, *path, *count;
+  size_t table_stride, path_stride;
+  uint32_t pages, page_size, max_added, kv_heads, head_dim;
+};
+
+constexpr int kKeepThreads = 256, kKeepTokens = 16;
+
+// A work-group a request and head takes kKeepTokens nodes of the path at a time: their rows into LDS, then
+// from there to their places.  Nodes ascend and lie at or past their new places, so that what is still
+// to be read lies past what has been written.
+__global__ __launch_bounds__(kKeepThreads) void kv_keep_q4_0(KeepArgs a) {
+  __shared__ uint16_t s_row[kKeepTokens * (2 * (256 / 4 + 256 / kQK))];
+  const uint32_t request = blockIdx.x, head = blockIdx.y;
+  const Nodes nodes(a.first, a.length, request, 0x7fffffffu);
+  const int most = min(nodes.count, static_cast<int>(a.max_added));
+  const int32_t *const path = a.path + request * a.path_stride;
+  const int count = min(a.count[request], static_cast<int>(min(
+                                              static_cast<size_t>(most), a.path_stride)));
+  const PageHead lay(a.page_size, a.head_dim);
+  const RowUnits units(a.head_dim);
+  const int32_t *const table = a.block_table + request * a.table_stride;
+  // the head's part of the page of the request's token t, and its place there; nullptr where there is none
+  const auto place = [&](int64_t t, uint32_t &token) -> uint8_t * {
+    if (t < 0 || static_cast<size_t>(t) / a.page_size >= a.table_stride)
+      return nullptr;
+    const uint32_t column = static_cast<uint32_t>(t) / a.page_size;
+    token = static_cast<uint32_t>(t) - column * a.page_size;
+    const uint32_t page = static_cast<uint32_t>(table[column]);
+    return page < a.pages ? a.cache + (static_cast<size_t>(page) * a.kv_heads + head) * lay.bytes()
+                          : nullptr;
+  };
+  for (int k0 = 0; k0 < count; k0 += kKeepTokens) {
+    const uint32_t all = min(count - k0, kKeepTokens) * units.all;
+    const auto moves = [&](uint32_t i, bool write) {
+      const int k = k0 + static_cast<int>(i / units.all);
+      const uint32_t unit = i % units.all;
+      const int node = path[k];
+      if (node == k || node < 0 || node >= most)
+        return;
+      uint32_t from = 0, to = 0;
+      uint8_t *const source = place(static_cast<int64_t>(nodes.cached) + node, from);
+      uint8_t *const target = place(static_cast<int64_t>(nodes.cached) + k, to);
+      if (!source || !target)
+        return;
+      if (write)
+        *reinterpret_cast<uint16_t *>(target + units.at(lay, to, unit)) = s_row[i];
+      else
+        s_row[i] = *reinterpret_cast<const uint16_t *>(source + units.at(lay, from, unit));
+    };
+    for (uint32_t i = threadIdx.x; i < all; i += kKeepThreads)
+      moves(i, false);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < all; i += kKeepThreads)
+      moves(i, true);
+    __syncthreads();
+  }
+}
+
+}  // namespace
+}  // namespace tcrv
+
+extern "C" {
+
+int tcrv_hip_tree_tables(const int32_t *parents, const int32_t *first, const int32_t *length,
+                         size_t requests, uint64_t *ancestors, size_t words, int32_t *positions,
+                         size_t max_tokens, void *stream) {
+  using namespace tcrv_host;
+  if (max_tokens == 0)
+    return TCRV_HIP_OK;
+  if (max_tokens > 0x7fffffffu || requests >= kMostGroups || words > 0x7fffffffu)
+    return TCRV_HIP_ERR_TOO_LARGE;
+  if (words == 0)
+    return TCRV_HIP_ERR_BAD_SIZE;
+  if (!ancestors || !positions || (requests && (!parents || !first || !length)))
+    return TCRV_HIP_ERR_NULL_POINTER;
+  if (!aligned_to(ancestors, 8) || !aligned4(positions) || !aligned4(parents) || !aligned4(first) ||
+      !aligned4(length))
+    return TCRV_HIP_ERR_MISALIGNED;
+  tcrv::tree_tables<<<dim3(static_cast<unsigned>(requests) + 1), dim3(tcrv::kTreeThreads), 0,
+                      as_stream(stream)>>>(parents, first, length, static_cast<uint32_t>(requests),
+                                           ancestors, words, positions,
+                                           static_cast<uint32_t>(max_tokens));
+  return launch_status();
+}
+
+int tcrv_hip_kv_keep_q4_0(uint8_t *cache, size_t pages, size_t page_size, const int32_t *block_table,
+                          size_t table_stride, const int32_t *first, const int32_t *length,
+                          const int32_t *path, size_t path_stride, const int32_t *count,
+                          size_t requests, size_t max_added, size_t kv_heads, size_t head_dim,
+                          void *stream) {
+  using namespace tcrv_host;
+  if (!cache_sizes_ok(page_size, kv_heads, head_dim))
+    return TCRV_HIP_ERR_BAD_SIZE;
+  if (requests == 0 || max_added == 0 || path_stride == 0 || pages == 0 || table_stride == 0)
+    return TCRV_HIP_OK;
+  if (requests > kMostGroups || max_added > 0x7fffffffu || pages > 0x7fffffffu ||
+      table_stride > 0x7fffffffu)
+    return TCRV_HIP_ERR_TOO_LARGE;
+  if (!cache || !block_table || !first || !length || !path || !count)
+    return TCRV_HIP_ERR_NULL_POINTER;
+  if (!aligned16(cache) || !aligned4(block_table) || !aligned4(first) || !aligned4(length) ||
+      !aligned4(path) || !aligned4(count))
+    return TCRV_HIP_ERR_MISALIGNED;
+  const tcrv::KeepArgs a{cache,
+                         block_table,
+                         first,
+                         length,
+                         path,
+                         count,
+                         table_stride,
+                         path_stride,
+                         static_cast<uint32_t>(pages),
+                         static_cast<uint32_t>(page_size),
+                         static_cast<uint32_t>(max_added),
+                         static_cast<uint32_t>(kv_heads),
+                         static_cast<uint32_t>(head_dim)};
+  tcrv::kv_keep_q4_0<<<dim3(static_cast<unsigned>(requests), static_cast<unsigned>(kv_heads)),
+                       dim3(tcrv::kKeepThreads), 0, as_stream(stream)>>>(a);
+  return launch_status();
+}
+
+}  // extern "C"

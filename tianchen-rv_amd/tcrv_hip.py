@@ -36,6 +36,7 @@ ERR_SCRATCH_LIMIT = -6
 FLOAT_ELEM = {"f32": 7, "f16": 9, "bf16": 10}
 ROPE_LAYOUT = {"interleaved": 0, "half": 1}
 ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+ACTIVATION = {"silu": 0, "gelu_tanh": 1, "gelu": 2, "relu": 3}
 
 BINARY_ADD, BINARY_SUB, BINARY_MUL = 0, 1, 2
 ELEM = {"i8": 0, "u8": 1, "i16": 2, "u16": 3, "i32": 4, "u32": 5, "i64": 6, "f32": 7, "f64": 8}
@@ -102,6 +103,14 @@ SIGNATURES = {
                               _p],
     "tcrv_hip_attn_q4_0": [_int, _p, _sz, _sz, _p, _sz, _sz, _p, _sz, _p, _p, _sz, _sz, _sz, _sz,
                            _sz, _sz, _sz, _f32, _int, _sz, _p, _sz, _sz, _p, _sz, _p],
+    "tcrv_hip_add_rms_norm": [_int, _p, _sz, _p, _sz, _p, _sz, _p, _f64, _p, _sz, _p, _sz, _sz,
+                              _sz, _p],
+    "tcrv_hip_gated_q4_0_q8_0": [_int, _int, _sz, _p, _sz, _p, _sz, _p, _p, _sz, _p, _sz, _sz, _sz,
+                                 _p],
+    "tcrv_hip_tree_tables": [_p, _p, _p, _sz, _p, _sz, _p, _sz, _p],
+    "tcrv_hip_attn_tree_q4_0": [_int, _p, _sz, _sz, _p, _sz, _sz, _p, _sz, _p, _p, _p, _sz, _sz, _sz,
+                                _sz, _sz, _sz, _sz, _sz, _f32, _sz, _p, _sz, _sz, _p, _sz, _p],
+    "tcrv_hip_kv_keep_q4_0": [_p, _sz, _sz, _p, _sz, _p, _p, _p, _sz, _p, _sz, _sz, _sz, _sz, _p],
 }
 # size queries (return size_t)
 SIZE_FUNCS = {"tcrv_hip_gemm_tiles_bytes": [_sz, _sz],
@@ -109,7 +118,9 @@ SIZE_FUNCS = {"tcrv_hip_gemm_tiles_bytes": [_sz, _sz],
               "tcrv_hip_q4_0_q8_0_gemm_workspace_bytes": [_sz, _sz, _sz],
               "tcrv_hip_q8_0_q8_0_gemm_noalloc_max_bytes": [],
               "tcrv_hip_kv_q4_0_page_bytes": [_sz, _sz, _sz],
-              "tcrv_hip_attn_q4_0_workspace_bytes": [_int, _sz, _sz, _sz, _sz, _sz, _sz, _sz]}
+              "tcrv_hip_attn_q4_0_workspace_bytes": [_int, _sz, _sz, _sz, _sz, _sz, _sz, _sz],
+              "tcrv_hip_attn_tree_q4_0_workspace_bytes": [_int, _sz, _sz, _sz, _sz, _sz, _sz,
+                                                          _sz]}
 STRING_FUNCS = {"tcrv_hip_status_string": [_int], "tcrv_hip_version": []}
 
 _lib: Optional[ctypes.CDLL] = None
@@ -482,6 +493,55 @@ def attn_q4_0(elem: str, q, q_token: int, q_head: int, cache, pages: int, page_s
                 block_table, table_stride, first, length, requests, tokens, max_added, max_length,
                 heads, kv_heads, head_dim, scale, causal, window, out, out_token, out_head, ws,
                 ws_bytes, _stream(stream))
+
+
+# ---- between the quantized products of a step, and drafted tokens over the cache.  act is a key of
+# ACTIVATION; None where an output is not wanted.
+
+def add_rms_norm(elem: str, x, x_token: int, residual, residual_token: int, total, total_token: int,
+                 weight, eps: float, y, y_token: int, q8, q8_token: int, tokens: int, n: int,
+                 stream=None):
+    return call("tcrv_hip_add_rms_norm", FLOAT_ELEM[elem], x, x_token, residual, residual_token, total,
+                total_token, weight, eps, y, y_token, q8, q8_token, tokens, n, _stream(stream))
+
+
+def gated_q4_0_q8_0(elem: str, act: str, n: int, out, out_token: int, q8, q8_token: int, gate, up,
+                    bx: int, vy, by: int, nr: int, nc: int, stream=None):
+    return call("tcrv_hip_gated_q4_0_q8_0", FLOAT_ELEM[elem], ACTIVATION[act], n, out, out_token, q8,
+                q8_token, gate, up, bx, vy, by, nr, nc, _stream(stream))
+
+
+def tree_tables(parents, first, length, requests: int, ancestors, words: int, positions,
+                max_tokens: int, stream=None):
+    return call("tcrv_hip_tree_tables", parents, first, length, requests, ancestors, words, positions,
+                max_tokens, _stream(stream))
+
+
+def attn_tree_q4_0_workspace_bytes(elem: str, requests: int, tokens: int, max_added: int,
+                                   max_length: int, heads: int, kv_heads: int,
+                                   head_dim: int) -> int:
+    return load().tcrv_hip_attn_tree_q4_0_workspace_bytes(FLOAT_ELEM[elem], requests, tokens,
+                                                          max_added, max_length, heads, kv_heads,
+                                                          head_dim)
+
+
+def attn_tree_q4_0(elem: str, q, q_token: int, q_head: int, cache, pages: int, page_size: int,
+                   block_table, table_stride: int, first, length, ancestors, words: int,
+                   requests: int, tokens: int, max_added: int, max_length: int, heads: int,
+                   kv_heads: int, head_dim: int, scale: float, window: int, out, out_token: int,
+                   out_head: int, ws=None, ws_bytes: int = 0, stream=None):
+    return call("tcrv_hip_attn_tree_q4_0", FLOAT_ELEM[elem], q, q_token, q_head, cache, pages,
+                page_size, block_table, table_stride, first, length, ancestors, words, requests,
+                tokens, max_added, max_length, heads, kv_heads, head_dim, scale, window, out,
+                out_token, out_head, ws, ws_bytes, _stream(stream))
+
+
+def kv_keep_q4_0(cache, pages: int, page_size: int, block_table, table_stride: int, first, length,
+                 path, path_stride: int, count, requests: int, max_added: int, kv_heads: int,
+                 head_dim: int, stream=None):
+    return call("tcrv_hip_kv_keep_q4_0", cache, pages, page_size, block_table, table_stride, first,
+                length, path, path_stride, count, requests, max_added, kv_heads, head_dim,
+                _stream(stream))
 
 
 def synchronize(stream=None):
