@@ -51,7 +51,8 @@ GATED = dict(elem=F32, act=0, n=4096, out=A, out_token=11008, q8=B, q8_token=116
     (ALIGN, dict(q8=B + 1)), (ALIGN, dict(q8_token=11697)), (ALIGN, dict(gate=C + 1)),
     (ALIGN, dict(up=D + 1)), (ALIGN, dict(vy=E + 1)), (ALIGN, dict(bx=2305)),
     (ALIGN, dict(by=4353)), (LARGE, dict(nr=0x80000000, out_token=1 << 33, q8_token=1 << 33)),
-    (LARGE, dict(nc=1 << 24)), (LARGE, dict(n=1 << 36)), (OK, dict(nr=0)), (OK, dict(nc=0)),
+    (LARGE, dict(nc=1 << 24)), (LARGE, dict(n=1 << 36)), (LARGE, dict(bx=(1 << 26) + 2)),
+    (LARGE, dict(by=(1 << 26) + 2)), (LARGE, dict(n=1 << 26)), (OK, dict(nr=0)), (OK, dict(nc=0)),
     (OK, dict(nr=0, out=0, q8=0, gate=0, up=0, vy=0)),
 ])
 def test_gated(want, changed):
@@ -150,8 +151,8 @@ def attn(requests, tokens, added, length=16, heads=1, kv=1, dim=64):
 
 @pytest.mark.parametrize("call,want", [
     (norm(MOST, 4096), OK), (norm(MOST, 64), OK), (norm(MOST, 1 << 20), OK),
-    (gated(64, MOST), OK), (gated(0xfffffe0, 1), OK), (gated(0xfffffe0, 5), OK),
-    (gated(0xfffffe0, MOST), LARGE), (gated(0xfffffe1, 1), LARGE),
+    (gated(64, MOST), OK), (gated(32, MOST), OK), (gated(1, MOST), OK), (gated(0x3fffffc, 1), OK), (gated(0x3fffffc, 5), OK),
+    (gated(0x3fffffc, MOST), LARGE), (gated(0x3fffffd, 1), LARGE),
     (("tcrv_hip_tree_tables", (P, Q, R, MOST - 1, S, 1, T, 0x7fffffff)), OK),
     (("tcrv_hip_kv_keep_q4_0", (P, 64, 16, Q, 8, R, S, T, 8, U, MOST, 8, 65535, 64)), OK),
     (attn(MOST, MOST, 1), OK), (attn(MOST + 1, MOST + 1, 1), LARGE),

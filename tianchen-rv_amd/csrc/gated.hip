@@ -3,6 +3,8 @@
 //
 // Both sums of a block are integers (|sum| <= 32 8 128), exact in whatever order; each is scaled by the
 // weights' and the token's scale and added in f32.
+#include <type_traits>
+
 #include "kv_cache.h"
 #include "mfma_fold.h"
 #include "q8_block.h"
@@ -11,6 +13,7 @@ namespace tcrv {
 namespace {
 
 typedef uint32_t u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32a2 __attribute__((aligned(2)));
 
 struct GatedArgs {
   const uint8_t *gate, *up, *vy;
@@ -39,7 +42,7 @@ __device__ __forceinline__ float activation(float g, int act) {
 }
 
 // Lane `part` of eight with four of the 32 outputs from feature `at` on, of one token.
-template <typename T>
+template <typename T, bool kBlocks = true>
 __device__ __forceinline__ void emit(const GatedArgs &a, size_t token, uint32_t at, int part,
                                      const float (&v)[4]) {
   const uint32_t f = at + 4 * part;
@@ -54,13 +57,10 @@ __device__ __forceinline__ void emit(const GatedArgs &a, size_t token, uint32_t 
           to[i] = narrow<T>(v[i]);
     }
   }
-  if (a.q8 && at + kQK <= a.nr)
+  if (kBlocks && a.q8 && at + kQK <= a.nr)
     store_q8_part(a.q8 + token * a.q8_token + static_cast<size_t>(at / kQK) * kQ8Bytes, part, v);
 }
 
-// ---------------------------------------------------------------------------
-// A few tokens: a work-group takes 32 features, a wave kF of them, a lane one block in 64 of their rows.
-// ---------------------------------------------------------------------------
 struct Q4Block {
   u32x4a2 q;
   uint16_t d;
@@ -78,162 +78,226 @@ __device__ __forceinline__ Q8Block load_q8(const uint8_t *p) {
           *reinterpret_cast<const uint16_t *>(p)};
 }
 
+// ---------------------------------------------------------------------------
+// One token: a wave takes a feature, a lane a pair of the blocks of its two rows (or the one that they have).  A
+// work-group is four features; of the 32 of a Q8_0 block (kBlocks) its sixteen waves take two each.
+// ---------------------------------------------------------------------------
+constexpr int one_waves(bool blocks) { return blocks ? 16 : 4; }
+
+// The sum over the lanes, in the last one.
 __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1)
-    v += __shfl_xor(v, m);
+  const auto add = [&](auto control, auto lines) __attribute__((always_inline)) {
+    v += __builtin_bit_cast(
+        float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(control)::value,
+                                           decltype(lines)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());  // 1, 2, 4, 8 before, in 16
+  add(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+  add(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+  add(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+  add(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());  // the last of the 16 before
+  add(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());
   return v;
 }
 
-template <typename T, int kCols, int kF>
-__global__ __launch_bounds__(32 / kF * 64) void gated_few(GatedArgs a) {
-  __shared__ float s_out[kCols][kQK];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t at = blockIdx.x * kQK, f0 = at + wave * kF;
-  const uint8_t *row[2 * kF];
+// sum of (n - 8) y over a block: 16 bytes of quants n, 32 of y, and -8 times the sum of y
+__device__ __forceinline__ float block_sum(const uint32_t (&q)[4], const uint32_t (&y)[8], int seed) {
+  int sum = seed;
 #pragma unroll
-  for (int f = 0; f < kF; ++f) {
-    const size_t r = min(f0 + f, a.nr - 1);
-    row[2 * f] = a.gate + r * a.bx;
-    row[2 * f + 1] = a.up + r * a.bx;
+  for (int k = 0; k < 4; ++k) {
+    sum = sdot4(q[k] & 0x0f0f0f0fu, y[k], sum);
+    sum = sdot4(q[k] >> 4 & 0x0f0f0f0fu, y[k + 4], sum);
   }
-  float acc[kCols][2 * kF] = {};
-  for (uint32_t b0 = 0; b0 < a.nb; b0 += 64) {
-    const uint32_t b = min(b0 + lane, a.nb - 1);
-    const bool live = b0 + lane < a.nb;
-    Q4Block w[2 * kF];
+  return static_cast<float>(sum);
+}
+
+__device__ __forceinline__ int seed_of(const uint32_t (&y)[8]) {
+  int sum = 0;
 #pragma unroll
-    for (int r = 0; r < 2 * kF; ++r)
-      w[r] = load_q4(row[r] + static_cast<size_t>(b) * kQ4Bytes);
+  for (int k = 0; k < 8; ++k)
+    sum = sdot4(y[k], 0x01010101u, sum);
+  return -8 * sum;
+}
+
+template <typename T, bool kPairs, bool kBlocks>
+__global__ __launch_bounds__(one_waves(kBlocks) * 64) void gated_one(GatedArgs a) {
+  constexpr int kWaves = one_waves(kBlocks), kTurns = kBlocks ? 2 : 1, kFeatures = kWaves * kTurns;
+  __shared__ float s_out[kFeatures];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t at = blockIdx.x * kFeatures;
+  const uint32_t items = kPairs ? (a.nb + 1) / 2 : a.nb;
+  for (int turn = 0; turn < kTurns; ++turn) {
+    const size_t feature = min(at + turn * kWaves + wave, a.nr - 1);
+    const uint8_t *const row[2] = {a.gate + feature * a.bx, a.up + feature * a.bx};
+    float acc[2] = {};
+    for (uint32_t i0 = 0; i0 < items; i0 += 64) {
+      const uint32_t i = min(i0 + lane, items - 1);
+      const bool live = i0 + lane < items;
+      if constexpr (kPairs) {
+        // an odd number's last block is the second of the pair with the one before it
+        const uint32_t b = min(2 * i, a.nb - 2);
+        uint32_t w[2][9], y[17];
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-      const Q8Block y = load_q8(a.vy + c * a.by + static_cast<size_t>(b) * kQ8Bytes);
-      int seed = 0;  // the quants are n - 8
+        for (int r = 0; r < 2; ++r) {
+          const u32a2 *const p = reinterpret_cast<const u32a2 *>(row[r] + b * kQ4Bytes);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        seed = sdot4(y.q[0][k], 0x01010101u, seed);
-        seed = sdot4(y.q[1][k], 0x01010101u, seed);
-      }
-      const float dy = live ? fp16_bits_to_f32(y.d) : 0.0f;
-#pragma unroll
-      for (int r = 0; r < 2 * kF; ++r) {
-        int sum = -8 * seed;
+          for (int k = 0; k < 2; ++k) {
+            const u32x4a2 v = *reinterpret_cast<const u32x4a2 *>(p + 4 * k);
+            w[r][4 * k] = v.x;
+            w[r][4 * k + 1] = v.y;
+            w[r][4 * k + 2] = v.z;
+            w[r][4 * k + 3] = v.w;
+          }
+          w[r][8] = p[8];
+        }
+        const u32a2 *const p = reinterpret_cast<const u32a2 *>(a.vy + b * kQ8Bytes);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          sum = sdot4(w[r].q[k] & 0x0f0f0f0fu, y.q[0][k], sum);
-          sum = sdot4(w[r].q[k] >> 4 & 0x0f0f0f0fu, y.q[1][k], sum);
+          const u32x4a2 v = *reinterpret_cast<const u32x4a2 *>(p + 4 * k);
+          y[4 * k] = v.x;
+          y[4 * k + 1] = v.y;
+          y[4 * k + 2] = v.z;
+          y[4 * k + 3] = v.w;
         }
-        acc[c][r] = fmaf(static_cast<float>(sum) * fp16_bits_to_f32(w[r].d), dy, acc[c][r]);
+        y[16] = p[16];
+        // the even block's quants lie 2 bytes off a dword, the odd one's on one
+        uint32_t even[8], odd[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          even[k] = funnel16(y[k], y[k + 1]);
+          odd[k] = y[k + 9];
+        }
+        const int even_seed = seed_of(even), odd_seed = seed_of(odd);
+        const float even_d = live && b == 2 * i ? fp16_bits_to_f32(y[0] & 0xffffu) : 0.0f;
+        const float odd_d = live ? fp16_bits_to_f32(y[8] >> 16) : 0.0f;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t e[4] = {funnel16(w[r][0], w[r][1]), funnel16(w[r][1], w[r][2]),
+                                 funnel16(w[r][2], w[r][3]), funnel16(w[r][3], w[r][4])};
+          const uint32_t o[4] = {w[r][5], w[r][6], w[r][7], w[r][8]};
+          acc[r] = fmaf(block_sum(e, even, even_seed) * fp16_bits_to_f32(w[r][0] & 0xffffu), even_d,
+                        acc[r]);
+          acc[r] = fmaf(block_sum(o, odd, odd_seed) * fp16_bits_to_f32(w[r][4] >> 16), odd_d, acc[r]);
+        }
+      } else {
+        const Q4Block w[2] = {load_q4(row[0] + i * kQ4Bytes), load_q4(row[1] + i * kQ4Bytes)};
+        const Q8Block b = load_q8(a.vy + i * kQ8Bytes);
+        uint32_t y[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          y[k] = b.q[0][k];
+          y[k + 4] = b.q[1][k];
+        }
+        const int seed = seed_of(y);
+        const float d = live ? fp16_bits_to_f32(b.d) : 0.0f;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t q[4] = {w[r].q.x, w[r].q.y, w[r].q.z, w[r].q.w};
+          acc[r] = fmaf(block_sum(q, y, seed) * fp16_bits_to_f32(w[r].d), d, acc[r]);
+        }
       }
     }
+    const float g = lanes_sum(acc[0]), u = lanes_sum(acc[1]);
+    if (lane == 63)
+      s_out[turn * kWaves + wave] = activation(g, a.act) * u;
   }
-#pragma unroll
-  for (int c = 0; c < kCols; ++c)
-#pragma unroll
-    for (int f = 0; f < kF; ++f) {
-      const float g = lanes_sum(acc[c][2 * f]), u = lanes_sum(acc[c][2 * f + 1]);
-      if (lane == 0)
-        s_out[c][wave * kF + f] = activation(g, a.act) * u;
-    }
   __syncthreads();
-  if (threadIdx.x < 8 * kCols) {
-    const int c = threadIdx.x >> 3, part = threadIdx.x & 7;
-    const float v[4] = {s_out[c][4 * part], s_out[c][4 * part + 1], s_out[c][4 * part + 2],
-                        s_out[c][4 * part + 3]};
-    emit<T>(a, c, at, part, v);
+  if (threadIdx.x < kFeatures / 4) {
+    const int part = threadIdx.x;
+    const float v[4] = {s_out[4 * part], s_out[4 * part + 1], s_out[4 * part + 2],
+                        s_out[4 * part + 3]};
+    emit<T, kBlocks>(a, 0, at, part, v);
   }
 }
 
 // ---------------------------------------------------------------------------
-// More tokens: kFT x kNT tiles of 32 features x 32 tokens a work-group, kKS waves a tile, which share out
-// its blocks.  A wave holds the gate's and the up projection's sums of its tile, so that they meet in its
-// registers.  The rows of kCB blocks are laid out in LDS as int8, the next ones loaded meanwhile.
+// Prompts: 32 kFT features x 128 tokens a work-group of eight waves, a wave kFW tiles of 32 features x 32 tokens
+// of both projections, so that their sums meet in its registers.  The rows of kCB blocks are laid out in LDS
+// as int8, the next ones on their way in registers.
 //
 // v_mfma_i32_32x32x32_i8 takes a block at a time, tokens as its rows, so that a lane holds one feature and
-// 16 tokens: a weight's scale is one value a lane.  Its accumulator starts at the bits of M = 1.5 2^23:
-// read as floats its results are M + sum exactly, and fma(M + sum, d, -M d) is the scaled sum, rounded once.
+// 16 tokens: a weight's scale is one value a lane, and the tokens' 16 serve 2 kFW products.  Quants stay
+// in the upper half of their bytes, 16 (n - 8) with a flipped top bit.  The accumulator starts at the bits of
+// M = 1.5 2^23: read as floats its results are M + sum exactly (|sum| <= 16 32 8 128 < 2^22), and fma(M + sum,
+// d, -M d) is the scaled sum, rounded once.
 // ---------------------------------------------------------------------------
-template <int kFT, int kNT, int kKS, int kCB> struct Tiles {
-  static constexpr int kWaves = kFT * kNT * kKS, kThreads = kWaves * 64;
-  static constexpr int kWRows = 64 * kFT, kYRows = 32 * kNT, kRows = kWRows + kYRows;
-  static constexpr int kRow = kCB * kQK + 16;  // 16-byte reads of 16 neighbouring rows meet no bank twice
+constexpr int kTileThreads = 512, kTileTokens = 128;
+
+template <int kFT> struct Tiles {
+  static constexpr int kCB = 4, kFW = kFT * (kTileTokens / 32) / (kTileThreads / 64);
+  static constexpr int kWRows = 64 * kFT, kRows = kWRows + kTileTokens;
+  static constexpr int kRow = kCB * kQK + 16;  // 16 bytes of 16 neighbouring rows in banks of their own
   static constexpr int kQuants = kRows * kRow, kStage = kQuants + kCB * kRows * 4;
-  static constexpr int kWTasks = (kWRows * kCB + kThreads - 1) / kThreads;
-  static constexpr int kYTasks = (kYRows * kCB + kThreads - 1) / kThreads;
-  static constexpr int kParts = kKS > 1 ? kWaves * 16 * 64 * 4 : 0;  // of one projection's sums
-  static constexpr int kOutRow = kFT * 32 + 4;
-  static constexpr int kOut = kYRows * kOutRow * 4;
-  static constexpr int kLds = 2 * kStage > kParts + kOut ? 2 * kStage : kParts + kOut;
+  static constexpr int kWTasks = kWRows * kCB / kTileThreads;
+  static constexpr int kYTasks = kTileTokens * kCB / kTileThreads;
+  static constexpr int kOutRow = kFT * 32 + 4, kOut = kTileTokens * kOutRow * 4;
+  static constexpr int kLds = 2 * kStage > kOut ? 2 * kStage : kOut;
+  static __device__ __forceinline__ int at(int r, int b) { return r * kRow + b * kQK; }
 };
 
-template <typename T, int kFT, int kNT, int kKS, int kCB>
-__global__ __launch_bounds__((Tiles<kFT, kNT, kKS, kCB>::kThreads)) void gated_tiles(GatedArgs a) {
-  using S = Tiles<kFT, kNT, kKS, kCB>;
+template <typename T, int kFT>
+__global__ __launch_bounds__(kTileThreads, 2) void gated_tiles(GatedArgs a) {
+  using S = Tiles<kFT>;
+  constexpr int kCB = S::kCB, kFW = S::kFW;
   __shared__ __align__(16) uint8_t lds[S::kLds];
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ks = wave % kKS, nt = wave / kKS % kNT, ft = wave / (kKS * kNT);
+  const int nt = wave & 3, ft = (wave >> 2) * kFW;
   uint32_t tm, tn;
-  tile_of(blockIdx.x, (a.nr + 32 * kFT - 1) / (32 * kFT), (a.nc + 32 * kNT - 1) / (32 * kNT), tm, tn);
-  const uint32_t m0 = tm * (32 * kFT), n0 = tn * (32 * kNT);
+  tile_of(blockIdx.x, (a.nr + 32 * kFT - 1) / (32 * kFT), (a.nc + kTileTokens - 1) / kTileTokens, tm, tn);
+  const uint32_t m0 = tm * (32 * kFT), n0 = tn * kTileTokens;
 
   // The thread's blocks of a chunk: block t % kCB of row t / kCB.  Weight rows by tiles: 32 of the
   // gate, 32 of the up projection.
+  const int block = tid % kCB, row = tid / kCB;
+  constexpr int kRowsATask = kTileThreads / kCB;
   const uint8_t *w_at[S::kWTasks], *y_at[S::kYTasks];
 #pragma unroll
   for (int j = 0; j < S::kWTasks; ++j) {
-    const int t = j * S::kThreads + tid, r = min(t / kCB, S::kWRows - 1);
+    const int r = row + j * kRowsATask;
     const size_t f = min(m0 + (r >> 6) * 32 + (r & 31), a.nr - 1);
-    w_at[j] = (r & 32 ? a.up : a.gate) + f * a.bx + t % kCB * kQ4Bytes;
+    w_at[j] = (r & 32 ? a.up : a.gate) + f * a.bx;
   }
 #pragma unroll
-  for (int j = 0; j < S::kYTasks; ++j) {
-    const int t = j * S::kThreads + tid, r = min(t / kCB, S::kYRows - 1);
-    y_at[j] = a.vy + static_cast<size_t>(min(n0 + r, a.nc - 1)) * a.by + t % kCB * kQ8Bytes;
-  }
+  for (int j = 0; j < S::kYTasks; ++j)
+    y_at[j] = a.vy + static_cast<size_t>(min(n0 + row + j * kRowsATask, a.nc - 1)) * a.by;
   Q4Block w[S::kWTasks];
   Q8Block y[S::kYTasks];
-  const auto load = [&](int blocks) __attribute__((always_inline)) {
+  // past the last block that one again, which nothing folds
+  const auto load = [&](int c) __attribute__((always_inline)) {
+    const uint32_t b = min(static_cast<uint32_t>(c * kCB + block), a.nb - 1);
 #pragma unroll
-    for (int j = 0; j < S::kWTasks; ++j) {
-      if ((j * S::kThreads + tid) % kCB < blocks)
-        w[j] = load_q4(w_at[j]);
-      w_at[j] += kCB * kQ4Bytes;
-    }
+    for (int j = 0; j < S::kWTasks; ++j)
+      w[j] = load_q4(w_at[j] + b * kQ4Bytes);
 #pragma unroll
-    for (int j = 0; j < S::kYTasks; ++j) {
-      if ((j * S::kThreads + tid) % kCB < blocks)
-        y[j] = load_q8(y_at[j]);
-      y_at[j] += kCB * kQ8Bytes;
-    }
+    for (int j = 0; j < S::kYTasks; ++j)
+      y[j] = load_q8(y_at[j] + b * kQ8Bytes);
   };
-  const auto put = [&](uint8_t *stage, int blocks) __attribute__((always_inline)) {
-    float *const scales = reinterpret_cast<float *>(stage + S::kQuants);
+  const auto put = [&](uint8_t *stage) __attribute__((always_inline)) {
+    float *const scales = reinterpret_cast<float *>(stage + S::kQuants) + block * S::kRows;
 #pragma unroll
     for (int j = 0; j < S::kWTasks; ++j) {
-      const int t = j * S::kThreads + tid, r = t / kCB, b = t % kCB;
-      if (t >= S::kWRows * kCB || b >= blocks)
-        continue;
-      u32x4 *const to = reinterpret_cast<u32x4 *>(stage + r * S::kRow + b * kQK);
+      const int r = row + j * kRowsATask;
       u32x4 low, high;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        low[k] = nibbles_to_i8x4(w[j].q[k]);
-        high[k] = nibbles_to_i8x4(w[j].q[k] >> 4);
+        const uint32_t q = w[j].q[k] ^ 0x88888888u;
+        low[k] = q << 4 & 0xf0f0f0f0u;
+        high[k] = q & 0xf0f0f0f0u;
       }
+      u32x4 *const to = reinterpret_cast<u32x4 *>(stage + S::at(r, block));
       to[0] = low;
       to[1] = high;
-      scales[b * S::kRows + r] = fp16_bits_to_f32(w[j].d);
+      scales[r] = 0.0625f * fp16_bits_to_f32(w[j].d);
     }
 #pragma unroll
     for (int j = 0; j < S::kYTasks; ++j) {
-      const int t = j * S::kThreads + tid, r = S::kWRows + t / kCB, b = t % kCB;
-      if (t >= S::kYRows * kCB || b >= blocks)
-        continue;
-      u32x4 *const to = reinterpret_cast<u32x4 *>(stage + r * S::kRow + b * kQK);
+      const int r = S::kWRows + row + j * kRowsATask;
+      u32x4 *const to = reinterpret_cast<u32x4 *>(stage + S::at(r, block));
       to[0] = y[j].q[0];
       to[1] = y[j].q[1];
-      scales[b * S::kRows + r] = fp16_bits_to_f32(y[j].d);
+      scales[r] = fp16_bits_to_f32(y[j].d);
     }
   };
 
@@ -242,12 +306,11 @@ __global__ __launch_bounds__((Tiles<kFT, kNT, kKS, kCB>::kThreads)) void gated_t
   for (int e = 0; e < 16; ++e)
     seed[e] = kSeedBits;
   asm("" : "+v"(seed));  // kept in registers: as a constant it is made anew for every product
-  float acc[2][16] = {};
-  const int g_row = ft * 64 + li, y_row = S::kWRows + nt * 32;
+  float acc[2 * kFW][16] = {};
+  const int w_row = ft * 64 + li, y_row = S::kWRows + nt * 32;
   const auto fold = [&](const uint8_t *stage, int b) __attribute__((always_inline)) {
-    const uint8_t *const q = stage + b * kQK + 16 * h;
     const float *const d = reinterpret_cast<const float *>(stage + S::kQuants) + b * S::kRows;
-    const v4i tokens = *reinterpret_cast<const v4i *>(q + (y_row + li) * S::kRow);
+    const v4i tokens = *reinterpret_cast<const v4i *>(stage + S::at(y_row + li, b) + 16 * h);
     float dy[16];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -257,80 +320,60 @@ __global__ __launch_bounds__((Tiles<kFT, kNT, kKS, kCB>::kThreads)) void gated_t
       dy[4 * k + 2] = v.z;
       dy[4 * k + 3] = v.w;
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const v4i weights = *reinterpret_cast<const v4i *>(q + (g_row + 32 * i) * S::kRow);
-      const float dx = d[g_row + 32 * i], off = -kSeed * dx;
-      const v16f sums = __builtin_bit_cast(
+    const auto product = [&](int i) __attribute__((always_inline)) {
+      const v4i weights =
+          *reinterpret_cast<const v4i *>(stage + S::at(w_row + 32 * i, b) + 16 * h);
+      return __builtin_bit_cast(
           v16f, __builtin_amdgcn_mfma_i32_32x32x32_i8(tokens, weights, seed, 0, 0, 0));
+    };
+    v16f sums = product(0);
+#pragma unroll
+    for (int i = 0; i < 2 * kFW; ++i) {
+      v16f next;
+      if (i + 1 < 2 * kFW)
+        next = product(i + 1);  // on its way while this one is added
+      const float dx = d[w_row + 32 * i], off = -kSeed * dx;
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         acc[i][e] = fmaf(fmaf(sums[e], dx, off), dy[e], acc[i][e]);
+      if (i + 1 < 2 * kFW)
+        sums = next;
     }
   };
 
-  const int chunks = static_cast<int>((a.nb + kCB - 1) / kCB);
-  const auto blocks_of = [&](int c) { return min(static_cast<int>(a.nb) - c * kCB, kCB); };
-  if (chunks > 0) {
-    load(blocks_of(0));
-    put(lds, blocks_of(0));
-  }
-  __syncthreads();
-  for (int c = 0; c < chunks; ++c) {
-    const uint8_t *const stage = lds + (c & 1) * S::kStage;
-    const int blocks = blocks_of(c);
-    if (c + 1 < chunks)
-      load(blocks_of(c + 1));
-    if (blocks == kCB) {
+  if (a.nb > 0) {
+    const int whole = static_cast<int>(a.nb / kCB);
+    load(0);
+    put(lds);
+    load(1);
+    __syncthreads();
+    // chunk c is folded, c + 1 laid out, c + 2 set out for
+    for (int c = 0; c < whole; ++c) {
+      const uint8_t *const stage = lds + (c & 1) * S::kStage;
 #pragma unroll
-      for (int b = 0; b < kCB / kKS; ++b) {
-        fold(stage, b * kKS + ks);
+      for (int b = 0; b < kCB; ++b) {
+        fold(stage, b);
         __builtin_amdgcn_sched_barrier(0);
       }
-    } else {
-      for (int b = ks; b < blocks; b += kKS)
-        fold(stage, b);
+      put(lds + ((c + 1) & 1) * S::kStage);
+      load(c + 2);
+      __syncthreads();
     }
-    if (c + 1 < chunks)
-      put(lds + ((c + 1) & 1) * S::kStage, blocks_of(c + 1));
+    for (int b = whole * kCB; b < static_cast<int>(a.nb); ++b)
+      fold(lds + (whole & 1) * S::kStage, b - whole * kCB);
     __syncthreads();
   }
 
-  // the tile's outputs, 16 / kKS elements a wave
-  float *const out = reinterpret_cast<float *>(lds + S::kParts);
-  constexpr int kMine = 16 / kKS;
-  float sum[2][kMine];
+  // through LDS, so that a block's values are whole and rows are written by whole lines
+  float *const out = reinterpret_cast<float *>(lds);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if constexpr (kKS == 1) {
+  for (int f = 0; f < kFW; ++f)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        sum[i][e] = acc[i][e];
-    } else {
-      float *const parts = reinterpret_cast<float *>(lds) + (wave - ks) * 1024;
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        parts[ks * 1024 + e * 64 + lane] = acc[i][e];
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < kMine; ++e) {
-        sum[i][e] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kKS; ++k)
-          sum[i][e] += parts[k * 1024 + (ks * kMine + e) * 64 + lane];
-      }
-      __syncthreads();
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kMine; ++i) {
-    const int e = ks * kMine + i;
-    out[(nt * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) * S::kOutRow + ft * 32 + li] =
-        activation(sum[0][i], a.act) * sum[1][i];
-  }
+    for (int e = 0; e < 16; ++e)
+      out[(nt * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) * S::kOutRow + (ft + f) * 32 + li] =
+          activation(acc[2 * f][e], a.act) * acc[2 * f + 1][e];
   __syncthreads();
-  static_assert(S::kYRows * kFT * 8 % S::kThreads == 0 || S::kThreads > S::kYRows * kFT * 8, "");
-  for (int t = tid; t < S::kYRows * kFT * 8; t += S::kThreads) {
+  for (int t = tid; t < kTileTokens * kFT * 8; t += kTileThreads) {
     const int part = t & 7, block = (t >> 3) % kFT, row = t / (8 * kFT);
     const float4 x = *reinterpret_cast<const float4 *>(out + row * S::kOutRow + block * 32 + 4 * part);
     const float v[4] = {x.x, x.y, x.z, x.w};
@@ -339,47 +382,268 @@ __global__ __launch_bounds__((Tiles<kFT, kNT, kKS, kCB>::kThreads)) void gated_t
   }
 }
 
-template <typename T, int kCols> void launch_few(const GatedArgs &a, hipStream_t st) {
-  gated_few<T, kCols, 4><<<dim3((a.nr + kQK - 1) / kQK), dim3(512), 0, st>>>(a);
+// ---------------------------------------------------------------------------
+// Some tens of tokens: 32 features x 32 tokens a work-group.  Sixteen blocks of its rows at a time go to LDS as
+// they lie in memory, in pieces of 16 bytes, and each of the eight waves takes a pair of them through both
+// tiles; the waves' sums come together at the end.
+//
+// An operand of v_mfma_i32_32x32x32_i8 is 16 quants of a row a lane: lane group h (lanes 32 h ..) takes those
+// of a Q4_0 block's bytes 8 h .. 8 h + 7, 8 h .. and 16 + 8 h .., and the same of a token's.  Of a pair the even
+// block's quants lie 2 bytes off a dword, the odd one's on one; the dwords that hold them also hold the even
+// scale in group 0 and the odd one in group 1, the operands of the v_mfma_f32_32x32x8_f16 that gives the
+// products of the scales.  Quants stay in the upper half of their bytes, 16 (n - 8) with a flipped top bit.
+// ---------------------------------------------------------------------------
+constexpr int kSpanWaves = 8, kSpanThreads = kSpanWaves * 64, kSpanBlocks = 2 * kSpanWaves;
+
+struct Spans {
+  static constexpr int kWSpan = kSpanBlocks * kQ4Bytes, kYSpan = kSpanBlocks * kQ8Bytes;
+  // twice an odd number of dwords: a dword of 32 rows in banks of its own each
+  static constexpr int kWRow = kWSpan + 8, kYRow = kYSpan + 8;
+  static_assert(kWRow % 16 == 8 && kYRow % 16 == 8, "");
+  // pieces by 64, of one matrix each; a thread's
+  static constexpr int kWGroups = 32 * (kWSpan / 16) / 64, kYGroups = 32 * (kYSpan / 16) / 64;
+  static constexpr int kGroups = 2 * kWGroups + kYGroups;
+  static constexpr int kPieces = (kGroups + kSpanWaves - 1) / kSpanWaves;
+  static constexpr int kYAt = 64 * kWRow, kStage = kYAt + 32 * kYRow;
+  static constexpr int kMine = 16 / kSpanWaves;  // a lane's sums of a projection
+  static constexpr int kParts = kSpanWaves * 16 * 64 * 4, kOutRow = 36;
+  static constexpr int kLds = 2 * kStage;
+  static_assert(kLds >= kParts + 32 * kOutRow * 4, "");
+};
+
+template <typename T>
+__global__ __launch_bounds__(kSpanThreads, 4) void gated_spans(GatedArgs a) {
+  using S = Spans;
+  __shared__ __align__(16) uint8_t lds[S::kLds];
+  const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, h = lane >> 5;
+  const int ks = __builtin_amdgcn_readfirstlane(tid >> 6);
+  uint32_t tm, tn;
+  tile_of(blockIdx.x, (a.nr + kQK - 1) / kQK, (a.nc + 31) / 32, tm, tn);
+  const uint32_t m0 = tm * kQK, n0 = tn * 32;
+  // The thread's pieces, by 64 of one matrix: its address stays in scalar registers.  Waves that have one
+  // less take the last group's again.
+  struct Piece {
+    const uint8_t *base;   // of the matrix's rows in this work-group, and of the chunk
+    uint32_t row, at, to;  // the row's offset, the place in it, the place in LDS
+    bool tokens;
+  };
+  const auto piece_of = [&](int j) __attribute__((always_inline)) {
+    const int g = min(j * kSpanWaves + ks, S::kGroups - 1), matrix = min(g / S::kWGroups, 2);
+    const int q = (g - matrix * S::kWGroups) * 64 + lane;
+    Piece p;
+    p.tokens = matrix == 2;
+    const int r = p.tokens ? q / (S::kYSpan / 16) : q / (S::kWSpan / 16);
+    p.at = 16 * (p.tokens ? q % (S::kYSpan / 16) : q % (S::kWSpan / 16));
+    p.to = (p.tokens ? S::kYAt + r * S::kYRow : (32 * matrix + r) * S::kWRow) + p.at;
+    p.base = p.tokens ? a.vy + static_cast<size_t>(n0) * a.by
+                      : (matrix ? a.up : a.gate) + static_cast<size_t>(m0) * a.bx;
+    p.row = p.tokens ? min(static_cast<uint32_t>(r), a.nc - 1 - n0) * static_cast<uint32_t>(a.by)
+                     : min(static_cast<uint32_t>(r), a.nr - 1 - m0) * static_cast<uint32_t>(a.bx);
+    return p;
+  };
+  const uint8_t *base[S::kPieces];
+  uint32_t from[S::kPieces], to[S::kPieces], step[S::kPieces];
+#pragma unroll
+  for (int j = 0; j < S::kPieces; ++j) {
+    const Piece p = piece_of(j);
+    base[j] = p.base;
+    from[j] = p.row + p.at;
+    to[j] = p.to;
+    step[j] = p.tokens ? S::kYSpan : S::kWSpan;
+  }
+  u32x4a2 held[S::kPieces];
+  const auto load = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < S::kPieces; ++j) {
+      held[j] = *reinterpret_cast<const u32x4a2 *>(base[j] + from[j]);
+      base[j] += step[j];
+    }
+  };
+  const auto put = [&](uint8_t *stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < S::kPieces; ++j) {
+      u32x2 *const p = reinterpret_cast<u32x2 *>(stage + to[j]);
+      p[0] = u32x2{held[j].x, held[j].y};
+      p[1] = u32x2{held[j].z, held[j].w};
+    }
+  };
+  // a part of a chunk: a row's last piece begins 16 bytes before its end, and goes as much before its
+  // place; so do those that lie past it
+  const auto lay_part = [&](uint8_t *stage, int blocks) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < S::kPieces; ++j) {
+      const Piece p = piece_of(j);
+      const uint32_t end = blocks * (p.tokens ? kQ8Bytes : kQ4Bytes) - 16, at = min(p.at, end);
+      *reinterpret_cast<u32x4a2 *>(stage + p.to - (p.at - at)) =
+          *reinterpret_cast<const u32x4a2 *>(base[j] + (p.row + at));
+    }
+  };
+
+  const uint32_t m_even = h ? 0u : 0xffffu, m_odd = h ? 0xffff0000u : 0u;
+  const int w_at = li * S::kWRow + ks * (2 * kQ4Bytes) + 8 * h;
+  const int y_at = S::kYAt + li * S::kYRow + ks * (2 * kQ8Bytes) + 8 * h;
+  float acc[2][16] = {};
+  const auto weights = [&](uint32_t q0, uint32_t q1) __attribute__((always_inline)) {
+    q0 ^= 0x88888888u;
+    q1 ^= 0x88888888u;
+    const u32x4 v = {q0 << 4 & 0xf0f0f0f0u, q1 << 4 & 0xf0f0f0f0u, q0 & 0xf0f0f0f0u, q1 & 0xf0f0f0f0u};
+    return __builtin_bit_cast(v4i, v);
+  };
+  const auto fold = [&](float (&to)[16], const u32x4 &y, const v4i &w, uint32_t dy,
+                        uint32_t dw) __attribute__((always_inline)) {
+    const v16i sums = q8_sumi(__builtin_bit_cast(v4i, y), w);
+    const v16f scales = q8_dxy(dy, dw);
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      to[e] = fmaf(static_cast<float>(sums[e]), scales[e], to[e]);
+    // one product at a time, folded here and nothing moved across: 128 registers hold no two
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      asm volatile("" : "+v"(to[e]));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // the wave's pair of a chunk, or its even block alone
+  const auto pair = [&](const uint8_t *stage, bool odd) __attribute__((always_inline)) {
+    const uint32_t *const x[2] = {reinterpret_cast<const uint32_t *>(stage + w_at),
+                                  reinterpret_cast<const uint32_t *>(stage + w_at + 32 * S::kWRow)};
+    const uint32_t *const y = reinterpret_cast<const uint32_t *>(stage + y_at);
+    v4i w[2];
+    uint32_t dw[2], odd_dw[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[i] = weights(funnel16(x[i][0], x[i][1]), funnel16(x[i][1], x[i][2]));
+      dw[i] = x[i][0] & m_even;
+      odd_dw[i] = x[i][2] & m_odd;
+    }
+    const u32x4 even = {funnel16(y[0], y[1]), funnel16(y[1], y[2]), funnel16(y[4], y[5]),
+                        funnel16(y[5], y[6])};
+    const uint32_t odd_dy = y[6] & m_odd;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      fold(acc[i], even, w[i], y[0] & m_even, dw[i]);
+    if (!odd)
+      return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      w[i] = weights(x[i][5], x[i][6]);
+    const u32x4 last = {y[9], y[10], y[13], y[14]};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      fold(acc[i], last, w[i], odd_dy, odd_dw[i]);
+  };
+  const int whole = static_cast<int>(a.nb / kSpanBlocks);
+  const int rest = static_cast<int>(a.nb) - whole * kSpanBlocks;
+  if (whole > 0) {
+    load();
+    put(lds);
+    if (whole > 1)
+      load();
+    __syncthreads();
+    for (int c = 0; c < whole; ++c) {
+      pair(lds + (c & 1) * S::kStage, true);
+      if (c + 1 < whole) {
+        put(lds + ((c + 1) & 1) * S::kStage);
+        if (c + 2 < whole)
+          load();
+      }
+      __syncthreads();
+    }
+  }
+  if (rest > 0) {
+    lay_part(lds, rest);
+    __syncthreads();
+    if (2 * ks < rest)
+      pair(lds, 2 * ks + 1 < rest);
+    __syncthreads();
+  }
+
+  // the waves' sums together, kMine of a lane's each
+  float *const parts = reinterpret_cast<float *>(lds);
+  float *const out = reinterpret_cast<float *>(lds + S::kParts);
+  float sum[2][S::kMine];
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      parts[(ks * 16 + e) * 64 + lane] = acc[p][e];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < S::kMine; ++q) {
+      sum[p][q] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kSpanWaves; ++k)
+        sum[p][q] += parts[(k * 16 + ks * S::kMine + q) * 64 + lane];
+      sum[p][q] *= 0.0625f;  // of the quants
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int q = 0; q < S::kMine; ++q) {
+    const int e = ks * S::kMine + q;
+    out[(8 * (e >> 2) + 4 * h + (e & 3)) * S::kOutRow + li] = activation(sum[0][q], a.act) * sum[1][q];
+  }
+  __syncthreads();
+  if (tid < 32 * 8) {
+    const int part = tid & 7, row = tid >> 3;
+    const float4 x = *reinterpret_cast<const float4 *>(out + row * S::kOutRow + 4 * part);
+    const float v[4] = {x.x, x.y, x.z, x.w};
+    if (n0 + row < a.nc)
+      emit<T>(a, n0 + row, m0, part, v);
+  }
 }
 
-template <typename T, int kFT, int kNT, int kKS, int kCB>
-int launch_tiles(const GatedArgs &a, hipStream_t st) {
-  const uint64_t tiles = static_cast<uint64_t>((a.nr + 32 * kFT - 1) / (32 * kFT)) *
-                         ((a.nc + 32 * kNT - 1) / (32 * kNT));
-  using S = Tiles<kFT, kNT, kKS, kCB>;
-  if (tiles > 0xffffffffu / S::kThreads)
+size_t up_by(size_t n, size_t by) { return (n + by - 1) / by; }
+
+template <typename T> int launch_spans(const GatedArgs &a, hipStream_t st) {
+  const size_t tiles = up_by(a.nr, kQK) * up_by(a.nc, 32);
+  if (tiles > 0xffffffffu / kSpanThreads)
     return TCRV_HIP_ERR_TOO_LARGE;
-  gated_tiles<T, kFT, kNT, kKS, kCB>
-      <<<dim3(static_cast<unsigned>(tiles)), dim3(S::kThreads), 0, st>>>(a);
+  gated_spans<T><<<dim3(static_cast<unsigned>(tiles)), dim3(kSpanThreads), 0, st>>>(a);
+  return tcrv_host::launch_status();
+}
+
+template <typename T, int kFT> int launch_tiles(const GatedArgs &a, hipStream_t st) {
+  const size_t tiles = up_by(a.nr, 32 * kFT) * up_by(a.nc, kTileTokens);
+  if (tiles > 0xffffffffu / kTileThreads)
+    return TCRV_HIP_ERR_TOO_LARGE;
+  gated_tiles<T, kFT>
+      <<<dim3(static_cast<unsigned>(tiles)), dim3(kTileThreads), 0, st>>>(a);
   return tcrv_host::launch_status();
 }
 
 template <typename T> int launch_elem(const GatedArgs &a, hipStream_t st) {
-  switch (a.nc) {
-  case 1:
-    launch_few<T, 1>(a, st);
-    break;
-  case 2:
-    launch_few<T, 2>(a, st);
-    break;
-  case 3:
-    launch_few<T, 3>(a, st);
-    break;
-  case 4:
-    launch_few<T, 4>(a, st);
-    break;
-  default:
-    return a.nc <= 128 ? launch_tiles<T, 1, 1, 8, 8>(a, st) : launch_tiles<T, 4, 4, 1, 4>(a, st);
+  if (a.nc == 1) {
+    const bool pairs = a.nb > 1;
+    const dim3 grid(static_cast<unsigned>(up_by(a.nr, a.q8 ? kQK : one_waves(false))));
+    const dim3 block(one_waves(a.q8 != nullptr) * 64);
+    if (a.q8)
+      pairs ? gated_one<T, true, true><<<grid, block, 0, st>>>(a)
+            : gated_one<T, false, true><<<grid, block, 0, st>>>(a);
+    else
+      pairs ? gated_one<T, true, false><<<grid, block, 0, st>>>(a)
+            : gated_one<T, false, false><<<grid, block, 0, st>>>(a);
+    return tcrv_host::launch_status();
   }
-  return tcrv_host::launch_status();
+  // By what the kernels take for a block of K, in ns: rounds of 256 work-groups, one a CU, of the tiles; the
+  // spans', two a CU, go on as CUs are free.  Measured at K 4096, us, spans / 64 features x 128 tokens / 128 x
+  // 128: 11008 features x 33 tokens 33 / 58 / 92, 14336 x 128 69 / 62 / 95, 11008 x 200 91 / 118 / 96, 4096 x
+  // 512 72 / 61 / 93, 14336 x 512 265 / 229 / 187, 2048 960 / 780 / 640.
+  const size_t groups = up_by(a.nr, kQK) * up_by(a.nc, 32);
+  const size_t spans = groups <= 256 ? 100 : groups * 3 / 10;
+  const size_t mid = 460 * up_by(up_by(a.nr, 64) * up_by(a.nc, kTileTokens), 256);
+  const size_t wide = 720 * up_by(up_by(a.nr, 128) * up_by(a.nc, kTileTokens), 256);
+  if (spans <= wide && spans <= mid)
+    return launch_spans<T>(a, st);
+  return mid <= wide ? launch_tiles<T, 2>(a, st) : launch_tiles<T, 4>(a, st);
 }
 
 }  // namespace
 }  // namespace tcrv
 
-// A launch holds less than 2^32 threads along an axis: work-groups of 512, one 32 features.
-constexpr size_t kMostFeatures = ((size_t{1} << 23) - 1) * tcrv::kQK;
+// A launch holds less than 2^32 threads along an axis: work-groups of 256, one four features.
+constexpr size_t kMostFeatures = ((size_t{1} << 24) - 1) * 4;
+// 32 rows' offsets are 32-bit.
+constexpr size_t kMostStride = size_t{1} << 26;
 
 extern "C" int tcrv_hip_gated_q4_0_q8_0(int elem, int act, size_t n, void *out, size_t out_token,
                                         uint8_t *q8, size_t q8_token, const uint8_t *gate,
@@ -391,7 +655,8 @@ extern "C" int tcrv_hip_gated_q4_0_q8_0(int elem, int act, size_t n, void *out, 
     return TCRV_HIP_ERR_UNSUPPORTED;
   if (nr == 0 || nc == 0)
     return TCRV_HIP_OK;
-  if (nr > kMostFeatures || nc > kMostTokens || nb > 0x7fffffffu / tcrv::kQ8Bytes)
+  if (nr > kMostFeatures || nc > kMostTokens || nb > kMostStride / tcrv::kQ8Bytes ||
+      (nr > 1 && bx > kMostStride) || (nc > 1 && by > kMostStride))
     return TCRV_HIP_ERR_TOO_LARGE;
   if ((!out && !q8) || (nb && (!gate || !up || !vy)))
     return TCRV_HIP_ERR_NULL_POINTER;
