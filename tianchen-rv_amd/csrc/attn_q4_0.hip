@@ -602,8 +602,18 @@ struct Branch {
     // the others are cached tokens; a row without bits takes its own as one
     lo = max(tree - static_cast<int>(min(left, a.window - 1)), 0);
   }
-  __device__ bool sees(int t) const {
-    return t < tree || (bits[(t - tree) >> 6] >> ((t - tree) & 63) & 1u);
+  // which of tokens t .. t + 31 are cached ones or have their bits set
+  __device__ uint32_t sees32(const AttnArgs &a, int t) const {
+    const int before = tree - t;
+    if (before >= 32)
+      return ~0u;
+    const uint32_t from = max(-before, 0), shift = from & 63;
+    const size_t w = from >> 6;
+    uint64_t x = w < a.words ? bits[w] >> shift : 0;
+    if (shift > 32 && w + 1 < a.words)
+      x |= bits[w + 1] << (64 - shift);
+    const uint32_t some = static_cast<uint32_t>(x);
+    return before > 0 ? some << before | ((1u << before) - 1) : some;
   }
 };
 
@@ -824,13 +834,12 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 4 ? 2 : 1) void attn_q4_0_rows16
       const bool edge = t0 < all_lo || t0 + kStep > all_hi || both != 3u;
       uint32_t seen = 0;
       if (edge) {
+        const uint32_t bits = kTree ? branch.sees32(a, t0) : ~0u;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int at = t0 + 16 * (i >> 2) + 4 * g + (i & 3);
-          bool sees = at >= my_lo && at < my_hi && (both >> (i >> 2) & 1u);
-          if constexpr (kTree)
-            sees = sees && branch.sees(at);
-          seen |= sees ? 1u << i : 0u;
+          const int in_step = 16 * (i >> 2) + 4 * g + (i & 3), at = t0 + in_step;
+          seen |= at >= my_lo && at < my_hi && (both >> (i >> 2) & 1u) && (bits >> in_step & 1u)
+                      ? 1u << i : 0u;
         }
       }
       attend<NB, NP>(row, t, edge, seen);
@@ -1092,7 +1101,7 @@ __device__ __forceinline__ bool find_piece(const AttnArgs &a, uint32_t w, int la
   }
 }
 
-template <int NB, int NP, typename T>
+template <int NB, int NP, typename T, bool kTree = false>
 __global__ __launch_bounds__((TileStep<NB, NP>::kThreads), (TileStep<NB, NP>::kWaves / 4)) void
 attn_q4_0_tiles(AttnArgs a) {
   using S = TileStep<NB, NP>;
@@ -1111,7 +1120,7 @@ attn_q4_0_tiles(AttnArgs a) {
   const uint32_t last = span.rows - 1;
   const uint32_t i0 = tile * S::kRows / a.share;
   const uint32_t i1 = min(tile * S::kRows + S::kRows - 1, last) / a.share;
-  int begin = span.lo(a, i0) & -kStep, end = span.hi(a, i1);
+  int begin = span.lo(a, kTree ? 0 : i0) & -kStep, end = span.hi(a, i1);
   bool cut = false;
   if (mine.part_tokens) {
     const int part = mine.part_tokens;
@@ -1128,11 +1137,19 @@ attn_q4_0_tiles(AttnArgs a) {
   // the wave's rows, and what they see
   const uint32_t row0 = tile * S::kRows + wave * 32;
   const uint32_t w0 = min(row0, last) / a.share, w1 = min(row0 + 31, last) / a.share;
-  const int wave_lo = span.lo(a, w0), wave_hi = row0 <= last ? min(span.hi(a, w1), end) : 0;
-  const int all_lo = span.lo(a, w1), all_hi = min(span.hi(a, w0), end);
+  const int wave_lo = span.lo(a, kTree ? 0 : w0);
+  const int wave_hi = row0 <= last ? min(span.hi(a, w1), end) : 0;
+  const int all_lo = span.lo(a, w1);
+  const int all_hi = min(kTree ? span.position0 : span.hi(a, w0), end);
   const uint32_t r = min(row0 + col, last);
   const bool valid = row0 + col <= last;
-  const int lo = span.lo(a, r / a.share), hi = min(span.hi(a, r / a.share), end);
+  Branch branch;
+  int lo = span.lo(a, r / a.share);
+  if constexpr (kTree) {
+    branch = Branch(a, span, r / a.share);
+    lo = branch.lo;
+  }
+  const int hi = min(span.hi(a, r / a.share), end);
   const uint32_t token = span.first + r / a.share, head = kv_head * a.share + r % a.share;
 
   // the thread's piece of a step
@@ -1423,10 +1440,11 @@ attn_q4_0_tiles(AttnArgs a) {
 #pragma unroll
           for (int i = 0; i < 2; ++i)
             hi_at[i] = mine >> (kAbsentAt + 2 * sub + i) & 1u ? 0 : hi - t0 - 32 * sub - 4 * hh;
+          const uint32_t bits = kTree ? branch.sees32(a, t0 + 32 * sub) >> 4 * hh : ~0u;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int at = 8 * (i >> 2) + (i & 3);
-            z[i] = at >= lo_at && at < hi_at[i >> 3] ? z[i] : kNone;
+            z[i] = at >= lo_at && at < hi_at[i >> 3] && (!kTree || (bits >> at & 1u)) ? z[i] : kNone;
           }
         }
         float high = z[0];
@@ -1526,7 +1544,9 @@ attn_q4_0_tiles(AttnArgs a) {
         for (int sub = 0; sub < kTokens / 32; ++sub) {
           const int first = min(max(lo - t0 - 32 * sub, 0), 32);
           const int stop = min(max(hi - t0 - 32 * sub, 0), 32);
-          const uint32_t sees = static_cast<uint32_t>((1ull << stop) - (1ull << min(first, stop)));
+          uint32_t sees = static_cast<uint32_t>((1ull << stop) - (1ull << min(first, stop)));
+          if constexpr (kTree)
+            sees &= branch.sees32(a, t0 + 32 * sub);
 #pragma unroll
           for (int b = 0; b < NB; ++b)
             o[b] += s_bad[n & 1][b][sub] & sees ? __builtin_nanf("") : 0.0f;
@@ -1697,7 +1717,7 @@ __global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join(AttnArgs a, uint3
   const uint32_t i = token - span.first;
   const uint32_t row0 = (i * a.share + head % a.share) / tile_rows * tile_rows;
   const uint32_t i0 = row0 / a.share, i1 = min(row0 + tile_rows - 1, span.rows - 1) / a.share;
-  const int tokens = max(span.hi(a, i1) - (span.lo(a, i0) & -kStep), 1);
+  const int tokens = max(span.hi(a, i1) - (span.lo(a, a.ancestors ? 0 : i0) & -kStep), 1);
   const uint32_t part_tokens = a.plan[0].x;
   const uint32_t splits = min((tokens + part_tokens - 1) / part_tokens, a.splits);
   if (splits == 1)
@@ -1803,10 +1823,10 @@ size_t parts_bytes(size_t parts, size_t head_dim) {
 // The shares of the kernel of few rows, for lengths up to max_length; none where no tile has enough
 // tokens to be cut.
 Plan few_plan(size_t requests, size_t max_added, size_t max_length, size_t window, size_t heads,
-              size_t kv_heads, size_t head_dim, size_t most_rows) {
+              size_t kv_heads, size_t head_dim) {
   Plan p{};
   const size_t share = heads / kv_heads;
-  const size_t rows = std::min(max_added * share, most_rows);
+  const size_t rows = std::min(max_added * share, few_rows_of(requests, max_added * share, kv_heads));
   p.tile_rows = tcrv::kRows;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const size_t items = requests * p.tiles * kv_heads;
@@ -1857,17 +1877,13 @@ Plan many_plan(int elem, size_t requests, size_t tokens, size_t max_added, size_
   return p;
 }
 
-// Which of the two kernels a call launches, and the rows up to which the first serves: all of them of trees.
+// Which of the two kernels a call launches, and the rows up to which the first serves.
 struct Kernels {
   bool few, many;
   size_t few_rows;
 };
-Kernels kernels_of(bool tree, size_t requests, size_t tokens, size_t max_added, size_t heads,
-                   size_t kv_heads) {
-  const size_t rows = max_added * (heads / kv_heads);
-  if (tree)
-    return {true, false, rows};
-  const size_t few = few_rows_of(requests, rows, kv_heads);
+Kernels kernels_of(size_t requests, size_t tokens, size_t max_added, size_t heads, size_t kv_heads) {
+  const size_t rows = max_added * (heads / kv_heads), few = few_rows_of(requests, rows, kv_heads);
   if (rows <= few)
     return {true, false, few};
   // one request, or all as long as the longest: none is short
@@ -1893,25 +1909,25 @@ void launch_rows16(const AttnArgs &a, size_t head_dim, unsigned groups, hipStrea
   }
 }
 
-template <int NB, int NP, typename T>
+template <int NB, int NP, typename T, bool kTree>
 void launch_tiles(const AttnArgs &a, dim3 grid, hipStream_t st) {
-  tcrv::attn_q4_0_tiles<NB, NP, T><<<grid, dim3(tcrv::TileStep<NB, NP>::kThreads), 0, st>>>(a);
+  tcrv::attn_q4_0_tiles<NB, NP, T, kTree><<<grid, dim3(tcrv::TileStep<NB, NP>::kThreads), 0, st>>>(a);
 }
 
-template <int NP, typename T>
+template <int NP, typename T, bool kTree>
 void launch_tiles(const AttnArgs &a, size_t head_dim, dim3 grid, hipStream_t st) {
   switch (head_dim) {
   case 64:
-    launch_tiles<2, NP, T>(a, grid, st);
+    launch_tiles<2, NP, T, kTree>(a, grid, st);
     break;
   case 128:
-    launch_tiles<4, NP, T>(a, grid, st);
+    launch_tiles<4, NP, T, kTree>(a, grid, st);
     break;
   case 192:
-    launch_tiles<6, NP, T>(a, grid, st);
+    launch_tiles<6, NP, T, kTree>(a, grid, st);
     break;
   default:
-    launch_tiles<8, NP, T>(a, grid, st);
+    launch_tiles<8, NP, T, kTree>(a, grid, st);
     break;
   }
 }
@@ -1940,14 +1956,14 @@ void launch_all(AttnArgs a, Kernels k, const Plan &few, const Plan &many, size_t
           <<<dim3(a.groups, static_cast<unsigned>(rows)), join_block, 0, st>>>(a, dim);
     }
   }
-  if (!kTree && k.many) {
+  if (k.many) {
     a.plan = reinterpret_cast<uint4 *>(workspace + (k.few ? few.workspace / sizeof(float) : 0));
     a.parts = reinterpret_cast<float *>(a.plan + 1);
     a.tiles = static_cast<uint32_t>(many.tiles);
     a.splits = static_cast<uint32_t>(many.splits);
     a.few_least = few_most ? few_most + 1 : 0;
     a.few_most = 0xffffffffu;
-    launch_tiles<NP, T>(a, head_dim, dim3(static_cast<unsigned>(many.launch)), st);
+    launch_tiles<NP, T, kTree>(a, head_dim, dim3(static_cast<unsigned>(many.launch)), st);
     if (many.splits > 1) {
       const uint32_t tile_rows = static_cast<uint32_t>(many.tile_rows);
       const uint32_t groups = tcrv::kJoinThreads / (dim / 4);
@@ -1977,17 +1993,17 @@ bool attn_too_large(size_t requests, size_t tokens, size_t max_added, size_t max
          requests * max_added * heads > (size_t{1} << 40);
 }
 
-size_t workspace_bytes_of(bool tree, int elem, size_t requests, size_t tokens, size_t max_added,
+size_t workspace_bytes_of(int elem, size_t requests, size_t tokens, size_t max_added,
                           size_t max_length, size_t heads, size_t kv_heads, size_t head_dim) {
   if (!tcrv_host::float_elem_bytes(elem) || !attn_sizes_ok(heads, kv_heads, head_dim) ||
       attn_too_large(requests, tokens, max_added, max_length, heads) || !requests || !tokens ||
       !max_added)
     return 0;
-  const Kernels k = kernels_of(tree, requests, tokens, max_added, heads, kv_heads);
+  const Kernels k = kernels_of(requests, tokens, max_added, heads, kv_heads);
   size_t need = 0;
   for (const bool few : {true, false})
     if (few ? k.few : k.many)
-      need += (few ? few_plan(requests, max_added, max_length, 0, heads, kv_heads, head_dim, k.few_rows)
+      need += (few ? few_plan(requests, max_added, max_length, 0, heads, kv_heads, head_dim)
                    : many_plan(elem, requests, tokens, max_added, max_length, 0, heads, kv_heads, head_dim))
                   .workspace;
   return need;
@@ -2026,10 +2042,10 @@ int attend(int elem, const void *q, size_t q_token, size_t q_head, const uint8_t
     return TCRV_HIP_ERR_BAD_SIZE;
   if (pages == 0)
     max_length = 0;  // nothing to read
-  const Kernels k = kernels_of(tree, requests, tokens, max_added, heads, kv_heads);
+  const Kernels k = kernels_of(requests, tokens, max_added, heads, kv_heads);
   const size_t bound = causal ? window : 0;
   const Plan few =
-      few_plan(requests, max_added, max_length, bound, heads, kv_heads, head_dim, k.few_rows);
+      few_plan(requests, max_added, max_length, bound, heads, kv_heads, head_dim);
   const Plan many =
       many_plan(elem, requests, tokens, max_added, max_length, bound, heads, kv_heads, head_dim);
   // rows16 numbers its tiles in 32 bits; a work-group of the other kernel has two threads a row
@@ -2103,14 +2119,14 @@ extern "C" {
 size_t tcrv_hip_attn_q4_0_workspace_bytes(int elem, size_t requests, size_t tokens,
                                           size_t max_added, size_t max_length, size_t heads,
                                           size_t kv_heads, size_t head_dim) {
-  return workspace_bytes_of(false, elem, requests, tokens, max_added, max_length, heads, kv_heads,
+  return workspace_bytes_of(elem, requests, tokens, max_added, max_length, heads, kv_heads,
                             head_dim);
 }
 
 size_t tcrv_hip_attn_tree_q4_0_workspace_bytes(int elem, size_t requests, size_t tokens,
                                                size_t max_added, size_t max_length, size_t heads,
                                                size_t kv_heads, size_t head_dim) {
-  return workspace_bytes_of(true, elem, requests, tokens, max_added, max_length, heads, kv_heads,
+  return workspace_bytes_of(elem, requests, tokens, max_added, max_length, heads, kv_heads,
                             head_dim);
 }
 
