@@ -1785,8 +1785,11 @@ using tcrv::AttnArgs;
 // / tiles: 64 requests of 4096 tokens and 8 new ones, 32 rows, 100 / 205, 32 of 2048 42 / 75, 8 of 4096
 // and 16 new 42 / 56; one request of 4096 and 16 new 32 / 24; 8 of 4096 and 64 new, up to 256 rows, with
 // the limit at 64 rows 77, at 16 63).
-size_t few_rows_of(size_t requests, size_t max_rows, size_t kv_heads) {
-  return max_rows <= 64 && requests * kv_heads >= 64 ? 64 : 16;
+// Of trees up to four tiles, whatever else there is (us, f16, 8 kv heads of 128, rows16 / tiles: one request of
+// 531 and 7 nodes, 28 rows, 12 / 19, of 4096 and 16 22 / 24, 8 of up to 4096 and 16 41 / 52, 64 of up to 4096
+// and 8 98 / 295; f32, 8 of 4096 and 32, 128 rows, 77 / 63, bf16, 6 of 8192 and 64 126 / 87).
+size_t few_rows_of(bool tree, size_t requests, size_t max_rows, size_t kv_heads) {
+  return max_rows <= 64 && (tree || requests * kv_heads >= 64) ? 64 : 16;
 }
 
 // Rows of a tile of attn_q4_0_tiles.
@@ -1822,11 +1825,12 @@ size_t parts_bytes(size_t parts, size_t head_dim) {
 
 // The shares of the kernel of few rows, for lengths up to max_length; none where no tile has enough
 // tokens to be cut.
-Plan few_plan(size_t requests, size_t max_added, size_t max_length, size_t window, size_t heads,
-              size_t kv_heads, size_t head_dim) {
+Plan few_plan(bool tree, size_t requests, size_t max_added, size_t max_length, size_t window,
+              size_t heads, size_t kv_heads, size_t head_dim) {
   Plan p{};
   const size_t share = heads / kv_heads;
-  const size_t rows = std::min(max_added * share, few_rows_of(requests, max_added * share, kv_heads));
+  const size_t rows =
+      std::min(max_added * share, few_rows_of(tree, requests, max_added * share, kv_heads));
   p.tile_rows = tcrv::kRows;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   const size_t items = requests * p.tiles * kv_heads;
@@ -1882,8 +1886,10 @@ struct Kernels {
   bool few, many;
   size_t few_rows;
 };
-Kernels kernels_of(size_t requests, size_t tokens, size_t max_added, size_t heads, size_t kv_heads) {
-  const size_t rows = max_added * (heads / kv_heads), few = few_rows_of(requests, rows, kv_heads);
+Kernels kernels_of(bool tree, size_t requests, size_t tokens, size_t max_added, size_t heads,
+                   size_t kv_heads) {
+  const size_t rows = max_added * (heads / kv_heads);
+  const size_t few = few_rows_of(tree, requests, rows, kv_heads);
   if (rows <= few)
     return {true, false, few};
   // one request, or all as long as the longest: none is short
@@ -1993,17 +1999,17 @@ bool attn_too_large(size_t requests, size_t tokens, size_t max_added, size_t max
          requests * max_added * heads > (size_t{1} << 40);
 }
 
-size_t workspace_bytes_of(int elem, size_t requests, size_t tokens, size_t max_added,
+size_t workspace_bytes_of(bool tree, int elem, size_t requests, size_t tokens, size_t max_added,
                           size_t max_length, size_t heads, size_t kv_heads, size_t head_dim) {
   if (!tcrv_host::float_elem_bytes(elem) || !attn_sizes_ok(heads, kv_heads, head_dim) ||
       attn_too_large(requests, tokens, max_added, max_length, heads) || !requests || !tokens ||
       !max_added)
     return 0;
-  const Kernels k = kernels_of(requests, tokens, max_added, heads, kv_heads);
+  const Kernels k = kernels_of(tree, requests, tokens, max_added, heads, kv_heads);
   size_t need = 0;
   for (const bool few : {true, false})
     if (few ? k.few : k.many)
-      need += (few ? few_plan(requests, max_added, max_length, 0, heads, kv_heads, head_dim)
+      need += (few ? few_plan(tree, requests, max_added, max_length, 0, heads, kv_heads, head_dim)
                    : many_plan(elem, requests, tokens, max_added, max_length, 0, heads, kv_heads, head_dim))
                   .workspace;
   return need;
@@ -2042,10 +2048,10 @@ int attend(int elem, const void *q, size_t q_token, size_t q_head, const uint8_t
     return TCRV_HIP_ERR_BAD_SIZE;
   if (pages == 0)
     max_length = 0;  // nothing to read
-  const Kernels k = kernels_of(requests, tokens, max_added, heads, kv_heads);
+  const Kernels k = kernels_of(tree, requests, tokens, max_added, heads, kv_heads);
   const size_t bound = causal ? window : 0;
   const Plan few =
-      few_plan(requests, max_added, max_length, bound, heads, kv_heads, head_dim);
+      few_plan(tree, requests, max_added, max_length, bound, heads, kv_heads, head_dim);
   const Plan many =
       many_plan(elem, requests, tokens, max_added, max_length, bound, heads, kv_heads, head_dim);
   // rows16 numbers its tiles in 32 bits; a work-group of the other kernel has two threads a row
@@ -2119,14 +2125,14 @@ extern "C" {
 size_t tcrv_hip_attn_q4_0_workspace_bytes(int elem, size_t requests, size_t tokens,
                                           size_t max_added, size_t max_length, size_t heads,
                                           size_t kv_heads, size_t head_dim) {
-  return workspace_bytes_of(elem, requests, tokens, max_added, max_length, heads, kv_heads,
+  return workspace_bytes_of(false, elem, requests, tokens, max_added, max_length, heads, kv_heads,
                             head_dim);
 }
 
 size_t tcrv_hip_attn_tree_q4_0_workspace_bytes(int elem, size_t requests, size_t tokens,
                                                size_t max_added, size_t max_length, size_t heads,
                                                size_t kv_heads, size_t head_dim) {
-  return workspace_bytes_of(elem, requests, tokens, max_added, max_length, heads, kv_heads,
+  return workspace_bytes_of(true, elem, requests, tokens, max_added, max_length, heads, kv_heads,
                             head_dim);
 }
 
