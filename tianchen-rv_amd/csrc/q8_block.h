@@ -31,6 +31,14 @@ __device__ __forceinline__ float max8(float v) {
   return v;
 }
 
+// The same over the 4 lanes of a quad.
+__device__ __forceinline__ float max4(float v) {
+  v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v),
+                                                                  0xB1, 0xf, 0xf, false)));
+  return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v),
+                                                                     0x4E, 0xf, 0xf, false)));
+}
+
 // Four of a block's values as this lane's part of it; every lane of the group takes part.
 __device__ __forceinline__ void store_q8_part(uint8_t *block, int part, const float (&v)[4]) {
   using u32a2 = uint32_t __attribute__((aligned(2)));
