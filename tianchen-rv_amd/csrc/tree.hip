@@ -90,7 +90,7 @@ struct RowUnits {
       return lay.key_scale(nb, token, unit);
     unit -= nb;
     if (unit < keys)
-      return lay.value(nb, token, unit / (nb / 2), unit % (nb / 2));
+      return lay.value(nb, token, 0, 0) + 8 * unit;
     return lay.value_scale(nb, token, unit - keys);
   }
 };
@@ -102,19 +102,29 @@ struct KeepArgs {
   uint32_t pages, page_size, max_added, kv_heads, head_dim;
 };
 
-constexpr int kKeepThreads = 256, kKeepTokens = 16;
+constexpr int kKeepWaves = 4, kKeepTokens = 16;
+constexpr int kKeepUnits = 2 * (256 / 4 + 256 / kQK);  // at most, of a row
 
-// A work-group a request and head takes kKeepTokens nodes of the path at a time: their rows into LDS, then
-// from there to their places.  Nodes ascend and lie at or past their new places, so that what is still
-// to be read lies past what has been written.
-__global__ __launch_bounds__(kKeepThreads) void kv_keep_q4_0(KeepArgs a) {
-  __shared__ uint16_t s_row[kKeepTokens * (2 * (256 / 4 + 256 / kQK))];
+// A work-group a request and head takes kKeepTokens nodes of the path at a time, a wave every fourth of
+// them: their rows into registers, then from there to their places.  Nodes ascend and lie at or past
+// their new places, so that what is still to be read lies past what has been written.  A thread a node
+// looks up both places first: the chain of reads (path, table, row) bounds the call.
+__global__ __launch_bounds__(kKeepWaves * 64) void kv_keep_q4_0(KeepArgs a) {
+  struct Move {
+    const uint8_t *source;  // the head's part of the page; nullptr: stays
+    uint8_t *target;
+    uint32_t from, to;  // tokens there
+  };
+  __shared__ Move s_move[kKeepTokens];
+  constexpr int kTurns = kKeepTokens / kKeepWaves, kRounds = (kKeepUnits + 63) / 64;
   const uint32_t request = blockIdx.x, head = blockIdx.y;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int32_t *const path = a.path + request * a.path_stride;
+  const int stride = static_cast<int>(min(a.path_stride, static_cast<size_t>(a.max_added)));
+  int node = threadIdx.x < kKeepTokens && static_cast<int>(threadIdx.x) < stride ? path[threadIdx.x] : -1;
   const Nodes nodes(a.first, a.length, request, 0x7fffffffu);
   const int most = min(nodes.count, static_cast<int>(a.max_added));
-  const int32_t *const path = a.path + request * a.path_stride;
-  const int count = min(a.count[request], static_cast<int>(min(
-                                              static_cast<size_t>(most), a.path_stride)));
+  const int count = min(a.count[request], min(most, stride));
   const PageHead lay(a.page_size, a.head_dim);
   const RowUnits units(a.head_dim);
   const int32_t *const table = a.block_table + request * a.table_stride;
@@ -129,28 +139,40 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_q4_0(KeepArgs a) {
                           : nullptr;
   };
   for (int k0 = 0; k0 < count; k0 += kKeepTokens) {
-    const uint32_t all = min(count - k0, kKeepTokens) * units.all;
-    const auto moves = [&](uint32_t i, bool write) {
-      const int k = k0 + static_cast<int>(i / units.all);
-      const uint32_t unit = i % units.all;
-      const int node = path[k];
-      if (node == k || node < 0 || node >= most)
-        return;
-      uint32_t from = 0, to = 0;
-      uint8_t *const source = place(static_cast<int64_t>(nodes.cached) + node, from);
-      uint8_t *const target = place(static_cast<int64_t>(nodes.cached) + k, to);
-      if (!source || !target)
-        return;
-      if (write)
-        *reinterpret_cast<uint16_t *>(target + units.at(lay, to, unit)) = s_row[i];
-      else
-        s_row[i] = *reinterpret_cast<const uint16_t *>(source + units.at(lay, from, unit));
-    };
-    for (uint32_t i = threadIdx.x; i < all; i += kKeepThreads)
-      moves(i, false);
+    if (threadIdx.x < kKeepTokens) {
+      const int k = k0 + static_cast<int>(threadIdx.x);
+      if (k0)
+        node = k < count ? path[k] : -1;
+      Move move{nullptr, nullptr, 0, 0};
+      if (k < count && node != k && node >= 0 && node < most) {
+        move.source = place(static_cast<int64_t>(nodes.cached) + node, move.from);
+        move.target = place(static_cast<int64_t>(nodes.cached) + k, move.to);
+        if (!move.target)
+          move.source = nullptr;
+      }
+      s_move[threadIdx.x] = move;
+    }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < all; i += kKeepThreads)
-      moves(i, true);
+    uint16_t row[kTurns][kRounds];
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const Move &move = s_move[wave + i * kKeepWaves];
+#pragma unroll
+      for (int j = 0; j < kRounds; ++j)
+        if (move.source && lane + 64u * j < units.all)
+          row[i][j] = *reinterpret_cast<const uint16_t *>(
+              move.source + units.at(lay, move.from, lane + 64 * j));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const Move &move = s_move[wave + i * kKeepWaves];
+#pragma unroll
+      for (int j = 0; j < kRounds; ++j)
+        if (move.source && lane + 64u * j < units.all)
+          *reinterpret_cast<uint16_t *>(move.target + units.at(lay, move.to, lane + 64 * j)) =
+              row[i][j];
+    }
     __syncthreads();
   }
 }
@@ -214,7 +236,7 @@ int tcrv_hip_kv_keep_q4_0(uint8_t *cache, size_t pages, size_t page_size, const 
                          static_cast<uint32_t>(kv_heads),
                          static_cast<uint32_t>(head_dim)};
   tcrv::kv_keep_q4_0<<<dim3(static_cast<unsigned>(requests), static_cast<unsigned>(kv_heads)),
-                       dim3(tcrv::kKeepThreads), 0, as_stream(stream)>>>(a);
+                       dim3(tcrv::kKeepWaves * 64), 0, as_stream(stream)>>>(a);
   return launch_status();
 }
 
