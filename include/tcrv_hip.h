@@ -628,9 +628,9 @@ TCRV_HIP_API int tcrv_hip_tree_tables(const int32_t *parents, const int32_t *fir
  * length[r] - the request's nodes, all: its token's `words` words of `ancestors`
  * (8-byte aligned; 64 words >= max_added, else TCRV_HIP_ERR_BAD_SIZE).  Bits past
  * the token's own are not looked at.  window > 0: of positions p - window + 1 .. p,
- * where p is the cached tokens' number plus the row's bits up to its own less one, and
- * a new token's position is that of its place among these bits.  A row whose bits
- * leave nothing, and no cached token, is zero. */
+ * where p is the cached tokens' number plus the row's bits up to its own less one (a
+ * row without bits counts as one), and a new token's position is that of its place
+ * among these bits.  A row whose bits leave nothing, and no cached token, is zero. */
 TCRV_HIP_API size_t tcrv_hip_attn_tree_q4_0_workspace_bytes(int elem, size_t requests,
                                                             size_t tokens, size_t max_added,
                                                             size_t max_length, size_t heads,

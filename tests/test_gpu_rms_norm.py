@@ -40,6 +40,10 @@ def rows_of(t, off, rows, n, stride):
     (9, 96, 0, 2), (4, 1000, 0, 0), (5, 1024, 32, 0), (3, 1025, 0, 0), (2, 1056, 0, 0),
     (3, 4096, 0, 0), (1, 4096, 0, 1), (2, 4100, 0, 0), (2, 5120, 4, 0), (1, 16384, 0, 0),
     (2, 16385, 0, 0), (2, 16416, 0, 0), (1, 40000, 0, 0), (1027, 64, 0, 0), (300, 320, 0, 0),
+    # many rows, of fewer lanes or registers each than a few rows take
+    (535, 300, 0, 0), (530, 512, 0, 0), (531, 800, 0, 0), (513, 1600, 0, 0), (521, 4096, 0, 0),
+    (514, 8192, 0, 0), (601, 35, 1, 1), (602, 301, 3, 1), (603, 1001, 0, 0), (513, 2001, 0, 0),
+    (515, 4001, 1, 3), (47, 128, 0, 0), (33, 256, 8, 0),
 ])
 def test_sum_norm_and_blocks(hip, dev, elem, tokens, n, pad, off):
     rng = np.random.default_rng(tokens * 100003 + n)

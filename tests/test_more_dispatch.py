@@ -1,0 +1,92 @@
+"""Which kernels the norm, the gated products and the attention over trees launch at a size, and their grids,
+replayed without a GPU (tests/launches.py)."""
+import re
+
+import pytest
+
+import launches
+import tcrv_hip
+
+A, B, C, D, E, F, G, H = ((k + 1) << 40 for k in range(8))
+KERNEL = r"(add_rms_norm_rows|gated_one|gated_spans|gated_tiles|attn_q4_0_(?:rows16|tiles|join_few|join))"
+
+
+def run(call):
+    status, made = launches.replay([call])[0]
+    assert status == 0
+    return [(re.search(KERNEL, x.name)[1], x.grid[0], x.block[0]) for x in made]
+
+
+def norm(elem, tokens, n, pad=0):
+    return "tcrv_hip_add_rms_norm", (tcrv_hip.FLOAT_ELEM[elem], A, n + pad, B, n + pad, C, n + pad, D,
+                                     1e-5, E, n + pad, F, n // 32 * 34, tokens, n)
+
+
+@pytest.mark.parametrize("args,want", [
+    # heads' rows: 16 a work-group
+    (("f16", 60000, 128), (3750, 256)), (("f32", 1, 256), (1, 256)), (("f16", 4096, 512), (256, 256)),
+    (("f32", 4096, 257), (1024, 256)),
+    # a few long rows, on as many threads as a work-group has
+    (("f32", 1, 4096), (1, 1024)), (("f16", 512, 8192), (512, 1024)), (("f32", 3, 1024), (3, 1024)),
+    # many: four, or one, a work-group
+    (("f16", 513, 1024), (129, 256)), (("f32", 4096, 1024), (1024, 256)), (("f16", 4096, 4096), (4096, 256)),
+    (("f32", 4096, 4096), (4096, 256)), (("f32", 4096, 4100), (4096, 1024)),
+    # past a row's registers
+    (("f32", 2, 16388), (2, 1024)), (("f16", 1000, 40000), (1000, 1024)),
+])
+def test_rows_of_the_norm(args, want):
+    (name, grid, block), = run(norm(*args))
+    assert (grid, block) == want
+
+
+def gated(tokens, n, wide, q8=False, elem="f32"):
+    return "tcrv_hip_gated_q4_0_q8_0", (tcrv_hip.FLOAT_ELEM[elem], 0, n, A, wide, B if q8 else 0,
+                                        wide // 32 * 34, C, D, n // 32 * 18, E, n // 32 * 34, wide,
+                                        tokens)
+
+
+@pytest.mark.parametrize("args,want", [
+    ((1, 4096, 11008), ("gated_one", 2752, 256)), ((1, 4096, 11008, True), ("gated_one", 344, 1024)),
+    ((1, 32, 33), ("gated_one", 9, 256)), ((1, 32, 33, True), ("gated_one", 2, 1024)),
+    ((2, 4096, 11008), ("gated_spans", 344, 512)), ((64, 4096, 11008), ("gated_spans", 688, 512)),
+    ((128, 4096, 14336), ("gated_tiles", 224, 512)), ((512, 4096, 14336), ("gated_tiles", 448, 512)),
+    ((2048, 4096, 14336), ("gated_tiles", 1792, 512)), ((2048, 64, 96), ("gated_spans", 192, 512)),
+])
+def test_kernel_of_the_products(args, want):
+    assert run(gated(*args)) == [want]
+
+
+def tree(elem, requests, tokens, nodes, length, heads, kv, dim, window=0):
+    return "tcrv_hip_attn_tree_q4_0", (
+        tcrv_hip.FLOAT_ELEM[elem], A, heads * dim, dim, B, 1 << 20, 16, C, 1 << 16, D, E, F,
+        -(-nodes // 64), requests, tokens, nodes, length, heads, kv, dim, dim ** -0.5, window, G,
+        heads * dim, dim, H, 1 << 50)
+
+
+@pytest.mark.parametrize("args,want", [
+    # up to 64 rows a kv head go on the tiles of few rows, whatever the requests
+    (("f32", 1, 7, 7, 538, 32, 8, 128), ["rows16", "join_few"]),
+    (("f16", 4, 64, 16, 100, 32, 8, 128), ["rows16"]),
+    (("f16", 64, 512, 8, 4104, 32, 8, 128), ["rows16", "join_few"]),
+    (("bf16", 1, 16, 16, 20, 8, 2, 64), ["rows16"]),
+    # more rows on those of prompts
+    (("f16", 6, 384, 64, 8256, 32, 8, 128), ["tiles", "join"]),
+    (("f16", 200, 200 * 64, 64, 600, 32, 8, 128), ["tiles"]),
+])
+def test_kernels_of_trees(args, want):
+    got = [name.replace("attn_q4_0_", "") for name, _, _ in run(tree(*args))]
+    assert got == want
+
+
+@pytest.mark.parametrize("nodes", [1, 16, 17, 200])
+@pytest.mark.parametrize("length", [210, 4000, 131072, 1 << 30])
+def test_workspace_of_trees_serves_every_window(nodes, length):
+    for requests, heads, kv, dim in ((1, 32, 8, 128), (64, 32, 8, 128), (5, 14, 2, 64), (3, 16, 4, 256)):
+        tokens = requests * nodes
+        need = tcrv_hip.attn_tree_q4_0_workspace_bytes("f16", requests, tokens, nodes, length, heads, kv,
+                                                       dim)
+        calls = []
+        for window in (0, 1, 100, 5000, 1 << 40):
+            name, args = tree("f16", requests, tokens, nodes, length, heads, kv, dim, window)
+            calls.append((name, args[:-1] + (need,)))
+        assert all(status == 0 for status, _ in launches.replay(calls))

@@ -23,7 +23,8 @@ constexpr int kTreeHeld = 8192;  // parents in LDS
 
 // A work-group a request, a thread a node, which walks up its ancestors: their numbers go down, so that
 // the words of its bits are made one after the other.  Parents are fetched once, into LDS: a walk is a
-// chain of reads.  The last work-group fills what lies past the last token.
+// chain of reads, one a generation, and bounds the call (4 requests of 64 nodes: 3.6 us, 301 of 17: 3.5 us,
+// where an empty kernel takes 1.5 us).  The last work-group fills what lies past the last token.
 __global__ __launch_bounds__(kTreeThreads) void tree_tables(const int32_t *parents,
                                                             const int32_t *first,
                                                             const int32_t *length,
@@ -108,7 +109,10 @@ constexpr int kKeepUnits = 2 * (256 / 4 + 256 / kQK);  // at most, of a row
 // A work-group a request and head takes kKeepTokens nodes of the path at a time, a wave every fourth of
 // them: their rows into registers, then from there to their places.  Nodes ascend and lie at or past
 // their new places, so that what is still to be read lies past what has been written.  A thread a node
-// looks up both places first: the chain of reads (path, table, row) bounds the call.
+// looks up both places first: the chain of reads (path, table, row) bounds the call.  The rows' units of
+// 16 bits lie in lines that hold four tokens', so that more is moved than the rows' bytes.  128 requests of
+// 64 drafted tokens, 8 heads of 128: 7.6 us (12.9 us with a look-up for each unit and the rows in LDS);
+// one request of 7: 2.7 us, where an empty kernel takes 1.5 us.
 __global__ __launch_bounds__(kKeepWaves * 64) void kv_keep_q4_0(KeepArgs a) {
   struct Move {
     const uint8_t *source;  // the head's part of the page; nullptr: stays
