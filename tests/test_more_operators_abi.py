@@ -157,7 +157,8 @@ def attn(requests, tokens, added, length=16, heads=1, kv=1, dim=64):
     (("tcrv_hip_kv_keep_q4_0", (P, 64, 16, Q, 8, R, S, T, 8, U, MOST, 8, 65535, 64)), OK),
     (attn(MOST, MOST, 1), OK), (attn(MOST + 1, MOST + 1, 1), LARGE),
     (attn(1 << 20, 1 << 20, 1, heads=16, kv=16), LARGE),
-    (attn(1, MOST, MOST, heads=1), OK), (attn(1, MOST, MOST, heads=64, kv=64), LARGE),
+    (attn(1, MOST, MOST, heads=1), OK), (attn(1, MOST, MOST, heads=127, kv=127), OK),
+    (attn(1, MOST, MOST, heads=128, kv=128), LARGE),
 ])
 def test_most_that_a_launch_holds(call, want):
     (got, made), = launches.replay([call])

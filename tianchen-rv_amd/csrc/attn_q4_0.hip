@@ -1616,12 +1616,16 @@ attn_q4_0_tiles(AttnArgs a) {
   }
 }
 
-// The stretches of a tile of attn_q4_0_rows16 together: a work-group takes a row of the tile that one
-// of the kernel's work-groups has begun, 4 elements a thread, and groups of head_dim / 4 threads share
-// out the stretches.
+// The stretches of a tile of attn_q4_0_rows16 together, of the tile that one of the kernel's work-groups has
+// begun, 4 elements a thread.  A work-group takes a row, and groups of head_dim / 4 threads share out
+// its stretches; where tiles are many (kSide) the groups take rows side by side, and share out those of
+// a tile of more than kFewStretches stretches one row after the other.  The same sums in the same order: a
+// group that has one stretch leaves it as it is.  Latency bounds it, the launch and two dependent reads: of
+// 512 work-groups' tiles of 16 rows of 128, f16, 10.5 us a work-group a row and 4.6 side by side.
 constexpr int kJoinThreads = 256;
+constexpr uint32_t kFewStretches = 4;  // head_dim 256 has as many groups
 
-template <typename T>
+template <typename T, bool kSide>
 __global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join_few(AttnArgs a, uint32_t head_dim) {
   __shared__ f32x4 s_o[kJoinThreads];
   __shared__ float2 s_ml[kJoinThreads];
@@ -1630,58 +1634,102 @@ __global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join_few(AttnArgs a, u
     return;
   const uint32_t stretches = begun.z - blockIdx.x + 1;
   const uint32_t kv_heads = a.heads / a.share, tile = begun.y / kv_heads;
-  const Span span(a, begun.x);
-  const uint32_t row = tile * kRows + blockIdx.y;
-  if (row >= span.rows)
-    return;
   const uint32_t per_head = head_dim / 4, groups = kJoinThreads / per_head;
   const uint32_t e = 4 * (threadIdx.x % per_head), group = threadIdx.x / per_head;
   // the first one's part is its work-group's second, the others' their first
-  const auto at = [&](uint32_t s) {
-    return (2 * (blockIdx.x + s) + (s == 0 ? 1 : 0)) * static_cast<size_t>(kRows) + blockIdx.y;
+  const auto at = [&](uint32_t s, uint32_t row) {
+    return (2 * (blockIdx.x + s) + (s == 0 ? 1 : 0)) * static_cast<size_t>(kRows) + row;
   };
   const float2 *const ml = reinterpret_cast<const float2 *>(
       a.parts + static_cast<size_t>(a.groups) * (2 * kRows) * head_dim);
-  float m = kNone, l = 0.0f;
-  f32x4 o{};
-  if (group < groups) {
-#pragma unroll 4
-    for (uint32_t s = group; s < stretches; s += groups) {
-      // as they come: 16 bytes of output and 8 of its maximum and sum in one turn
-      const float2 x = ml[at(s)];
-      const f32x4 v = *reinterpret_cast<const f32x4 *>(a.parts + at(s) * head_dim + e);
-      const float top = fmaxf(m, x.x);
-      const float f = m == top ? 1.0f : exp2_fast(m - top), h = x.x == top ? 1.0f : exp2_fast(x.x - top);
-      l = l * f + x.y * h;
-      o = o * f + v * h;
-      m = top;
+  const auto part = [&](uint32_t s, uint32_t row) {
+    return *reinterpret_cast<const f32x4 *>(a.parts + at(s, row) * head_dim + e);
+  };
+  const auto put = [&](const Span &span, uint32_t row, const f32x4 &o, float l) {
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      v[k] = l == 0.0f ? 0.0f : o[k] / l;
+    const uint32_t token = span.first + row / a.share;
+    const uint32_t head = (begun.y - tile * kv_heads) * a.share + row % a.share;
+    store_values<4>(static_cast<T *>(a.out) + static_cast<size_t>(token) * a.out_token +
+                        static_cast<size_t>(head) * a.out_head + e,
+                    v, a.out_vec);
+  };
+  if constexpr (kSide) {
+    const uint32_t row = blockIdx.y * groups + group;
+    if (stretches <= kFewStretches) {
+      if (group >= groups || row >= kRows)
+        return;
+      float2 x[kFewStretches];
+      f32x4 v[kFewStretches];
+#pragma unroll
+      for (uint32_t s = 0; s < kFewStretches; ++s) {
+        const uint32_t from = min(s, stretches - 1);
+        x[s] = ml[at(from, row)];
+        v[s] = part(from, row);
+      }
+      const Span span(a, begun.x);
+      if (tile * kRows + row >= span.rows)
+        return;
+      float top = kNone, l = 0.0f;
+      f32x4 o{};
+#pragma unroll
+      for (uint32_t s = 0; s < kFewStretches; ++s)
+        top = fmaxf(top, x[s].x);
+#pragma unroll
+      for (uint32_t s = 0; s < kFewStretches; ++s) {
+        if (s < stretches) {
+          const float f = x[s].x == top ? 1.0f : exp2_fast(x[s].x - top);
+          l += x[s].y * f;
+          o += v[s] * f;
+        }
+      }
+      put(span, tile * kRows + row, o, l);
+      return;
     }
   }
-  s_o[threadIdx.x] = o;
-  s_ml[threadIdx.x] = make_float2(m, l);
-  __syncthreads();
-  if (group != 0)
-    return;
-  float top = kNone;
-  for (uint32_t k = 0; k < groups; ++k)
-    top = fmaxf(top, s_ml[k * per_head + threadIdx.x].x);
-  o = f32x4{};
-  l = 0.0f;
-  for (uint32_t k = 0; k < groups; ++k) {
-    const float2 x = s_ml[k * per_head + threadIdx.x];
-    const float f = x.x == top ? 1.0f : exp2_fast(x.x - top);
-    l += x.y * f;
-    o += s_o[k * per_head + threadIdx.x] * f;
+  const Span span(a, begun.x);
+  const uint32_t rows = kSide ? groups : 1;
+  for (uint32_t r = 0; r < rows; ++r) {
+    const uint32_t place = blockIdx.y * rows + r, row = tile * kRows + place;
+    if (place >= kRows || row >= span.rows)
+      return;
+    float m = kNone, l = 0.0f;
+    f32x4 o{};
+    if (group < groups) {
+#pragma unroll 4
+      for (uint32_t s = group; s < stretches; s += groups) {
+        // as they come: 16 bytes of output and 8 of its maximum and sum in one turn
+        const float2 x = ml[at(s, place)];
+        const f32x4 v = part(s, place);
+        const float top = fmaxf(m, x.x);
+        const float f = m == top ? 1.0f : exp2_fast(m - top), h = x.x == top ? 1.0f : exp2_fast(x.x - top);
+        l = l * f + x.y * h;
+        o = o * f + v * h;
+        m = top;
+      }
+    }
+    if (r > 0)
+      __syncthreads();
+    s_o[threadIdx.x] = o;
+    s_ml[threadIdx.x] = make_float2(m, l);
+    __syncthreads();
+    if (group == 0) {
+      float top = kNone;
+      for (uint32_t k = 0; k < groups; ++k)
+        top = fmaxf(top, s_ml[k * per_head + threadIdx.x].x);
+      o = f32x4{};
+      l = 0.0f;
+      for (uint32_t k = 0; k < groups; ++k) {
+        const float2 x = s_ml[k * per_head + threadIdx.x];
+        const float f = x.x == top ? 1.0f : exp2_fast(x.x - top);
+        l += x.y * f;
+        o += s_o[k * per_head + threadIdx.x] * f;
+      }
+      put(span, row, o, l);
+    }
   }
-  float v[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    v[k] = l == 0.0f ? 0.0f : o[k] / l;
-  const uint32_t token = span.first + row / a.share;
-  const uint32_t head = (begun.y - tile * kv_heads) * a.share + row % a.share;
-  store_values<4>(static_cast<T *>(a.out) + static_cast<size_t>(token) * a.out_token +
-                      static_cast<size_t>(head) * a.out_head + e,
-                  v, a.out_vec);
 }
 
 // The parts of a row of attn_q4_0_tiles together, 4 elements a thread.  Of few parts a group of
@@ -1958,8 +2006,15 @@ void launch_all(AttnArgs a, Kernels k, const Plan &few, const Plan &many, size_t
     launch_rows16<NP, T, kTree>(a, head_dim, static_cast<unsigned>(few.launch), st);
     if (few.groups) {
       const size_t rows = std::min(static_cast<size_t>(a.max_added) * a.share, few.tile_rows);
-      tcrv::attn_q4_0_join_few<T>
-          <<<dim3(a.groups, static_cast<unsigned>(rows)), join_block, 0, st>>>(a, dim);
+      const size_t beside = tcrv::kJoinThreads / (dim / 4);
+      // tiles of few stretches, as far as the host knows them
+      if (few.groups <= 2 * requests * few.tiles * (a.heads / a.share))
+        tcrv::attn_q4_0_join_few<T, true>
+            <<<dim3(a.groups, static_cast<unsigned>((rows + beside - 1) / beside)), join_block, 0, st>>>(
+                a, dim);
+      else
+        tcrv::attn_q4_0_join_few<T, false>
+            <<<dim3(a.groups, static_cast<unsigned>(rows)), join_block, 0, st>>>(a, dim);
     }
   }
   if (k.many) {
