@@ -23,7 +23,7 @@ After a model's last layer the accepted path is known, and in every layer
     kv_keep_q4_0        the path's keys and values to follow the cached tokens
 
 Prompts go the same way with attn_q4_0.  Trees, paths and lengths are known here as the scheduler knows
-them, so that no call waits for the device.
+them, so that nothing is read back from the device.
 """
 import os
 import sys

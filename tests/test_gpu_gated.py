@@ -147,6 +147,74 @@ def test_larger_and_ragged(hip, dev, elem, tokens, n, wide_):
     Case(n, wide_, tokens, seed=3).check(hip, dev, elem, "silu")
 
 
+# Many features and tokens, where tiles of 64 and of 128 features serve (tests/test_more_dispatch.py holds that),
+# ragged both ways.
+TILES = {"tiles of 64": (500, 4090), "tiles of 128": (630, 4590)}
+
+
+@pytest.mark.parametrize("elem,n", [("f32", 32), ("f32", 96), ("f32", 1056), ("f16", 224), ("bf16", 416)])
+@pytest.mark.parametrize("tiles", TILES)
+def test_tiles(hip, dev, elem, n, tiles):
+    tokens, wide_ = TILES[tiles]
+    Case(n, wide_, tokens, seed=4).check(hip, dev, elem, "silu")
+
+
+@pytest.mark.parametrize("apart,layout", [((2, 2), "apart"), ((14, 34), "apart"), ((0, 0), "in turn")])
+@pytest.mark.parametrize("tiles", TILES)
+def test_tiles_of_strided_rows(hip, dev, apart, layout, tiles):
+    tokens, wide_ = TILES[tiles]
+    Case(160, wide_, tokens, seed=6, apart=apart, layout=layout).check(hip, dev, "f16", "gelu_tanh")
+
+
+@pytest.mark.parametrize("tiles", TILES)
+def test_tiles_of_extremes_and_scales_that_are_not_finite(hip, dev, tiles):
+    """Blocks of the largest quants, a token and two features whose scales are infinite or NaN: theirs alone are
+    lost."""
+    tokens, wide_ = TILES[tiles]
+    c = Case(288, wide_, tokens, seed=10)
+    for m, step, quants in ((c.gate, 18, 0x00), (c.up, 18, 0x00), (c.y, 34, 0x80)):
+        m.reshape(m.shape[0], -1, step)[::3, ::2, 2:] = quants
+    plain_ = c.run(hip, dev, "f32", "relu")[0]
+    want, tol = want_of(c.gate, c.up, c.y, "relu", "f32")
+    assert (np.abs(plain_ - want) <= tol).all()
+    clean = c.run(hip, dev, "f32", "silu")[0].copy()
+    inf, nan = (np.array([x], np.uint16).view(np.uint8) for x in (0x7C00, 0x7E00))
+    c.y[7, 102:104], c.gate[40, 144:146], c.up[wide_ - 1, 0:2] = inf, nan, inf
+    got = c.run(hip, dev, "f32", "silu")[0]
+    lost = np.zeros(got.shape, bool)
+    lost[7], lost[:, [40, wide_ - 1]] = True, True
+    assert not np.isfinite(got[lost]).any()
+    assert np.array_equal(got[~lost], clean[~lost])
+
+
+@pytest.mark.parametrize("tokens,n,wide_", [(1, 64, 70), (6, 64, 70), (500, 64, 4090)])
+def test_rows_more_than_32_bits_apart(hip, dev, tokens, n, wide_):
+    """Weight rows, rows of activations and of results whose offsets pass 2^32 bytes, the products and their
+    blocks what they are side by side."""
+    c = Case(n, wide_, tokens, seed=12)
+    out, out8 = c.run(hip, dev, "f16", "silu")
+    bx = (1 << 33) // wide_ // 2 * 2
+    by, step, row8 = ((1 << 33) // tokens // 2 * 2 if tokens > 1 else 0 for _ in range(3))
+    by = min(by, 1 << 26)
+    bx = min(bx, 1 << 26)
+
+    def apart(rows, stride):
+        t = torch.empty(rows.shape[0] * stride + rows.shape[1] if rows.shape[0] > 1 else rows.shape[1],
+                        dtype=torch.uint8, device=dev)
+        torch.as_strided(t, rows.shape, (stride, 1)).copy_(to_dev(rows, dev))
+        return t
+
+    gate, up, y = apart(c.gate, bx), apart(c.up, bx), apart(c.y, by)
+    to = torch.empty(max(tokens - 1, 0) * step + wide_, dtype=torch.float16, device=dev)
+    to8 = torch.empty(max(tokens - 1, 0) * row8 + wide_ // 32 * 34, dtype=torch.uint8, device=dev)
+    hip.gated_q4_0_q8_0("f16", "silu", n, to, step, to8, row8, gate, up, bx, y, by, wide_, tokens)
+    assert np.array_equal(wide(torch.as_strided(to, (tokens, wide_), (step, 1)).contiguous()), out)
+    got = torch.as_strided(to8, (tokens, wide_ // 32 * 34), (row8, 1)).contiguous()
+    assert np.array_equal(from_dev(got), out8)
+    del gate, up, y, to, to8, got
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("tokens", [1, 3, 40, 140])
 def test_activations(hip, dev, act, tokens):

@@ -161,3 +161,24 @@ def test_captured_and_replayed(hip, dev):
         h, y = plain(a, b, None)
         assert np.array_equal(from_dev(total), h)
         assert np.array_equal(from_dev(q8).reshape(-1), synth.quantize_q8_0(y))
+
+
+def test_rows_more_than_32_bits_apart(hip, dev):
+    n, tokens, stride = 1000, 300, 1 << 23
+    rng = np.random.default_rng(8)
+    x, r = (kv_plain.round_to(rng.standard_normal((tokens, n)), "f16") for _ in range(2))
+    h, y = plain(x, r, None)
+    far = [torch.empty((tokens - 1) * stride + n, dtype=torch.float16, device=dev) for _ in range(4)]
+    rows = [torch.as_strided(t, (tokens, n), (stride, 1)) for t in far]
+    for t, v in zip(rows, (x, r)):
+        t.copy_(dev_rows(v, "f16", dev))
+    row8 = 1 << 24
+    q8 = torch.empty((tokens - 1) * row8 + 31 * 34, dtype=torch.uint8, device=dev)
+    hip.add_rms_norm("f16", far[0], stride, far[1], stride, far[2], stride, None, EPS, far[3], stride, q8,
+                     row8, tokens, n)
+    for t, want in zip(rows[2:], (h, y)):
+        assert np.array_equal(wide(t.contiguous()), kv_plain.round_to(want, "f16"))
+    got = torch.as_strided(q8, (tokens, 31 * 34), (row8, 1)).contiguous()
+    assert np.array_equal(from_dev(got).reshape(-1), synth.quantize_q8_0(np.ascontiguousarray(y[:, :992])))
+    del far, rows, q8, got
+    torch.cuda.empty_cache()

@@ -45,6 +45,7 @@ def words_of(trees, words):
 @pytest.mark.parametrize("nodes,words,room", [
     ([1], 1, 0), ([64], 1, 3), ([65], 2, 0), ([0, 5, 0, 0, 9], 1, 1), ([300, 1, 17], 5, 0),
     ([130, 70], 2, -20), ([200], 2, 0), ([9000], 1, 0), ([3] * 400, 1, 60), ([12, 12], 3, -12),
+    ([5, 3], 2, 3000),
 ])
 def test_tables(hip, dev, nodes, words, room):
     """Also nodes that have no bits, more tokens than are asked for, and parents that are none."""
@@ -361,3 +362,29 @@ def test_keep_of_what_is_not_there(hip, dev):
     hip.kv_keep_q4_0(b[0], t.pages, 16, b[1], t.stride, b[2], b[3], to_dev(path, dev), 7,
                      to_dev(np.array([0, -3, -2 ** 31], np.int32), dev), 3, 40, 2, 64)
     assert np.array_equal(from_dev(b[0]).reshape(t.cache.bytes.shape), t.cache.bytes)
+
+
+# ------------------------------------------------------- caches past 4 GiB ---
+
+@pytest.mark.parametrize("nodes", [[7, 16], [80, 2]])
+def test_pages_past_32_bits(hip, dev, nodes):
+    """The pages lie more than 2^32 bytes into the cache: the same attention and the same moves."""
+    t = Trees(dev, "f16", [300, 90], nodes, 8, 2, 128, 16, seed=13)
+    want = wide(t.run(hip))
+    near = t.buffers()
+    page_bytes = near[0].numel() // t.pages
+    pages = (9 << 30) // page_bytes
+    cache = torch.empty(pages * page_bytes, dtype=torch.uint8, device=dev)
+    base = pages - t.pages
+    cache[base * page_bytes:] = near[0].view(-1)
+    used = (near[1] >= 0) & (near[1] < t.pages)
+    far = [cache, torch.where(used, near[1] + base, near[1].clamp(max=-1)), *near[2:]]
+    few, t.pages = t.pages, pages
+    assert np.array_equal(wide(t.run(hip, bufs=tuple(far))), want)
+    path = to_dev(np.array([[1, 4, 6], [0, 1, 1]], np.int32), dev)
+    count = to_dev(np.array([3, 2], np.int32), dev)
+    for b, n in ((near, few), (far, pages)):
+        hip.kv_keep_q4_0(b[0], n, 16, b[1], t.stride, b[2], b[3], path, 3, count, 2, max(nodes), 2, 128)
+    assert np.array_equal(from_dev(cache[base * page_bytes:]), from_dev(near[0].view(-1)))
+    del far, cache
+    torch.cuda.empty_cache()

@@ -51,6 +51,8 @@ def gated(tokens, n, wide, q8=False, elem="f32"):
     ((2, 4096, 11008), ("gated_spans", 344, 512)), ((64, 4096, 11008), ("gated_spans", 688, 512)),
     ((128, 4096, 14336), ("gated_tiles", 224, 512)), ((512, 4096, 14336), ("gated_tiles", 448, 512)),
     ((2048, 4096, 14336), ("gated_tiles", 1792, 512)), ((2048, 64, 96), ("gated_spans", 192, 512)),
+    # tiles of 64 and of 128 features, of tests/test_gpu_gated.py
+    ((500, 32, 4090), ("gated_tiles", 64 * 4, 512)), ((630, 32, 4590), ("gated_tiles", 36 * 5, 512)),
 ])
 def test_kernel_of_the_products(args, want):
     assert run(gated(*args)) == [want]

@@ -24,7 +24,7 @@ constexpr int kTreeHeld = 8192;  // parents in LDS
 // A work-group a request, a thread a node, which walks up its ancestors: their numbers go down, so that
 // the words of its bits are made one after the other.  Parents are fetched once, into LDS: a walk is a
 // chain of reads, one a generation, and bounds the call (4 requests of 64 nodes: 3.6 us, 301 of 17: 3.5 us,
-// where an empty kernel takes 1.5 us).  The last work-group fills what lies past the last token.
+// where an empty kernel takes 1.5 us).  The work-groups past the requests' fill what lies past the last token.
 __global__ __launch_bounds__(kTreeThreads) void tree_tables(const int32_t *parents,
                                                             const int32_t *first,
                                                             const int32_t *length,
@@ -32,9 +32,10 @@ __global__ __launch_bounds__(kTreeThreads) void tree_tables(const int32_t *paren
                                                             size_t words, int32_t *positions,
                                                             uint32_t tokens) {
   __shared__ int32_t s_parent[kTreeHeld];
-  if (blockIdx.x == requests) {
-    const uint32_t end = requests ? max(first[requests], 0) : 0;
-    for (uint32_t i = end + threadIdx.x; i < tokens; i += kTreeThreads) {
+  if (blockIdx.x >= requests) {
+    const uint64_t end = requests ? max(first[requests], 0) : 0;
+    const uint64_t by = static_cast<uint64_t>(gridDim.x - requests) * kTreeThreads;
+    for (uint64_t i = end + (blockIdx.x - requests) * kTreeThreads + threadIdx.x; i < tokens; i += by) {
       positions[i] = -1;
       for (size_t w = 0; w < words; ++w)
         ancestors[i * words + w] = 0;
@@ -201,7 +202,9 @@ int tcrv_hip_tree_tables(const int32_t *parents, const int32_t *first, const int
   if (!aligned_to(ancestors, 8) || !aligned4(positions) || !aligned4(parents) || !aligned4(first) ||
       !aligned4(length))
     return TCRV_HIP_ERR_MISALIGNED;
-  tcrv::tree_tables<<<dim3(static_cast<unsigned>(requests) + 1), dim3(tcrv::kTreeThreads), 0,
+  // what may lie past the last token: a pass of up to 256 work-groups
+  const size_t fill = std::min({(max_tokens - 1) / tcrv::kTreeThreads + 1, size_t{256}, kMostGroups - requests});
+  tcrv::tree_tables<<<dim3(static_cast<unsigned>(requests + fill)), dim3(tcrv::kTreeThreads), 0,
                       as_stream(stream)>>>(parents, first, length, static_cast<uint32_t>(requests),
                                            ancestors, words, positions,
                                            static_cast<uint32_t>(max_tokens));
