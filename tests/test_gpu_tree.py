@@ -45,7 +45,7 @@ def words_of(trees, words):
 @pytest.mark.parametrize("nodes,words,room", [
     ([1], 1, 0), ([64], 1, 3), ([65], 2, 0), ([0, 5, 0, 0, 9], 1, 1), ([300, 1, 17], 5, 0),
     ([130, 70], 2, -20), ([200], 2, 0), ([9000], 1, 0), ([3] * 400, 1, 60), ([12, 12], 3, -12),
-    ([5, 3], 2, 3000),
+    ([5, 3], 2, 3000), ([4096, 64, 128], 64, 0), ([4200, 4097], 66, 2), ([4160], 3, 0),
 ])
 def test_tables(hip, dev, nodes, words, room):
     """Also nodes that have no bits, more tokens than are asked for, and parents that are none."""
@@ -73,6 +73,21 @@ def test_tables(hip, dev, nodes, words, room):
     assert np.array_equal(got[:most].view(np.uint64), want) and (got[most:] == 0x5555).all()
     got = from_dev(positions)
     assert np.array_equal(got[:most], where) and (got[most:] == 99).all()
+
+
+@pytest.mark.parametrize("nodes", [64, 65, 640, 4300])
+def test_tables_of_chains_and_stars(hip, dev, nodes):
+    """The deepest tree, the flattest, one whose paths go through every second word, and one by twos."""
+    words = -(-nodes // 64)
+    i = np.arange(nodes)
+    for parents in (i - 1, np.zeros_like(i) - (i == 0), i - 65, i - 2):
+        tree = [int(max(p, -1)) for p in parents]
+        bits = torch.zeros(nodes, words, dtype=torch.int64, device=dev)
+        positions = torch.zeros(nodes, dtype=torch.int32, device=dev)
+        hip.tree_tables(to_dev(np.array(tree, np.int32), dev), to_dev(np.array([0, nodes], np.int32), dev),
+                        to_dev(np.array([nodes + 7], np.int32), dev), 1, bits, words, positions, nodes)
+        assert np.array_equal(from_dev(bits).view(np.uint64), words_of([tree], words))
+        assert from_dev(positions).tolist() == [7 + d for d in bits_of(tree)[1]]
 
 
 def test_tables_of_nothing(hip, dev):
