@@ -79,10 +79,11 @@ __device__ __forceinline__ Q8Block load_q8(const uint8_t *p) {
 }
 
 // ---------------------------------------------------------------------------
-// One token: a wave takes a feature, a lane a pair of the blocks of its two rows (or the one that they have).  A
-// work-group is four features; of the 32 of a Q8_0 block (kBlocks) its sixteen waves take two each.  The read of
-// the weights bounds it: 2 x 14336 features of 4096, past the last-level cache, 12.6 us (5.2 TB/s) into elements and
-// 13.9 us into Q8_0; 2 x 4096 of 4096 5.4 us.
+// One token, or a few: a wave takes a feature, a lane a pair of the blocks of its two rows (or the one that they
+// have).  A work-group is four features; of the 32 of a Q8_0 block (kBlocks) its sixteen waves take two each.  The
+// read of the weights bounds it: 2 x 14336 features of 4096, past the last-level cache, 12.6 us (5.2 TB/s) into
+// elements and 13.9 us into Q8_0; 2 x 4096 of 4096 5.4 us.  Two features a wave, which share the tokens' loads,
+// took as long for 2 tokens and longer for 4: those are bound by VALU issue.
 // ---------------------------------------------------------------------------
 constexpr int one_waves(bool blocks) { return blocks ? 16 : 4; }
 
@@ -122,24 +123,26 @@ __device__ __forceinline__ int seed_of(const uint32_t (&y)[8]) {
   return -8 * sum;
 }
 
-template <typename T, bool kPairs, bool kBlocks>
+template <typename T, int kTokens, bool kPairs, bool kBlocks>
 __global__ __launch_bounds__(one_waves(kBlocks) * 64) void gated_one(GatedArgs a) {
   constexpr int kWaves = one_waves(kBlocks), kTurns = kBlocks ? 2 : 1, kFeatures = kWaves * kTurns;
-  __shared__ float s_out[kFeatures];
+  __shared__ __align__(16) float s_out[kTokens][kFeatures];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t at = blockIdx.x * kFeatures;
   const uint32_t items = kPairs ? (a.nb + 1) / 2 : a.nb;
+  // past the last one that one again
+  const auto token = [&](uint32_t n) { return a.vy + min(n, a.nc - 1) * a.by; };
   for (int turn = 0; turn < kTurns; ++turn) {
     const size_t feature = min(at + turn * kWaves + wave, a.nr - 1);
     const uint8_t *const row[2] = {a.gate + feature * a.bx, a.up + feature * a.bx};
-    float acc[2] = {};
+    float acc[kTokens][2] = {};
     for (uint32_t i0 = 0; i0 < items; i0 += 64) {
       const uint32_t i = min(i0 + lane, items - 1);
       const bool live = i0 + lane < items;
       if constexpr (kPairs) {
         // an odd number's last block is the second of the pair with the one before it
         const uint32_t b = min(2 * i, a.nb - 2);
-        uint32_t w[2][9], y[17];
+        uint32_t w[2][9];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const u32a2 *const p = reinterpret_cast<const u32a2 *>(row[r] + b * kQ4Bytes);
@@ -153,63 +156,73 @@ __global__ __launch_bounds__(one_waves(kBlocks) * 64) void gated_one(GatedArgs a
           }
           w[r][8] = p[8];
         }
-        const u32a2 *const p = reinterpret_cast<const u32a2 *>(a.vy + b * kQ8Bytes);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const u32x4a2 v = *reinterpret_cast<const u32x4a2 *>(p + 4 * k);
-          y[4 * k] = v.x;
-          y[4 * k + 1] = v.y;
-          y[4 * k + 2] = v.z;
-          y[4 * k + 3] = v.w;
-        }
-        y[16] = p[16];
-        // the even block's quants lie 2 bytes off a dword, the odd one's on one
-        uint32_t even[8], odd[8];
+        for (int n = 0; n < kTokens; ++n) {
+          const u32a2 *const p = reinterpret_cast<const u32a2 *>(token(n) + b * kQ8Bytes);
+          uint32_t y[17];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          even[k] = funnel16(y[k], y[k + 1]);
-          odd[k] = y[k + 9];
-        }
-        const int even_seed = seed_of(even), odd_seed = seed_of(odd);
-        const float even_d = live && b == 2 * i ? fp16_bits_to_f32(y[0] & 0xffffu) : 0.0f;
-        const float odd_d = live ? fp16_bits_to_f32(y[8] >> 16) : 0.0f;
+          for (int k = 0; k < 4; ++k) {
+            const u32x4a2 v = *reinterpret_cast<const u32x4a2 *>(p + 4 * k);
+            y[4 * k] = v.x;
+            y[4 * k + 1] = v.y;
+            y[4 * k + 2] = v.z;
+            y[4 * k + 3] = v.w;
+          }
+          y[16] = p[16];
+          // the even block's quants lie 2 bytes off a dword, the odd one's on one
+          uint32_t even[8], odd[8];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint32_t e[4] = {funnel16(w[r][0], w[r][1]), funnel16(w[r][1], w[r][2]),
-                                 funnel16(w[r][2], w[r][3]), funnel16(w[r][3], w[r][4])};
-          const uint32_t o[4] = {w[r][5], w[r][6], w[r][7], w[r][8]};
-          acc[r] = fmaf(block_sum(e, even, even_seed) * fp16_bits_to_f32(w[r][0] & 0xffffu), even_d,
-                        acc[r]);
-          acc[r] = fmaf(block_sum(o, odd, odd_seed) * fp16_bits_to_f32(w[r][4] >> 16), odd_d, acc[r]);
+          for (int k = 0; k < 8; ++k) {
+            even[k] = funnel16(y[k], y[k + 1]);
+            odd[k] = y[k + 9];
+          }
+          const int even_seed = seed_of(even), odd_seed = seed_of(odd);
+          const float even_d = live && b == 2 * i ? fp16_bits_to_f32(y[0] & 0xffffu) : 0.0f;
+          const float odd_d = live ? fp16_bits_to_f32(y[8] >> 16) : 0.0f;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t e[4] = {funnel16(w[r][0], w[r][1]), funnel16(w[r][1], w[r][2]),
+                                   funnel16(w[r][2], w[r][3]), funnel16(w[r][3], w[r][4])};
+            const uint32_t o[4] = {w[r][5], w[r][6], w[r][7], w[r][8]};
+            float &to = acc[n][r];
+            to = fmaf(block_sum(e, even, even_seed) * fp16_bits_to_f32(w[r][0] & 0xffffu), even_d, to);
+            to = fmaf(block_sum(o, odd, odd_seed) * fp16_bits_to_f32(w[r][4] >> 16), odd_d, to);
+          }
         }
       } else {
         const Q4Block w[2] = {load_q4(row[0] + i * kQ4Bytes), load_q4(row[1] + i * kQ4Bytes)};
-        const Q8Block b = load_q8(a.vy + i * kQ8Bytes);
-        uint32_t y[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          y[k] = b.q[0][k];
-          y[k + 4] = b.q[1][k];
-        }
-        const int seed = seed_of(y);
-        const float d = live ? fp16_bits_to_f32(b.d) : 0.0f;
+        for (int n = 0; n < kTokens; ++n) {
+          const Q8Block b = load_q8(token(n) + i * kQ8Bytes);
+          uint32_t y[8];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint32_t q[4] = {w[r].q.x, w[r].q.y, w[r].q.z, w[r].q.w};
-          acc[r] = fmaf(block_sum(q, y, seed) * fp16_bits_to_f32(w[r].d), d, acc[r]);
+          for (int k = 0; k < 4; ++k) {
+            y[k] = b.q[0][k];
+            y[k + 4] = b.q[1][k];
+          }
+          const int seed = seed_of(y);
+          const float d = live ? fp16_bits_to_f32(b.d) : 0.0f;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t q[4] = {w[r].q.x, w[r].q.y, w[r].q.z, w[r].q.w};
+            acc[n][r] = fmaf(block_sum(q, y, seed) * fp16_bits_to_f32(w[r].d), d, acc[n][r]);
+          }
         }
       }
     }
-    const float g = lanes_sum(acc[0]), u = lanes_sum(acc[1]);
-    if (lane == 63)
-      s_out[turn * kWaves + wave] = activation(g, a.act) * u;
+#pragma unroll
+    for (int n = 0; n < kTokens; ++n) {
+      const float g = lanes_sum(acc[n][0]), u = lanes_sum(acc[n][1]);
+      if (lane == 63)
+        s_out[n][turn * kWaves + wave] = activation(g, a.act) * u;
+    }
   }
   __syncthreads();
-  if (threadIdx.x < kFeatures / 4) {
-    const int part = threadIdx.x;
-    const float v[4] = {s_out[4 * part], s_out[4 * part + 1], s_out[4 * part + 2],
-                        s_out[4 * part + 3]};
-    emit<T, kBlocks>(a, 0, at, part, v);
+  const uint32_t part = threadIdx.x % (kFeatures / 4), n = threadIdx.x / (kFeatures / 4);
+  if (n < kTokens && n < a.nc) {
+    const float4 x = *reinterpret_cast<const float4 *>(&s_out[n][4 * part]);
+    const float v[4] = {x.x, x.y, x.z, x.w};
+    emit<T, kBlocks>(a, n, at, static_cast<int>(part), v);
   }
 }
 
@@ -621,19 +634,29 @@ template <typename T, int kFT> int launch_tiles(const GatedArgs &a, hipStream_t 
   return tcrv_host::launch_status();
 }
 
+template <typename T, int kTokens> int launch_one(const GatedArgs &a, hipStream_t st) {
+  const bool pairs = a.nb > 1;
+  const dim3 grid(static_cast<unsigned>(up_by(a.nr, a.q8 ? kQK : one_waves(false))));
+  const dim3 block(one_waves(a.q8 != nullptr) * 64);
+  if (a.q8)
+    pairs ? gated_one<T, kTokens, true, true><<<grid, block, 0, st>>>(a)
+          : gated_one<T, kTokens, false, true><<<grid, block, 0, st>>>(a);
+  else
+    pairs ? gated_one<T, kTokens, true, false><<<grid, block, 0, st>>>(a)
+          : gated_one<T, kTokens, false, false><<<grid, block, 0, st>>>(a);
+  return tcrv_host::launch_status();
+}
+
 template <typename T> int launch_elem(const GatedArgs &a, hipStream_t st) {
-  if (a.nc == 1) {
-    const bool pairs = a.nb > 1;
-    const dim3 grid(static_cast<unsigned>(up_by(a.nr, a.q8 ? kQK : one_waves(false))));
-    const dim3 block(one_waves(a.q8 != nullptr) * 64);
-    if (a.q8)
-      pairs ? gated_one<T, true, true><<<grid, block, 0, st>>>(a)
-            : gated_one<T, false, true><<<grid, block, 0, st>>>(a);
-    else
-      pairs ? gated_one<T, true, false><<<grid, block, 0, st>>>(a)
-            : gated_one<T, false, false><<<grid, block, 0, st>>>(a);
-    return tcrv_host::launch_status();
-  }
+  // Each token more costs gated_one 3.5 us beside its 12.6 at 14336 features of 4096, gated_spans nothing; us,
+  // gated_one / gated_spans: 2 tokens, 4096 features 6.8 / 13.5, 11008 13 / 21, 14336 16 / 23 and into Q8_0 20 / 23;
+  // 4 tokens, 4096 9.5 / 13.5, 11008 19 / 21, 14336 24 / 23, into Q8_0 4096 15.1 / 13.7.
+  if (a.nc == 1)
+    return launch_one<T, 1>(a, st);
+  if (a.nc == 2)
+    return launch_one<T, 2>(a, st);
+  if (a.nc <= 4 && !a.q8 && a.nr <= 12288)
+    return launch_one<T, 4>(a, st);
   // By what the kernels take for a block of K, in ns: rounds of 256 work-groups, one a CU, of the tiles; the
   // spans', two a CU, go on as CUs are free.  Measured at K 4096, us, spans / 64 features x 128 tokens / 128 x
   // 128: 11008 features x 33 tokens 33 / 58 / 92, 14336 x 128 69 / 62 / 95, 11008 x 200 91 / 118 / 96, 4096 x
