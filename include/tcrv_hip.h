@@ -586,7 +586,8 @@ TCRV_HIP_API int tcrv_hip_add_rms_norm(int elem, const void *x, size_t x_token,
  *   GELU       g (1 + erf(g / sqrt(2))) / 2
  *   RELU       max(g, 0)
  * Integer sums of a block are exact, the sums of blocks f32 in an order that follows
- * the sizes (not the one order of the GEMM); the same call gives the same bits.  An
+ * the sizes and which outputs are asked for (not the one order of the GEMM); the same
+ * call gives the same bits.  An
  * output whose rows hold a scale that is not finite is NaN or infinite.
  * nr up to 2^26 - 4, rows and strides bx and by up to 2^26 bytes, else
  * TCRV_HIP_ERR_TOO_LARGE. */

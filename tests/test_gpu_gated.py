@@ -116,15 +116,15 @@ class Case:
         assert (b[:, nb * 34 if q8 else 0:] == 0xEE).all() and (got8[self.tokens * row8:] == 0xEE).all()
         return a[:, :self.wide], b[:, :nb * 34]
 
-    def check(self, hip, dev, elem, act):
-        got, got8 = self.run(hip, dev, elem, act)
+    def check(self, hip, dev, elem, act, q8=True):
+        got, got8 = self.run(hip, dev, elem, act, q8=q8)
         want, tol = want_of(self.gate, self.up, self.y, act, elem)
         off = np.abs(got - want)
         assert np.isfinite(got).all()
         assert (off <= tol).all(), (off / tol).max()
         whole = self.wide // 32 * 32
-        exact = got if elem == "f32" else self.run(hip, dev, "f32", act, q8=False)[0]
-        if whole:
+        exact = got if elem == "f32" or not q8 else self.run(hip, dev, "f32", act)[0]
+        if whole and q8:
             assert np.array_equal(got8.reshape(-1),
                                   synth.quantize_q8_0(np.ascontiguousarray(exact[:, :whole])))
         return got
@@ -135,6 +135,13 @@ class Case:
 @pytest.mark.parametrize("n,wide_", [(32, 32), (64, 33), (96, 31), (288, 100), (2080, 64)])
 def test_sizes(hip, dev, elem, tokens, n, wide_):
     Case(n, wide_, tokens).check(hip, dev, elem, "silu")
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5, 33, 70])
+@pytest.mark.parametrize("n,wide_", [(32, 15), (64, 33), (96, 48), (544, 2050), (288, 4100), (2080, 64)])
+def test_elements_alone(hip, dev, elem, tokens, n, wide_):
+    Case(n, wide_, tokens, seed=2).check(hip, dev, elem, "silu", q8=False)
 
 
 @pytest.mark.parametrize("elem", ELEMS)
@@ -235,8 +242,9 @@ def test_strides(hip, dev, tokens, apart, layout):
         c.check(hip, dev, elem, "gelu_tanh")
 
 
-@pytest.mark.parametrize("tokens", [1, 5, 140])
+@pytest.mark.parametrize("tokens", [1, 2, 5, 140])
 def test_one_output_or_the_other(hip, dev, tokens):
+    """The same bits, where the same order of sums serves both."""
     c = Case(128, 96, tokens, seed=8)
     both = c.run(hip, dev, "f16", "relu")
     assert np.array_equal(c.run(hip, dev, "f16", "relu", q8=False)[0], both[0])

@@ -50,7 +50,10 @@ def gated(tokens, n, wide, q8=False, elem="f32"):
     ((1, 32, 33), ("gated_one", 9, 256)), ((1, 32, 33, True), ("gated_one", 2, 1024)),
     ((2, 4096, 11008), ("gated_one", 2752, 256)), ((2, 4096, 11008, True), ("gated_one", 344, 1024)),
     ((4, 4096, 11008), ("gated_one", 2752, 256)), ((3, 4096, 11008, True), ("gated_spans", 344, 512)),
-    ((4, 4096, 14336), ("gated_spans", 448, 512)), ((5, 4096, 11008), ("gated_spans", 344, 512)), ((64, 4096, 11008), ("gated_spans", 688, 512)),
+    ((4, 4096, 14336), ("gated_spans", 448, 512)), ((5, 4096, 11008), ("gated_spans", 344, 512)),
+    # 16 features a work-group
+    ((5, 4096, 4096), ("gated_spans", 256, 512)), ((5, 4096, 4097), ("gated_spans", 129, 512)),
+    ((64, 4096, 2048), ("gated_spans", 256, 512)), ((64, 4096, 4096, True), ("gated_spans", 256, 512)), ((64, 4096, 11008), ("gated_spans", 688, 512)),
     ((128, 4096, 14336), ("gated_tiles", 224, 512)), ((512, 4096, 14336), ("gated_tiles", 448, 512)),
     ((2048, 4096, 14336), ("gated_tiles", 1792, 512)), ((2048, 64, 96), ("gated_spans", 192, 512)),
     # tiles of 64 and of 128 features, of tests/test_gpu_gated.py

@@ -402,7 +402,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void gated_tiles(GatedArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Some tens of tokens: 32 features x 32 tokens a work-group.  Sixteen blocks of its rows at a time go to LDS as
+// Some tens of tokens: 32 (or 16) features x 32 tokens a work-group.  Sixteen blocks of its rows at a time go to LDS as
 // they lie in memory, in pieces of 16 bytes, and each of the eight waves takes a pair of them through both
 // tiles; the waves' sums come together at the end.
 //
@@ -412,37 +412,40 @@ __global__ __launch_bounds__(kTileThreads, 2) void gated_tiles(GatedArgs a) {
 // scale in group 0 and the odd one in group 1, the operands of the v_mfma_f32_32x32x8_f16 that gives the
 // products of the scales.  Quants stay in the upper half of their bytes, 16 (n - 8) with a flipped top bit.
 //
-// Latency bounds it where work-groups are one or two a CU: the chunks' loads, two under way.  2 x 11008 features of
-// 4096, 29 tokens, 20 us (23 past the last-level cache; the weights alone 10.5 at a copy's rate); 2 x 14336 and 64
-// tokens 41 us.
+// Where work-groups are one or two a CU the chain of a chunk bounds it, reads of LDS, two products and the sums'
+// scaling: more chunks' loads under way or sixteen waves a work-group changed nothing.  2 x 11008 features of 4096,
+// 29 tokens, 20 us (23 past the last-level cache; the weights alone 10.5 at a copy's rate); 2 x 14336 and 64 tokens
+// 41 us.
 // ---------------------------------------------------------------------------
 constexpr int kSpanWaves = 8, kSpanThreads = kSpanWaves * 64, kSpanBlocks = 2 * kSpanWaves;
 
-struct Spans {
+// kTiles: of 32 weight rows.  Two are 32 features' gate and up rows; one holds those of 16.
+template <int kTiles> struct Spans {
   static constexpr int kWSpan = kSpanBlocks * kQ4Bytes, kYSpan = kSpanBlocks * kQ8Bytes;
   // twice an odd number of dwords: a dword of 32 rows in banks of its own each
   static constexpr int kWRow = kWSpan + 8, kYRow = kYSpan + 8;
   static_assert(kWRow % 16 == 8 && kYRow % 16 == 8, "");
   // pieces by 64, of one matrix each; a thread's
   static constexpr int kWGroups = 32 * (kWSpan / 16) / 64, kYGroups = 32 * (kYSpan / 16) / 64;
-  static constexpr int kGroups = 2 * kWGroups + kYGroups;
+  static constexpr int kFeatures = 16 * kTiles;
+  static constexpr int kGroups = kTiles * kWGroups + kYGroups;
   static constexpr int kPieces = (kGroups + kSpanWaves - 1) / kSpanWaves;
-  static constexpr int kYAt = 64 * kWRow, kStage = kYAt + 32 * kYRow;
+  static constexpr int kYAt = 32 * kTiles * kWRow, kStage = kYAt + 32 * kYRow;
   static constexpr int kMine = 16 / kSpanWaves;  // a lane's sums of a projection
   static constexpr int kParts = kSpanWaves * 16 * 64 * 4, kOutRow = 36;
   static constexpr int kLds = 2 * kStage;
   static_assert(kLds >= kParts + 32 * kOutRow * 4, "");
 };
 
-template <typename T>
+template <typename T, int kTiles>
 __global__ __launch_bounds__(kSpanThreads, 4) void gated_spans(GatedArgs a) {
-  using S = Spans;
+  using S = Spans<kTiles>;
   __shared__ __align__(16) uint8_t lds[S::kLds];
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, h = lane >> 5;
   const int ks = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint32_t tm, tn;
-  tile_of(blockIdx.x, (a.nr + kQK - 1) / kQK, (a.nc + 31) / 32, tm, tn);
-  const uint32_t m0 = tm * kQK, n0 = tn * 32;
+  tile_of(blockIdx.x, (a.nr + S::kFeatures - 1) / S::kFeatures, (a.nc + 31) / 32, tm, tn);
+  const uint32_t m0 = tm * S::kFeatures, n0 = tn * 32;
   // The thread's pieces, by 64 of one matrix: its address stays in scalar registers.  Waves that have one
   // less take the last group's again.
   struct Piece {
@@ -451,17 +454,20 @@ __global__ __launch_bounds__(kSpanThreads, 4) void gated_spans(GatedArgs a) {
     bool tokens;
   };
   const auto piece_of = [&](int j) __attribute__((always_inline)) {
-    const int g = min(j * kSpanWaves + ks, S::kGroups - 1), matrix = min(g / S::kWGroups, 2);
-    const int q = (g - matrix * S::kWGroups) * 64 + lane;
+    const int g = min(j * kSpanWaves + ks, S::kGroups - 1), tile = min(g / S::kWGroups, kTiles);
+    const int q = (g - tile * S::kWGroups) * 64 + lane;
     Piece p;
-    p.tokens = matrix == 2;
+    p.tokens = tile == kTiles;
     const int r = p.tokens ? q / (S::kYSpan / 16) : q / (S::kWSpan / 16);
     p.at = 16 * (p.tokens ? q % (S::kYSpan / 16) : q % (S::kWSpan / 16));
-    p.to = (p.tokens ? S::kYAt + r * S::kYRow : (32 * matrix + r) * S::kWRow) + p.at;
+    p.to = (p.tokens ? S::kYAt + r * S::kYRow : (32 * tile + r) * S::kWRow) + p.at;
+    // of one tile the upper half are up rows
+    const bool up = kTiles == 2 ? tile == 1 : r >= S::kFeatures;
+    const uint32_t feature = r - (kTiles == 1 && up ? S::kFeatures : 0);
     p.base = p.tokens ? a.vy + static_cast<size_t>(n0) * a.by
-                      : (matrix ? a.up : a.gate) + static_cast<size_t>(m0) * a.bx;
+                      : (up ? a.up : a.gate) + static_cast<size_t>(m0) * a.bx;
     p.row = p.tokens ? min(static_cast<uint32_t>(r), a.nc - 1 - n0) * static_cast<uint32_t>(a.by)
-                     : min(static_cast<uint32_t>(r), a.nr - 1 - m0) * static_cast<uint32_t>(a.bx);
+                     : min(feature, a.nr - 1 - m0) * static_cast<uint32_t>(a.bx);
     return p;
   };
   const uint8_t *base[S::kPieces];
@@ -505,7 +511,7 @@ __global__ __launch_bounds__(kSpanThreads, 4) void gated_spans(GatedArgs a) {
   const uint32_t m_even = h ? 0u : 0xffffu, m_odd = h ? 0xffff0000u : 0u;
   const int w_at = li * S::kWRow + ks * (2 * kQ4Bytes) + 8 * h;
   const int y_at = S::kYAt + li * S::kYRow + ks * (2 * kQ8Bytes) + 8 * h;
-  float acc[2][16] = {};
+  float acc[kTiles][16] = {};
   const auto weights = [&](uint32_t q0, uint32_t q1) __attribute__((always_inline)) {
     q0 ^= 0x88888888u;
     q1 ^= 0x88888888u;
@@ -527,13 +533,15 @@ __global__ __launch_bounds__(kSpanThreads, 4) void gated_spans(GatedArgs a) {
   };
   // the wave's pair of a chunk, or its even block alone
   const auto pair = [&](const uint8_t *stage, bool odd) __attribute__((always_inline)) {
-    const uint32_t *const x[2] = {reinterpret_cast<const uint32_t *>(stage + w_at),
-                                  reinterpret_cast<const uint32_t *>(stage + w_at + 32 * S::kWRow)};
-    const uint32_t *const y = reinterpret_cast<const uint32_t *>(stage + y_at);
-    v4i w[2];
-    uint32_t dw[2], odd_dw[2];
+    const uint32_t *x[kTiles];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kTiles; ++i)
+      x[i] = reinterpret_cast<const uint32_t *>(stage + w_at + i * 32 * S::kWRow);
+    const uint32_t *const y = reinterpret_cast<const uint32_t *>(stage + y_at);
+    v4i w[kTiles];
+    uint32_t dw[kTiles], odd_dw[kTiles];
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
       w[i] = weights(funnel16(x[i][0], x[i][1]), funnel16(x[i][1], x[i][2]));
       dw[i] = x[i][0] & m_even;
       odd_dw[i] = x[i][2] & m_odd;
@@ -542,16 +550,16 @@ __global__ __launch_bounds__(kSpanThreads, 4) void gated_spans(GatedArgs a) {
                         funnel16(y[5], y[6])};
     const uint32_t odd_dy = y[6] & m_odd;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < kTiles; ++i)
       fold(acc[i], even, w[i], y[0] & m_even, dw[i]);
     if (!odd)
       return;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < kTiles; ++i)
       w[i] = weights(x[i][5], x[i][6]);
     const u32x4 last = {y[9], y[10], y[13], y[14]};
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < kTiles; ++i)
       fold(acc[i], last, w[i], odd_dy, odd_dw[i]);
   };
   const int whole = static_cast<int>(a.nb / kSpanBlocks);
@@ -583,9 +591,9 @@ __global__ __launch_bounds__(kSpanThreads, 4) void gated_spans(GatedArgs a) {
   // the waves' sums together, kMine of a lane's each
   float *const parts = reinterpret_cast<float *>(lds);
   float *const out = reinterpret_cast<float *>(lds + S::kParts);
-  float sum[2][S::kMine];
+  float sum[kTiles][S::kMine];
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
+  for (int p = 0; p < kTiles; ++p) {
 #pragma unroll
     for (int e = 0; e < 16; ++e)
       parts[(ks * 16 + e) * 64 + lane] = acc[p][e];
@@ -603,25 +611,37 @@ __global__ __launch_bounds__(kSpanThreads, 4) void gated_spans(GatedArgs a) {
 #pragma unroll
   for (int q = 0; q < S::kMine; ++q) {
     const int e = ks * S::kMine + q;
-    out[(8 * (e >> 2) + 4 * h + (e & 3)) * S::kOutRow + li] = activation(sum[0][q], a.act) * sum[1][q];
+    float &to = out[(8 * (e >> 2) + 4 * h + (e & 3)) * S::kOutRow + li];
+    if constexpr (kTiles == 2)
+      to = activation(sum[0][q], a.act) * sum[1][q];
+    else
+      to = sum[0][q];
   }
   __syncthreads();
-  if (tid < 32 * 8) {
-    const int part = tid & 7, row = tid >> 3;
+  constexpr int kOuts = S::kFeatures / 4;  // of a token, by four
+  if (tid < 32 * kOuts) {
+    const int part = tid % kOuts, row = tid / kOuts;
     const float4 x = *reinterpret_cast<const float4 *>(out + row * S::kOutRow + 4 * part);
-    const float v[4] = {x.x, x.y, x.z, x.w};
+    float v[4] = {x.x, x.y, x.z, x.w};
+    if constexpr (kTiles == 1) {
+      const float4 u = *reinterpret_cast<const float4 *>(out + row * S::kOutRow + S::kFeatures + 4 * part);
+      const float by[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        v[k] = activation(v[k], a.act) * by[k];
+    }
     if (n0 + row < a.nc)
-      emit<T>(a, n0 + row, m0, part, v);
+      emit<T, kTiles == 2>(a, n0 + row, m0, part, v);
   }
 }
 
 size_t up_by(size_t n, size_t by) { return (n + by - 1) / by; }
 
-template <typename T> int launch_spans(const GatedArgs &a, hipStream_t st) {
-  const size_t tiles = up_by(a.nr, kQK) * up_by(a.nc, 32);
+template <typename T, int kTiles> int launch_spans(const GatedArgs &a, hipStream_t st) {
+  const size_t tiles = up_by(a.nr, Spans<kTiles>::kFeatures) * up_by(a.nc, 32);
   if (tiles > 0xffffffffu / kSpanThreads)
     return TCRV_HIP_ERR_TOO_LARGE;
-  gated_spans<T><<<dim3(static_cast<unsigned>(tiles)), dim3(kSpanThreads), 0, st>>>(a);
+  gated_spans<T, kTiles><<<dim3(static_cast<unsigned>(tiles)), dim3(kSpanThreads), 0, st>>>(a);
   return tcrv_host::launch_status();
 }
 
@@ -657,6 +677,10 @@ template <typename T> int launch_elem(const GatedArgs &a, hipStream_t st) {
     return launch_one<T, 2>(a, st);
   if (a.nc <= 4 && !a.q8 && a.nr <= 12288)
     return launch_one<T, 4>(a, st);
+  // 16 features a work-group where all of those run at once, and no block of 32 outputs is wanted: 8 tokens,
+  // 4096 features of 4096, 10.2 us against 13.5, of 14336 25 against 34; past one a CU 15.4 and 14.3 (64 tokens)
+  if (!a.q8 && up_by(a.nr, Spans<1>::kFeatures) * up_by(a.nc, 32) <= 256)
+    return launch_spans<T, 1>(a, st);
   // By what the kernels take for a block of K, in ns: rounds of 256 work-groups, one a CU, of the tiles; the
   // spans', two a CU, go on as CUs are free.  Measured at K 4096, us, spans / 64 features x 128 tokens / 128 x
   // 128: 11008 features x 33 tokens 33 / 58 / 92, 14336 x 128 69 / 62 / 95, 11008 x 200 91 / 118 / 96, 4096 x
@@ -666,7 +690,7 @@ template <typename T> int launch_elem(const GatedArgs &a, hipStream_t st) {
   const size_t mid = 460 * up_by(up_by(a.nr, 64) * up_by(a.nc, kTileTokens), 256);
   const size_t wide = 720 * up_by(up_by(a.nr, 128) * up_by(a.nc, kTileTokens), 256);
   if (spans <= wide && spans <= mid)
-    return launch_spans<T>(a, st);
+    return launch_spans<T, 2>(a, st);
   return mid <= wide ? launch_tiles<T, 2>(a, st) : launch_tiles<T, 4>(a, st);
 }
 
