@@ -177,6 +177,10 @@ class Trees(Setup):
     ([4000], [2], 4, 1, 128, 128),
     ([700], [65], 40, 1, 128, 16),
     ([5, 0, 60], [0, 0, 3], 6, 2, 128, 16),
+    # tiles of few stretches and of many, rows of heads that one work-group's groups hold side by side or not
+    ([700, 1300, 2600, 6000], [3, 1, 4, 2], 4, 1, 256, 16),
+    ([700, 1300, 2600, 5000, 90], [3, 9, 4, 2, 12], 4, 1, 64, 16),
+    ([400, 900, 1700], [5, 3, 1], 14, 2, 192, 32),
 ])
 def test_trees(hip, dev, elem, cached, nodes, heads, kv, dim, page):
     t = Trees(dev, elem, cached, nodes, heads, kv, dim, page, seed=len(cached))

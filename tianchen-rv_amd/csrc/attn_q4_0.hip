@@ -1617,15 +1617,14 @@ attn_q4_0_tiles(AttnArgs a) {
 }
 
 // The stretches of a tile of attn_q4_0_rows16 together, of the tile that one of the kernel's work-groups has
-// begun, 4 elements a thread.  A work-group takes a row, and groups of head_dim / 4 threads share out
-// its stretches; where tiles are many (kSide) the groups take rows side by side, and share out those of
-// a tile of more than kFewStretches stretches one row after the other.  The same sums in the same order: a
-// group that has one stretch leaves it as it is.  Latency bounds it, the launch and two dependent reads: of
-// 512 work-groups' tiles of 16 rows of 128, f16, 10.5 us a work-group a row and 4.6 side by side.
+// begun, 4 elements a thread, by groups of head_dim / 4 threads.  Of few stretches (as many as groups, up to 8)
+// the groups take rows of the tile side by side, and the work-groups past them none; of more a work-group
+// takes a row, and its groups share them out.  The same sums in the same order: a group that has one
+// stretch leaves it as it is.  Latency bounds it, the launch and two dependent reads: 512 work-groups'
+// tiles of 16 rows of 128, f16, 10.5 us a work-group a row and 6 side by side.
 constexpr int kJoinThreads = 256;
-constexpr uint32_t kFewStretches = 4;  // head_dim 256 has as many groups
 
-template <typename T, bool kSide>
+template <typename T>
 __global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join_few(AttnArgs a, uint32_t head_dim) {
   __shared__ f32x4 s_o[kJoinThreads];
   __shared__ float2 s_ml[kJoinThreads];
@@ -1656,15 +1655,17 @@ __global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join_few(AttnArgs a, u
                         static_cast<size_t>(head) * a.out_head + e,
                     v, a.out_vec);
   };
-  if constexpr (kSide) {
+  if (stretches <= min(groups, 8u)) {
     const uint32_t row = blockIdx.y * groups + group;
-    if (stretches <= kFewStretches) {
-      if (group >= groups || row >= kRows)
-        return;
-      float2 x[kFewStretches];
-      f32x4 v[kFewStretches];
+    if (group >= groups || row >= kRows)
+      return;
+    // up to kMost stretches, read at once
+    const auto beside = [&](auto most) __attribute__((always_inline)) {
+      constexpr uint32_t kMost = decltype(most)::value;
+      float2 x[kMost];
+      f32x4 v[kMost];
 #pragma unroll
-      for (uint32_t s = 0; s < kFewStretches; ++s) {
+      for (uint32_t s = 0; s < kMost; ++s) {
         const uint32_t from = min(s, stretches - 1);
         x[s] = ml[at(from, row)];
         v[s] = part(from, row);
@@ -1675,10 +1676,10 @@ __global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join_few(AttnArgs a, u
       float top = kNone, l = 0.0f;
       f32x4 o{};
 #pragma unroll
-      for (uint32_t s = 0; s < kFewStretches; ++s)
+      for (uint32_t s = 0; s < kMost; ++s)
         top = fmaxf(top, x[s].x);
 #pragma unroll
-      for (uint32_t s = 0; s < kFewStretches; ++s) {
+      for (uint32_t s = 0; s < kMost; ++s) {
         if (s < stretches) {
           const float f = x[s].x == top ? 1.0f : exp2_fast(x[s].x - top);
           l += x[s].y * f;
@@ -1686,50 +1687,49 @@ __global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join_few(AttnArgs a, u
         }
       }
       put(span, tile * kRows + row, o, l);
-      return;
-    }
+    };
+    if (stretches <= 4)
+      beside(std::integral_constant<uint32_t, 4>());
+    else
+      beside(std::integral_constant<uint32_t, 8>());
+    return;
   }
   const Span span(a, begun.x);
-  const uint32_t rows = kSide ? groups : 1;
-  for (uint32_t r = 0; r < rows; ++r) {
-    const uint32_t place = blockIdx.y * rows + r, row = tile * kRows + place;
-    if (place >= kRows || row >= span.rows)
-      return;
-    float m = kNone, l = 0.0f;
-    f32x4 o{};
-    if (group < groups) {
+  const uint32_t row = tile * kRows + blockIdx.y;
+  if (row >= span.rows)
+    return;
+  float m = kNone, l = 0.0f;
+  f32x4 o{};
+  if (group < groups) {
 #pragma unroll 4
-      for (uint32_t s = group; s < stretches; s += groups) {
-        // as they come: 16 bytes of output and 8 of its maximum and sum in one turn
-        const float2 x = ml[at(s, place)];
-        const f32x4 v = part(s, place);
-        const float top = fmaxf(m, x.x);
-        const float f = m == top ? 1.0f : exp2_fast(m - top), h = x.x == top ? 1.0f : exp2_fast(x.x - top);
-        l = l * f + x.y * h;
-        o = o * f + v * h;
-        m = top;
-      }
-    }
-    if (r > 0)
-      __syncthreads();
-    s_o[threadIdx.x] = o;
-    s_ml[threadIdx.x] = make_float2(m, l);
-    __syncthreads();
-    if (group == 0) {
-      float top = kNone;
-      for (uint32_t k = 0; k < groups; ++k)
-        top = fmaxf(top, s_ml[k * per_head + threadIdx.x].x);
-      o = f32x4{};
-      l = 0.0f;
-      for (uint32_t k = 0; k < groups; ++k) {
-        const float2 x = s_ml[k * per_head + threadIdx.x];
-        const float f = x.x == top ? 1.0f : exp2_fast(x.x - top);
-        l += x.y * f;
-        o += s_o[k * per_head + threadIdx.x] * f;
-      }
-      put(span, row, o, l);
+    for (uint32_t s = group; s < stretches; s += groups) {
+      // as they come: 16 bytes of output and 8 of its maximum and sum in one turn
+      const float2 x = ml[at(s, blockIdx.y)];
+      const f32x4 v = part(s, blockIdx.y);
+      const float top = fmaxf(m, x.x);
+      const float f = m == top ? 1.0f : exp2_fast(m - top), h = x.x == top ? 1.0f : exp2_fast(x.x - top);
+      l = l * f + x.y * h;
+      o = o * f + v * h;
+      m = top;
     }
   }
+  s_o[threadIdx.x] = o;
+  s_ml[threadIdx.x] = make_float2(m, l);
+  __syncthreads();
+  if (group != 0)
+    return;
+  float top = kNone;
+  for (uint32_t k = 0; k < groups; ++k)
+    top = fmaxf(top, s_ml[k * per_head + threadIdx.x].x);
+  o = f32x4{};
+  l = 0.0f;
+  for (uint32_t k = 0; k < groups; ++k) {
+    const float2 x = s_ml[k * per_head + threadIdx.x];
+    const float f = x.x == top ? 1.0f : exp2_fast(x.x - top);
+    l += x.y * f;
+    o += s_o[k * per_head + threadIdx.x] * f;
+  }
+  put(span, row, o, l);
 }
 
 // The parts of a row of attn_q4_0_tiles together, 4 elements a thread.  Of few parts a group of
@@ -2006,15 +2006,8 @@ void launch_all(AttnArgs a, Kernels k, const Plan &few, const Plan &many, size_t
     launch_rows16<NP, T, kTree>(a, head_dim, static_cast<unsigned>(few.launch), st);
     if (few.groups) {
       const size_t rows = std::min(static_cast<size_t>(a.max_added) * a.share, few.tile_rows);
-      const size_t beside = tcrv::kJoinThreads / (dim / 4);
-      // tiles of few stretches, as far as the host knows them
-      if (few.groups <= 2 * requests * few.tiles * (a.heads / a.share))
-        tcrv::attn_q4_0_join_few<T, true>
-            <<<dim3(a.groups, static_cast<unsigned>((rows + beside - 1) / beside)), join_block, 0, st>>>(
-                a, dim);
-      else
-        tcrv::attn_q4_0_join_few<T, false>
-            <<<dim3(a.groups, static_cast<unsigned>(rows)), join_block, 0, st>>>(a, dim);
+      tcrv::attn_q4_0_join_few<T>
+          <<<dim3(a.groups, static_cast<unsigned>(rows)), join_block, 0, st>>>(a, dim);
     }
   }
   if (k.many) {
