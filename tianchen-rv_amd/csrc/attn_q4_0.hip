@@ -1621,7 +1621,7 @@ attn_q4_0_tiles(AttnArgs a) {
 // the groups take rows of the tile side by side, and the work-groups past them none; of more a work-group
 // takes a row, and its groups share them out.  The same sums in the same order: a group that has one
 // stretch leaves it as it is.  Latency bounds it, the launch and two dependent reads: 512 work-groups'
-// tiles of 16 rows of 128, f16, 10.5 us a work-group a row and 6 side by side.
+// tiles of 16 rows of 128, f16, 10.5 us a work-group a row and 5 side by side.
 constexpr int kJoinThreads = 256;
 
 template <typename T>
@@ -1632,8 +1632,12 @@ __global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join_few(AttnArgs a, u
   if (begun.z == 0)
     return;
   const uint32_t stretches = begun.z - blockIdx.x + 1;
+  const uint32_t per_head = head_dim / 4;
+  const uint32_t groups = head_dim <= 64 ? 16 : head_dim <= 128 ? 8 : head_dim <= 192 ? 5 : 4;
+  const bool side = stretches <= min(groups, 8u);
+  if (side && blockIdx.y * groups >= kRows)
+    return;
   const uint32_t kv_heads = a.heads / a.share, tile = begun.y / kv_heads;
-  const uint32_t per_head = head_dim / 4, groups = kJoinThreads / per_head;
   const uint32_t e = 4 * (threadIdx.x % per_head), group = threadIdx.x / per_head;
   // the first one's part is its work-group's second, the others' their first
   const auto at = [&](uint32_t s, uint32_t row) {
@@ -1655,7 +1659,7 @@ __global__ __launch_bounds__(kJoinThreads) void attn_q4_0_join_few(AttnArgs a, u
                         static_cast<size_t>(head) * a.out_head + e,
                     v, a.out_vec);
   };
-  if (stretches <= min(groups, 8u)) {
+  if (side) {
     const uint32_t row = blockIdx.y * groups + group;
     if (group >= groups || row >= kRows)
       return;
