@@ -27,9 +27,9 @@ def norm(elem, tokens, n, pad=0):
     (("f16", 60000, 128), (3750, 256)), (("f32", 1, 256), (1, 256)), (("f16", 4096, 512), (256, 256)),
     (("f32", 4096, 257), (1024, 256)),
     # a few long rows, on as many threads as a work-group has
-    (("f32", 1, 4096), (1, 1024)), (("f16", 512, 8192), (512, 1024)), (("f32", 3, 1024), (3, 1024)),
+    (("f32", 1, 4096), (1, 1024)), (("f16", 256, 8192), (256, 1024)), (("f32", 512, 4096), (512, 1024)), (("f16", 257, 8192), (257, 256)), (("f32", 3, 1024), (3, 1024)),
     # many: four, or one, a work-group
-    (("f16", 513, 1024), (129, 256)), (("f32", 4096, 1024), (1024, 256)), (("f16", 4096, 4096), (4096, 256)),
+    (("f16", 257, 1024), (65, 256)), (("f32", 4096, 1024), (1024, 256)), (("f16", 4096, 4096), (4096, 256)),
     (("f32", 4096, 4096), (4096, 256)), (("f32", 4096, 4100), (4096, 1024)),
     # past a row's registers
     (("f32", 2, 16388), (2, 1024)), (("f16", 1000, 40000), (1000, 1024)),

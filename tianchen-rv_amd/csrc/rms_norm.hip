@@ -235,11 +235,11 @@ void launch(const NormArgs &a, hipStream_t st) {
 
 // Threads of a row by its length, so that they have work and the row stays in registers.  16 for the short
 // rows of heads: 60000 rows of 128 f16 into Q8_0 take 16 us, 65 us with a wave a row.  1024 for a few long
-// rows, whose latency counts: one of 4096 f32 takes 2.6 us, 3.6 us with 256; of 600 rows of 4096 f16 the
-// fewer threads take 8.1 us and 1024 take 9.5 us.
-constexpr uint32_t kFewTokens = 512;
-
+// rows, whose latency counts: one of 4096 f32 takes 2.6 us, 3.6 us with 256.  Into Q8_0, us, fewer threads /
+// 1024: rows of 4096 f16, 64 4.0 / 3.7, 256 5.5 / 5.0, 384 6.2 / 6.8; f32, 64 6.2 / 4.0, 512 10.4 / 9.3; of 1024
+// f32, 512 6.4 / 5.4, 768 6.5 / 6.9.
 template <typename T, int kV, bool kVec> void launch_size(const NormArgs &a, hipStream_t st) {
+  constexpr uint32_t kFewTokens = kV == 8 ? 256 : 512;
   const uint32_t groups = (a.n + kV - 1) / kV;
   if (groups <= 16)
     launch<T, 16, 16, 1, kV, kVec>(a, st);
