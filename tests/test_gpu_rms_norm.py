@@ -115,6 +115,30 @@ def test_in_place(hip, dev, elem, n):
         assert np.array_equal(wide(out), kv_plain.round_to(y, elem))
 
 
+@pytest.mark.parametrize("off", [0, 2, 8])
+@pytest.mark.parametrize("elem,n,row8", [
+    ("f32", 32, 48), ("f32", 33, 48), ("f32", 64, 80), ("f32", 64, 96), ("f32", 64, 72), ("f32", 62, 48),
+    ("f16", 128, 144), ("bf16", 128, 160), ("f16", 128, 152), ("f16", 124, 112), ("bf16", 64, 80),
+    ("f32", 192, 208), ("f16", 512, 560),
+])
+def test_blocks_of_short_rows_at_other_strides(hip, dev, elem, n, row8, off):
+    """Rows of heads, sixteen a work-group, whose blocks begin at places of 16 and 8 bytes and others that are
+    not those of dense rows; what lies between them stays."""
+    tokens, nb = 37, n // 32
+    rng = np.random.default_rng(n + row8)
+    x = kv_plain.round_to(rng.standard_normal((tokens, n)), elem)
+    want = synth.quantize_q8_0(plain(x, None, None)[1][:, :nb * 32]).reshape(tokens, nb * 34)
+    q8 = torch.full((off + tokens * row8 + 32,), 0xEE, dtype=torch.uint8, device=dev)
+    assert q8.data_ptr() % 16 == 0
+    hip.add_rms_norm(elem, dev_rows(x, elem, dev), n, None, 0, None, 0, None, EPS, None, 0, q8[off:], row8,
+                     tokens, n)
+    got = from_dev(q8)
+    rows = got[off:off + tokens * row8].reshape(tokens, row8)
+    assert np.array_equal(rows[:, :nb * 34], want)
+    assert (rows[:, nb * 34:] == 0xEE).all() and (got[:off] == 0xEE).all()
+    assert (got[off + tokens * row8:] == 0xEE).all()
+
+
 def test_values_at_the_ends(hip, dev):
     """Rows of zeros (with and without eps), of values whose squares leave float32 both ways, and rows
     that hold an infinity or a NaN: those alone are lost."""

@@ -82,7 +82,10 @@ __global__ __launch_bounds__(kThreads *kRows) void add_rms_norm_rows(NormArgs a)
   constexpr int kWaves = kThreads > 64 ? kThreads / 64 : 1, kHeld = kPer ? kPer : 1;
   constexpr int kStaged = kThreads * kV / kQK * kQ8Bytes;  // bytes of a round of groups
   __shared__ double s_sum[kRows][kWaves];
-  __shared__ __align__(16) uint8_t s_q8[kRows][kHeld * kStaged];
+  // each row's begin at a 16-byte place, also where the caller's rows have others than these
+  constexpr int kQ8Row = (kHeld * kStaged + 15) & -16;
+  static_assert(kQ8Row % 16 == 0, "copy_lds_to_span reads from 16-byte places");
+  __shared__ __align__(16) uint8_t s_q8[kRows][kQ8Row];
   const int t = threadIdx.x % kThreads, r = threadIdx.x / kThreads;
   const uint32_t row = (blockIdx.y * gridDim.x + blockIdx.x) * kRows + r;
   const uint32_t token = min(row, a.tokens - 1);
