@@ -263,6 +263,27 @@ def test_what_a_row_does_not_see(hip, dev, elem):
             else np.abs(got[20:] - want[20:]) <= t.tolerance(want)).all()
 
 
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("cached,nodes,share", [([-10, 47], [30, 3], 2), ([-80, -1], [130, 5], 4)])
+def test_windows_wider_than_all_positions(hip, dev, elem, cached, nodes, share):
+    """They hide nothing, also where a request has fewer tokens than nodes, the first of which lie before
+    token 0 then and are not there."""
+    t = Trees(dev, elem, cached, nodes, 2 * share, 2, 64, 16, seed=14, chain=0.8)
+    whole = wide(t.run(hip))
+    for window in (2 ** 30, 2 ** 31 - 20, 2 ** 31 - 2, 2 ** 31 - 1, 2 ** 32 + 1):
+        assert np.array_equal(wide(t.run(hip, window=window)), whole), window
+    want = np.zeros_like(whole, dtype=np.float64)
+    for r, tree in enumerate(t.trees):
+        for i, sees in enumerate(bits_of(tree)[0]):
+            seen = list(range(cached[r])) + [cached[r] + j for j in np.flatnonzero(sees)]
+            seen = [x for x in seen if x >= 0]
+            for h in range(t.heads if seen else 0):
+                z = 0.125 * (t.k[r][seen, h // share] @ t.q[t.first[r] + i, h].astype(np.float64))
+                w = np.exp(z - z.max())
+                want[t.first[r] + i, h] = w @ t.v[r][seen, h // share] / w.sum()
+    assert (np.abs(whole - want) <= t.tolerance(want)).all() and (whole != 0).any()
+
+
 def test_bounds_rows_past_the_last_and_strides(hip, dev):
     t = Trees(dev, "f16", [50, 90], [5, 7], 4, 2, 64, 16, seed=9)
     want = wide(t.run(hip))

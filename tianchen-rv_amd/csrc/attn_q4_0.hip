@@ -599,8 +599,9 @@ struct Branch {
       }
       left -= n;
     }
-    // the others are cached tokens; a row without bits takes its own as one
-    lo = max(tree - static_cast<int>(min(left, a.window - 1)), 0);
+    // the others are cached tokens; a row without bits takes its own as one.  The first node may lie before
+    // token 0, from where a window near 2^31 would leave 32 bits
+    lo = max(max(tree, 0) - static_cast<int>(min(left, a.window - 1)), 0);
   }
   // which of tokens t .. t + 31 are cached ones or have their bits set
   __device__ uint32_t sees32(const AttnArgs &a, int t) const {
