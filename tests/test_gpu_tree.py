@@ -189,6 +189,31 @@ def test_trees(hip, dev, elem, cached, nodes, heads, kv, dim, page):
         t.check(hip, window=window)
 
 
+# (cached, nodes, heads, kv_heads, dim, page) whose windowed rows are shared out and joined; which kernels
+# they take is pinned by test_more_dispatch.py
+WINDOWED = [
+    # several tiles a kv head, in parts: each tile's range begins with what the first node sees
+    ([4100, 300, 2500], [200, 70, 130], 8, 2, 64, 16),
+    ([3500, 5000], [200, 3], 8, 2, 128, 32),
+    ([2900], [330], 4, 2, 192, 16),
+    ([3300], [150], 8, 2, 256, 16),
+    # up to 64 rows, in stretches
+    ([5000, 4100, 90], [16, 9, 16], 8, 2, 128, 16),
+    ([6000], [61], 2, 2, 64, 16),
+    ([3900, 800], [12, 16], 4, 1, 256, 48),
+]
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("cached,nodes,heads,kv,dim,page", WINDOWED)
+def test_windows_over_parts(hip, dev, elem, cached, nodes, heads, kv, dim, page):
+    """Long windows, whose tiles are in parts: a late node of little depth sees more of the cached tokens
+    than its number among the nodes would leave."""
+    t = Trees(dev, elem, cached, nodes, heads, kv, dim, page, seed=15)
+    for window in (700, 3000):
+        t.check(hip, window=window)
+
+
 @pytest.mark.parametrize("elem", ELEMS)
 def test_many_requests(hip, dev, elem):
     rng = np.random.default_rng(2)

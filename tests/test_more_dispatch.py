@@ -85,6 +85,24 @@ def test_kernels_of_trees(args, want):
     assert got == want
 
 
+@pytest.mark.parametrize("elem", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("window", [700, 3000])
+@pytest.mark.parametrize("cached,nodes,heads,kv,dim,want", [
+    # the sizes of test_gpu_tree.py whose tiles are in parts, which a join brings together
+    ([4100, 300, 2500], [200, 70, 130], 8, 2, 64, ["rows16", "join_few", "tiles", "join"]),
+    ([3500, 5000], [200, 3], 8, 2, 128, ["rows16", "join_few", "tiles", "join"]),
+    ([2900], [330], 4, 2, 192, ["tiles", "join"]),
+    ([3300], [150], 8, 2, 256, ["tiles", "join"]),
+    ([5000, 4100, 90], [16, 9, 16], 8, 2, 128, ["rows16", "join_few"]),
+    ([6000], [61], 2, 2, 64, ["rows16", "join_few"]),
+    ([3900, 800], [12, 16], 4, 1, 256, ["rows16", "join_few"]),
+])
+def test_windowed_trees_in_parts(elem, window, cached, nodes, heads, kv, dim, want):
+    length = max(c + n for c, n in zip(cached, nodes))
+    got = run(tree(elem, len(nodes), sum(nodes), max(nodes), length, heads, kv, dim, window))
+    assert [name.replace("attn_q4_0_", "") for name, _, _ in got] == want
+
+
 @pytest.mark.parametrize("nodes", [1, 16, 17, 200])
 @pytest.mark.parametrize("length", [210, 4000, 131072, 1 << 30])
 def test_workspace_of_trees_serves_every_window(nodes, length):
