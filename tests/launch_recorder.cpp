@@ -97,6 +97,15 @@ int hipGetSymbolAddress(void **p, const void *) {
   return 0;
 }
 
+// All kernels of the library, a line each.
+const char *recorder_kernels() {
+  static std::string out;
+  out.clear();
+  for (const auto &entry : names())
+    out += entry.second + "\n";
+  return out.c_str();
+}
+
 // The launches since the last call, a line each: name|grid x|y|z|block x|y|z.
 const char *recorder_take() {
   static std::string out;

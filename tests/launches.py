@@ -43,6 +43,15 @@ def replay(calls):
     return [(status, [Launch(*x) for x in xs]) for status, xs in json.loads(out.stdout)]
 
 
+@functools.lru_cache(None)
+def registered():
+    """The names of all kernels that the library holds."""
+    out = subprocess.run([sys.executable, os.path.abspath(__file__), _recorder()[1], "kernels"],
+                         input="[]", capture_output=True, text=True)
+    assert out.returncode == 0, out.stderr[-2000:]
+    return tuple(json.loads(out.stdout))
+
+
 def gemm_call(quant, entry, nr, nc, n, xpad=0, ypad=0, off=0):
     """The call of a GEMM over nr weight rows x nc tokens, operands `off` bytes past an aligned
     address and `xpad` / `ypad` bytes between rows.  entry: "plain", "ws", "tiles"
@@ -69,12 +78,17 @@ def kernels(calls):
     return out
 
 
-def main(recorder):
+def main(recorder, *what):
     sys.modules["torch"] = None  # the binding loads without it; no HIP runtime is initialised
     sys.path.insert(0, os.path.join(ROOT, "tianchen-rv_amd"))
     rec = ctypes.CDLL(recorder, mode=ctypes.RTLD_GLOBAL)
     rec.recorder_take.restype = ctypes.c_char_p
     import tcrv_hip
+    if what:
+        rec.recorder_kernels.restype = ctypes.c_char_p
+        tcrv_hip.load()
+        json.dump(rec.recorder_kernels().decode().splitlines(), sys.stdout)
+        return
     out = []
     for name, args in json.load(sys.stdin):
         status = tcrv_hip.call(name, *args, 0, check=False)
@@ -86,4 +100,4 @@ def main(recorder):
 
 
 if __name__ == "__main__":
-    main(sys.argv[1])
+    main(*sys.argv[1:])

@@ -115,3 +115,28 @@ def test_workspace_of_trees_serves_every_window(nodes, length):
             name, args = tree("f16", requests, tokens, nodes, length, heads, kv, dim, window)
             calls.append((name, args[:-1] + (need,)))
         assert all(status == 0 for status, _ in launches.replay(calls))
+
+
+def test_every_kernel_is_reached():
+    """No instantiation that no call launches."""
+    calls = []
+    for elem in ("f32", "f16", "bf16"):
+        for tokens in (1, 2, 4, 5, 128, 2048):
+            for n, wide, q8 in ((32, 4096, False), (32, 4096, True), (4096, 4096, False),
+                                (4096, 14336, True)):
+                calls.append(gated(tokens, n, wide, q8, elem))
+        for tokens in (3, 2000):
+            # whole groups of 8 and of 4 values, and others
+            for n in (64, 256, 512, 1024, 2048, 4096, 8192, 16384, 32768, 65536):
+                calls += [norm(elem, tokens, n + more) for more in (0, -4, -1)]
+        for dim in (64, 128, 192, 256):
+            for nodes in (4, 200):
+                calls.append(tree(elem, 2, 2 * nodes, nodes, 6000, 8, 1, dim))
+    calls += [("tcrv_hip_tree_tables", (A, B, C, 4, D, 2, E, 100)),
+              ("tcrv_hip_kv_keep_q4_0", (A, 64, 16, B, 8, C, D, E, 10, F, 3, 10, 8, 128))]
+    made = {x.name for _, xs in launches.replay(calls) for x in xs}
+    # names with _Float16 among their arguments stay as the compiler writes them
+    mine = (r"add_rms_norm_rows|gated_(one|spans|tiles)|tree_tables|kv_keep_q4_0"
+            r"|attn_q4_0_(rows16|tiles)(<.*true>|I.*Lb1E)")
+    held = {name for name in launches.registered() if re.search(mine, name)}
+    assert len(held) > 100 and not held - made, sorted(held - made)

@@ -654,16 +654,13 @@ template <typename T, int kFT> int launch_tiles(const GatedArgs &a, hipStream_t 
   return tcrv_host::launch_status();
 }
 
-template <typename T, int kTokens> int launch_one(const GatedArgs &a, hipStream_t st) {
-  const bool pairs = a.nb > 1;
-  const dim3 grid(static_cast<unsigned>(up_by(a.nr, a.q8 ? kQK : one_waves(false))));
-  const dim3 block(one_waves(a.q8 != nullptr) * 64);
-  if (a.q8)
-    pairs ? gated_one<T, kTokens, true, true><<<grid, block, 0, st>>>(a)
-          : gated_one<T, kTokens, false, true><<<grid, block, 0, st>>>(a);
+template <typename T, int kTokens, bool kBlocks> int launch_one(const GatedArgs &a, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(up_by(a.nr, kBlocks ? kQK : one_waves(false))));
+  const dim3 block(one_waves(kBlocks) * 64);
+  if (a.nb > 1)
+    gated_one<T, kTokens, true, kBlocks><<<grid, block, 0, st>>>(a);
   else
-    pairs ? gated_one<T, kTokens, true, false><<<grid, block, 0, st>>>(a)
-          : gated_one<T, kTokens, false, false><<<grid, block, 0, st>>>(a);
+    gated_one<T, kTokens, false, kBlocks><<<grid, block, 0, st>>>(a);
   return tcrv_host::launch_status();
 }
 
@@ -672,11 +669,11 @@ template <typename T> int launch_elem(const GatedArgs &a, hipStream_t st) {
   // gated_one / gated_spans: 2 tokens, 4096 features 6.8 / 13.5, 11008 13 / 21, 14336 16 / 23 and into Q8_0 20 / 23;
   // 4 tokens, 4096 9.5 / 13.5, 11008 19 / 21, 14336 24 / 23, into Q8_0 4096 15.1 / 13.7.
   if (a.nc == 1)
-    return launch_one<T, 1>(a, st);
+    return a.q8 ? launch_one<T, 1, true>(a, st) : launch_one<T, 1, false>(a, st);
   if (a.nc == 2)
-    return launch_one<T, 2>(a, st);
+    return a.q8 ? launch_one<T, 2, true>(a, st) : launch_one<T, 2, false>(a, st);
   if (a.nc <= 4 && !a.q8 && a.nr <= 12288)
-    return launch_one<T, 4>(a, st);
+    return launch_one<T, 4, false>(a, st);
   // 16 features a work-group where all of those run at once, and no block of 32 outputs is wanted: 8 tokens,
   // 4096 features of 4096, 10.2 us against 13.5, of 14336 25 against 34; past one a CU 15.4 and 14.3 (64 tokens)
   if (!a.q8 && up_by(a.nr, Spans<1>::kFeatures) * up_by(a.nc, 32) <= 256)
