@@ -589,8 +589,8 @@ TCRV_HIP_API int tcrv_hip_add_rms_norm(int elem, const void *x, size_t x_token,
  * the sizes and which outputs are asked for (not the one order of the GEMM); the same
  * call gives the same bits.  An
  * output whose rows hold a scale that is not finite is NaN or infinite.
- * nr up to 2^26 - 4, rows and strides bx and by up to 2^26 bytes, else
- * TCRV_HIP_ERR_TOO_LARGE. */
+ * nr up to 2^26 - 4, rows and strides bx and by up to 2^26 bytes, and of tiles of
+ * 128 features x 128 tokens less than 2^23 in all, else TCRV_HIP_ERR_TOO_LARGE. */
 enum {
   TCRV_HIP_ACT_SILU = 0,
   TCRV_HIP_ACT_GELU_TANH = 1,

@@ -131,6 +131,22 @@ def test_floats_reach_the_library():
     assert tcrv_hip.SIGNATURES["tcrv_hip_attn_tree_q4_0"][20] is ctypes.c_float
 
 
+@pytest.mark.parametrize("nr,nc,want", [
+    (14336, (1 << 24) - 1, LARGE), (8064, (1 << 24) - 1, OK), (8065, (1 << 24) - 1, LARGE),
+    (1 << 14, ((1 << 23) - 1) // 128 * 128, OK), (1 << 14, (1 << 23) - 127, LARGE), (0x3fffffc, 1920, OK),
+    (0x3fffffc, 2049, LARGE), (0x3fffffc, 64, OK), (192, (1 << 24) - 1, OK), (129, (1 << 24) - 1, OK),
+    (96, (1 << 24) - 1, OK),
+])
+@pytest.mark.parametrize("q8", [False, True])
+def test_gated_tiles_that_a_launch_holds(nr, nc, want, q8):
+    """Less than 2^23 tiles of 128 x 128, whichever kernel serves the call."""
+    assert (-(-nr // 128) * -(-nc // 128) < 1 << 23) == (want == OK)
+    (got, made), = launches.replay([("tcrv_hip_gated_q4_0_q8_0", (
+        9, 0, 64, P, nr, Q if q8 else 0, nr // 32 * 34, R, S, 36, T, 68, nr, nc))])
+    assert got == want and bool(made) == (want == OK)
+    assert all(g * b < 1 << 32 for x in made for g, b in zip(x.grid, x.block))
+
+
 MOST = (1 << 24) - 1
 P, Q, R, S, T, U, V, W = ((i + 1) << 50 for i in range(8))
 
