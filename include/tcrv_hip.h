@@ -566,8 +566,10 @@ TCRV_HIP_API int tcrv_hip_attn_q4_0(int elem, const void *q, size_t q_token, siz
  * sum), and as the Q8_0 blocks that tcrv_hip_quantize_row_q8_0 makes of it (q8; NULL:
  * not written; a partial last block is not written).  weight: n floats (NULL: ones).
  * h is the f32 sum, not rounded to `elem` first; squares, their mean and its root
- * are computed in f64: c, and with it every quant, does not depend on an order.
- * eps >= 0 and finite, else TCRV_HIP_ERR_BAD_SIZE. */
+ * are computed in f64: c, and with it every quant, is the same in any order of the
+ * sum, but for a row in tens of millions whose c lies within 2^-50 of a border
+ * between two floats.  eps >= 0 and finite, else TCRV_HIP_ERR_BAD_SIZE; n less than
+ * 2^31, else TCRV_HIP_ERR_TOO_LARGE. */
 TCRV_HIP_API int tcrv_hip_add_rms_norm(int elem, const void *x, size_t x_token,
                                        const void *residual, size_t residual_token, void *sum,
                                        size_t sum_token, const float *weight, double eps, void *y,
@@ -653,7 +655,8 @@ TCRV_HIP_API int tcrv_hip_attn_tree_q4_0(int elem, const void *q, size_t q_token
  * ascend; of one that does not, what the nodes' places hold is unspecified.  Nodes
  * that the request does not have are skipped, as are places without a page.
  * count[r] is cut to path_stride, and to the request's nodes; at most max_added
- * nodes of a request are looked at.  The pages past the kept tokens are free again. */
+ * nodes of a request are looked at.  A request's path is a row of path_stride
+ * numbers, all of which may be read.  The pages past the kept tokens are free again. */
 TCRV_HIP_API int tcrv_hip_kv_keep_q4_0(uint8_t *cache, size_t pages, size_t page_size,
                                        const int32_t *block_table, size_t table_stride,
                                        const int32_t *first, const int32_t *length,

@@ -4,7 +4,7 @@
 // A row's values stay in registers between the sum of their squares and their scaling, so that it is
 // read once; rows past what registers hold are read twice.  Squares are summed in f64: exact products
 // and sums off by some 2^-50 of theirs, so that c = 1 / sqrt(mean + eps) rounds to the same f32 for all
-// but one row in millions, however its work is laid out.
+// but one row in tens of millions, however its work is laid out.
 //
 // Memory bounds it for many rows, what it reads and writes once: 4096 rows of 4096 with residual and sum
 // into elements take 54 us in f32 (5.0 TB/s, a large copy's rate) and 30 us in f16 (4.5 TB/s), into Q8_0
