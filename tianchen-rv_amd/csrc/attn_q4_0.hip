@@ -1922,7 +1922,8 @@ Plan many_plan(int elem, size_t requests, size_t tokens, size_t max_added, size_
     const size_t most = std::max((seen + kLeastPart - 1) / kLeastPart, size_t{1});
     return std::min(std::min(std::max(kMostParts / groups, size_t{1}), most), size_t{64});
   };
-  // what a tile sees begins at a multiple of 32; `window` is 0 where it does not bound that
+  // what a tile sees begins at a multiple of 32; `window` is 0 where it does not bound that.  A tree's tile also
+  // sees from its request's first node's window on: its parts, no more than these, are longer then
   size_t seen = max_length + 31;
   if (window && window < seen)
     seen = std::min(seen, window + p.tile_rows / share + 34);

@@ -237,8 +237,8 @@ __global__ __launch_bounds__(one_waves(kBlocks) * 64) void gated_one(GatedArgs a
 // M = 1.5 2^23: read as floats its results are M + sum exactly (|sum| <= 16 32 8 128 < 2^22), and fma(M + sum,
 // d, -M d) is the scaled sum, rounded once.
 //
-// VALU issue bounds it, the scaling of a block's sums and the decode: 2 x 14336 features of 4096, 2048 tokens, 640 us
-// (0.75 POP/s) where tiles whose blocks several waves shared out took 1488.  Rows in LDS are padded; swizzled ones
+// VALU issue bounds it, 77 % of the SIMDs' cycles, 60 % the two instructions that scale and add a block's sum: 2 x 14336
+// features of 4096, 2048 tokens, 637 us (0.76 POP/s) where tiles whose blocks several waves shared out took 1488.  Rows in LDS are padded; swizzled ones
 // took longer, and so did two chunks under way by hand (828 us).
 // ---------------------------------------------------------------------------
 constexpr int kTileThreads = 512, kTileTokens = 128;
@@ -681,7 +681,9 @@ template <typename T> int launch_elem(const GatedArgs &a, hipStream_t st) {
   // By what the kernels take for a block of K, in ns: rounds of 256 work-groups, one a CU, of the tiles; the
   // spans', two a CU, go on as CUs are free.  Measured at K 4096, us, spans / 64 features x 128 tokens / 128 x
   // 128: 11008 features x 33 tokens 33 / 58 / 92, 14336 x 128 69 / 62 / 95, 11008 x 200 91 / 118 / 96, 4096 x
-  // 512 72 / 61 / 93, 14336 x 512 265 / 229 / 187, 2048 960 / 780 / 640.
+  // 512 72 / 61 / 93, 14336 x 512 265 / 229 / 187, 2048 960 / 780 / 640.  At K 1024 and 14336 what is taken is at most
+  // 13 % over the best kernel (11008 x 200 of 14336 292 for 259), but for 3 and 4 tokens above at K 1024 (4096 features
+  // 7.2 where 16 features a work-group take 5.2).
   const size_t groups = up_by(a.nr, kQK) * up_by(a.nc, 32);
   const size_t spans = groups <= 256 ? 100 : groups * 3 / 10;
   const size_t mid = 460 * up_by(up_by(a.nr, 64) * up_by(a.nc, kTileTokens), 256);
