@@ -238,8 +238,8 @@ __global__ __launch_bounds__(one_waves(kBlocks) * 64) void gated_one(GatedArgs a
 // d, -M d) is the scaled sum, rounded once.
 //
 // VALU issue bounds it, 77 % of the SIMDs' cycles, 60 % the two instructions that scale and add a block's sum:
-// 2 x 14336 features of 4096, 2048 tokens, 637 us (0.76 POP/s) where tiles whose blocks several waves shared out took 1488.
-// Rows in LDS are padded; swizzled ones took longer, and so did two chunks under way by hand (828 us).
+// 2 x 14336 features of 4096, 2048 tokens, 637 us (0.76 POP/s) where tiles whose blocks several waves shared out took
+// 1488.  Rows in LDS are padded; swizzled ones took longer, and so did two chunks under way by hand (828 us).
 // ---------------------------------------------------------------------------
 constexpr int kTileThreads = 512, kTileTokens = 128;
 
